@@ -392,6 +392,200 @@ int fth_b200_silu_mul(int32_t dtype, const void* gate, const void* up, void* out
                       fth_b200_stream_t stream);
 
 /* -------------------------------------------------------------------------------------------------
+ * Between the q / k / v projections and the o projection: rotary positions, a paged key / value cache held in 4 bits,
+ * the tables that address it, and the attention that reads it.  No counterpart in the reference's FP8 / INT8 path.  All
+ * are launched as programmatic dependents of the kernel in front; none allocates, synchronises or reads back, and every
+ * length that changes from step to step is read on the device, so a captured step can be replayed with other lengths.
+ * All pointers are device pointers unless a comment says "host".  Strides count elements.
+ *
+ * Rotary positions.  Pair i of a head (elements i and i + rotary_dim / 2, or 2i and 2i + 1) is turned by
+ * positions[t] * turns[i] full turns:
+ *   c = amplitude * cos, s = amplitude * sin;  y1 = x1 * c - x2 * s;  y2 = x2 * c + x1 * s
+ * The angle is reduced in 64 bits, so far positions keep their accuracy; the rest is FP32 with one rounding to the output.
+ * Elements from rotary_dim on are copied.  A row whose position is negative is not touched.  An output may be its own
+ * input (same pointer and stride); other overlaps are not allowed.  tokens = 0 does nothing.
+ * fth_b200_rope_turns fills the table on the HOST: base^(-2i / rotary_dim) / (2 pi), for longer contexts changed by
+ *   LINEAR  divided by `factor`
+ *   NTK     base raised to base * factor^(rotary_dim / (rotary_dim - 2))
+ *   YARN    divided by `factor` on a linear ramp over i between the pairs that make `fast` and `slow` turns within
+ *           `original` positions; amplitude 1 + ln(factor) / 10
+ *   BANDED  by the turns a pair makes within `original` positions: `fast` or more unchanged, `slow` or fewer divided by
+ *           `factor`, a linear blend between
+ * ------------------------------------------------------------------------------------------------- */
+enum { FTH_B200_ROPE_HALF = 0, FTH_B200_ROPE_INTERLEAVED = 1 };
+enum { FTH_B200_ROPE_SCALE_NONE = 0, FTH_B200_ROPE_SCALE_LINEAR = 1, FTH_B200_ROPE_SCALE_NTK = 2, FTH_B200_ROPE_SCALE_YARN = 3,
+       FTH_B200_ROPE_SCALE_BANDED = 4 };
+typedef struct {
+    int32_t rotary_dim;
+    int32_t scaling;   /* FTH_B200_ROPE_SCALE_* */
+    double base;
+    double factor;     /* >= 1; ignored without scaling */
+    double original;   /* YARN, BANDED: positions the model was made for */
+    double fast, slow; /* YARN, BANDED: turns, fast > slow > 0 */
+} fth_b200_rope_scaling;
+/* turns: host, rotary_dim / 2 doubles; amplitude: host, one float. */
+int fth_b200_rope_turns(const fth_b200_rope_scaling* scaling, double* turns, float* amplitude);
+typedef struct {
+    int32_t dtype;      /* FP32, FP16 or BF16: inputs and outputs */
+    int32_t layout;     /* FTH_B200_ROPE_* */
+    int64_t tokens;
+    int32_t head_dim;
+    int32_t rotary_dim; /* even, <= head_dim, <= 512 */
+    int32_t q_heads;    /* 0: no q */
+    int32_t k_heads;    /* 0: no k */
+    const void* q;      /* [tokens, q_heads, head_dim], heads head_dim apart; row stride ldq (0: dense) */
+    void* q_out;
+    const void* k;
+    void* k_out;
+    int64_t ldq, ldq_out, ldk, ldk_out;
+    const int32_t* positions; /* [tokens] */
+    const double* turns;      /* [rotary_dim / 2] */
+    float amplitude;
+} fth_b200_rope_desc;
+int fth_b200_rope(const fth_b200_rope_desc* desc, fth_b200_stream_t stream);
+
+/* One layer's cache: `blocks` blocks of `block_size` tokens.  A token's vector of one head is 4-bit codes with a BF16
+ * scale and minimum of its own: value = minimum + scale * code.
+ *   k_codes  [blocks][kv_heads][block_size][head_dim / 2] bytes; byte j holds elements 2j (low four bits) and 2j + 1
+ *   v_codes  [blocks][kv_heads][block_size / 2][head_dim / 4][2][2] bytes: two tokens share a row of 32-bit words, each
+ *            word four elements of the even token in its low half and the same four of the odd token in its high half
+ *            (what a matrix instruction wants of V, where tokens are summed over, without a shuffle)
+ *   k_params, v_params  [blocks][kv_heads][block_size] words: scale in the low half, minimum in the high half
+ * Storing x: minimum = largest BF16 <= min(x); scale = smallest BF16 >= (max(x) - minimum) / 15, at least 2^-126 unless the
+ * difference is zero; code = (x - minimum) / scale rounded to nearest, ties to even (decided in 64 bits).  A vector that
+ * holds a NaN or an infinity (or whose minimum leaves BF16 or range leaves FP32) is stored with scale NaN: whatever
+ * attends to it is NaN.
+ * A slot is block * block_size + offset. */
+typedef struct {
+    void* k_codes; /* 16-byte aligned */
+    void* v_codes; /* 16-byte aligned */
+    void* k_params;
+    void* v_params;
+    int64_t blocks;     /* blocks * block_size < 2^31 */
+    int32_t block_size; /* 16, 32, 64, 128 or 256 */
+    int32_t kv_heads;
+    int32_t head_dim;   /* 64, 128 or 256 */
+} fth_b200_kv4_cache;
+
+/* Tables of one step.  Request r holds cached_lens[r] tokens and appends new_lens[r] (0: idle).  The blocks it lacks are
+ * taken from the stack free_blocks[0 .. free_count): requests in order, blocks in order, the j-th block of the step is
+ * free_blocks[free_count - 1 - j].  Written: the new entries of block_table, total_lens = cached + new, query_start (row of
+ * each request's first token; [requests] is the number of rows), and per row the position within its request and the slot;
+ * -1 in rows behind the last.  A row whose table entry is no block gets slot -1.
+ * A step that does not fit is refused as a whole, on the device: status[0] = FTH_B200_KV4_*, nothing is taken, total_lens =
+ * cached_lens (0 where that is negative), query_start all 0, slots and positions all -1.
+ * In place: total_lens may be cached_lens, free_count_out may be free_count.  status: two words, zero-filled once. */
+enum { FTH_B200_KV4_OK = 0, FTH_B200_KV4_NO_BLOCKS = 1, FTH_B200_KV4_TABLE_FULL = 2, FTH_B200_KV4_TOO_MANY_TOKENS = 3, FTH_B200_KV4_BAD_LENGTH = 4 };
+typedef struct {
+    int32_t requests;
+    int32_t max_blocks;   /* row length of block_table */
+    int32_t block_size;   /* as in the cache */
+    int64_t blocks;       /* as in the cache; room of free_blocks */
+    int64_t tokens;       /* rows of slots and positions */
+    const int32_t* cached_lens;
+    const int32_t* new_lens;
+    const int32_t* free_blocks;
+    const int32_t* free_count;
+    int32_t* free_count_out;
+    int32_t* block_table; /* [requests, max_blocks] */
+    int32_t* total_lens;  /* [requests] */
+    int32_t* query_start; /* [requests + 1] */
+    int32_t* slots;
+    int32_t* positions;
+    int32_t* status;      /* [0]: result; [1]: used by the kernel, left at zero */
+} fth_b200_kv4_assign_desc;
+int fth_b200_kv4_assign(const fth_b200_kv4_assign_desc* desc, fth_b200_stream_t stream);
+
+/* Gives blocks back: request r shrinks from lens[r] to keep_lens[r] tokens (0: done; less than lens: rejected drafts).
+ * Blocks that hold none of the kept tokens go on the stack so that releasing what the last fth_b200_kv4_assign took
+ * restores it.  block_table is only read; lens_out (may be lens) = keep_lens.  Refused as a whole with BAD_LENGTH (negative,
+ * or keep > lens), TABLE_FULL (lens beyond the row) or NO_BLOCKS (more free blocks than there are); lens_out = lens then. */
+typedef struct {
+    int32_t requests;
+    int32_t max_blocks;
+    int32_t block_size;
+    int64_t blocks;
+    const int32_t* lens;
+    const int32_t* keep_lens;
+    int32_t* free_blocks;
+    const int32_t* free_count;
+    int32_t* free_count_out;
+    const int32_t* block_table;
+    int32_t* lens_out;
+    int32_t* status;
+} fth_b200_kv4_release_desc;
+int fth_b200_kv4_release(const fth_b200_kv4_release_desc* desc, fth_b200_stream_t stream);
+
+/* Stores k and v [tokens, kv_heads, head_dim] (heads head_dim apart, row strides ldk / ldv, 0: dense) at slots[t].  A
+ * negative slot skips the row; a slot beyond the cache skips it and is reported through fth_b200_device_status (site 40).
+ * The slots of one call differ from each other.  With `rope` (its k_heads = kv_heads, k = this k, same tokens, dtype and
+ * head_dim; k_out must be null; q optional) keys are turned before they are stored and q in the same launch; the cache
+ * and q_out receive the bytes of fth_b200_rope followed by fth_b200_kv4_append. */
+typedef struct {
+    fth_b200_kv4_cache cache;
+    int32_t dtype; /* FP32, FP16 or BF16 */
+    int64_t tokens;
+    const void* k;
+    const void* v;
+    int64_t ldk, ldv;
+    const int32_t* slots;
+    const fth_b200_rope_desc* rope; /* host, or null */
+} fth_b200_kv4_append_desc;
+int fth_b200_kv4_append(const fth_b200_kv4_append_desc* desc, fth_b200_stream_t stream);
+/* Reads slots back as values, rounded once to dtype: k_out, v_out [tokens, kv_heads, head_dim], row strides ldk / ldv;
+ * either may be null.  Rows with a negative slot (or one beyond the cache, reported as site 41) are left as they were. */
+typedef struct {
+    fth_b200_kv4_cache cache;
+    int32_t dtype;
+    int64_t tokens;
+    const int32_t* slots;
+    void* k_out;
+    void* v_out;
+    int64_t ldk, ldv;
+} fth_b200_kv4_gather_desc;
+int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* desc, fth_b200_stream_t stream);
+
+/* Attention of the step's rows over the cache.  Request r has the rows query_start[r] .. query_start[r + 1] (null: one row
+ * each, row r), its last tokens: row i of n sits at position p = total_lens[r] - n + i and sees the tokens 0 .. p (all of
+ * total_lens[r] without `causal`), of those the last `window` (window > 0; counted from p).  kv_heads divides q_heads;
+ * q head h reads kv head h / (q_heads / kv_heads).
+ *   out = softmax(scale * q . K) . V,  lse (optional, FP32 [tokens, q_heads]) = ln(sum(exp(scale * q . K)))
+ * A row that sees nothing gets zeros and lse = -infinity.  Rows behind query_start[requests] are left as they were.
+ * Scores, softmax statistics and sums are FP32.  q enters exactly (FP16 with a power of two per row; |q| < 2^100), codes
+ * are exact; a probability times the scale of its value is rounded to FP16 (11 bits, down to 2^-20 of the largest scale
+ * among the values seen).
+ * A block number outside the cache hides its tokens and is reported through fth_b200_device_status (site 42).
+ * max_query bounds the rows of a request (host-known; rows beyond it are not computed), max_blocks * block_size the tokens.
+ * The result does not depend on what else is in the batch only up to FP32 summation order; it is the same from run to run.
+ * workspace: device, 256-byte aligned, zero-filled once after allocation, left ready for the next call; calls that share
+ * one must not overlap.  fth_b200_kv4_attention_workspace_bytes depends on requests, tokens, max_query, heads and the
+ * cache's geometry only. */
+typedef struct {
+    fth_b200_kv4_cache cache;
+    int32_t dtype;       /* FP16 or BF16: q and out */
+    int32_t requests;
+    int64_t tokens;      /* rows of q and out that may be read and written */
+    int32_t q_heads;
+    int32_t max_blocks;
+    int32_t max_query;
+    int32_t causal;
+    int32_t window;      /* 0: none */
+    float scale;
+    const void* q;       /* [tokens, q_heads, head_dim], row stride ldq (0: dense) */
+    void* out;
+    int64_t ldq, ldo;
+    float* lse;
+    const int32_t* block_table; /* [requests, max_blocks] */
+    const int32_t* total_lens;
+    const int32_t* query_start; /* [requests + 1] or null */
+    void* workspace;
+    size_t workspace_bytes;
+} fth_b200_kv4_attention_desc;
+int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* desc, fth_b200_stream_t stream);
+int fth_b200_kv4_attention_supported(const fth_b200_kv4_attention_desc* desc);
+size_t fth_b200_kv4_attention_workspace_bytes(const fth_b200_kv4_attention_desc* desc);
+
+/* -------------------------------------------------------------------------------------------------
  * Host-buffer plans: the shape of KernelBase::Prepare() / compute() (include/core/kernel.h:162-163) for a
  * linear node whose weight is immutable.  create() uploads weight, scales and bias once (it allocates and
  * synchronises — never call it during capture); run() copies the activation from host memory, launches,

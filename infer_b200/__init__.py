@@ -37,8 +37,13 @@ EXPORTS = [
     "fth_b200_peer_buffer_create", "fth_b200_peer_buffer_open", "fth_b200_peer_buffer_close", "fth_b200_peer_buffer_destroy",
     "fth_b200_gather_sync", "fth_b200_gather_wait", "fth_b200_fp8_linear_argmax",
     "fth_b200_fp8_lm_head_argmax", "fth_b200_fp8_linear_fused", "fth_b200_fp8_linear_fused_supported", "fth_b200_qwen_rms_norm", "fth_b200_binary", "fth_b200_silu", "fth_b200_silu_mul",
+    "fth_b200_rope_turns", "fth_b200_rope", "fth_b200_kv4_assign", "fth_b200_kv4_release", "fth_b200_kv4_append", "fth_b200_kv4_gather",
+    "fth_b200_kv4_attention", "fth_b200_kv4_attention_supported", "fth_b200_kv4_attention_workspace_bytes",
 ]
 BINARY_ADD, BINARY_MUL = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "banded": 4}
+KV4_OK, KV4_NO_BLOCKS, KV4_TABLE_FULL, KV4_TOO_MANY_TOKENS, KV4_BAD_LENGTH = 0, 1, 2, 3, 4
 
 
 class Fp8LinearDesc(C.Structure):
@@ -95,6 +100,61 @@ class Int8Conv2dDesc(C.Structure):
     ]
 
 
+class RopeScaling(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double), ("factor", C.c_double), ("original", C.c_double),
+                ("fast", C.c_double), ("slow", C.c_double)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("layout", C.c_int32), ("tokens", C.c_int64), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+        ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("q", C.c_void_p), ("q_out", C.c_void_p), ("k", C.c_void_p), ("k_out", C.c_void_p),
+        ("ldq", C.c_int64), ("ldq_out", C.c_int64), ("ldk", C.c_int64), ("ldk_out", C.c_int64), ("positions", C.c_void_p),
+        ("turns", C.c_void_p), ("amplitude", C.c_float),
+    ]
+
+
+class Kv4Cache(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_params", C.c_void_p), ("v_params", C.c_void_p), ("blocks", C.c_int64),
+                ("block_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class Kv4AssignDesc(C.Structure):
+    _fields_ = [
+        ("requests", C.c_int32), ("max_blocks", C.c_int32), ("block_size", C.c_int32), ("blocks", C.c_int64), ("tokens", C.c_int64),
+        ("cached_lens", C.c_void_p), ("new_lens", C.c_void_p), ("free_blocks", C.c_void_p), ("free_count", C.c_void_p),
+        ("free_count_out", C.c_void_p), ("block_table", C.c_void_p), ("total_lens", C.c_void_p), ("query_start", C.c_void_p),
+        ("slots", C.c_void_p), ("positions", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class Kv4ReleaseDesc(C.Structure):
+    _fields_ = [
+        ("requests", C.c_int32), ("max_blocks", C.c_int32), ("block_size", C.c_int32), ("blocks", C.c_int64), ("lens", C.c_void_p),
+        ("keep_lens", C.c_void_p), ("free_blocks", C.c_void_p), ("free_count", C.c_void_p), ("free_count_out", C.c_void_p),
+        ("block_table", C.c_void_p), ("lens_out", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class Kv4AppendDesc(C.Structure):
+    _fields_ = [("cache", Kv4Cache), ("dtype", C.c_int32), ("tokens", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("ldk", C.c_int64),
+                ("ldv", C.c_int64), ("slots", C.c_void_p), ("rope", C.c_void_p)]
+
+
+class Kv4GatherDesc(C.Structure):
+    _fields_ = [("cache", Kv4Cache), ("dtype", C.c_int32), ("tokens", C.c_int64), ("slots", C.c_void_p), ("k_out", C.c_void_p),
+                ("v_out", C.c_void_p), ("ldk", C.c_int64), ("ldv", C.c_int64)]
+
+
+class Kv4AttentionDesc(C.Structure):
+    _fields_ = [
+        ("cache", Kv4Cache), ("dtype", C.c_int32), ("requests", C.c_int32), ("tokens", C.c_int64), ("q_heads", C.c_int32),
+        ("max_blocks", C.c_int32), ("max_query", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("out", C.c_void_p), ("ldq", C.c_int64), ("ldo", C.c_int64), ("lse", C.c_void_p), ("block_table", C.c_void_p),
+        ("total_lens", C.c_void_p), ("query_start", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -114,6 +174,7 @@ def lib():
         handle.fth_b200_fp8_linear_workspace_bytes.restype = C.c_size_t
         handle.fth_b200_int8_linear_workspace_bytes.restype = C.c_size_t
         handle.fth_b200_noalloc_scratch_bytes.restype = C.c_size_t
+        handle.fth_b200_kv4_attention_workspace_bytes.restype = C.c_size_t
         handle.fth_b200_plan_input_bytes.restype = C.c_int64
         handle.fth_b200_plan_output_bytes.restype = C.c_int64
         handle.fth_b200_plan_input_bytes.argtypes = [C.c_void_p]
@@ -293,6 +354,238 @@ def silu(dtype, x, out, count, stream=None) -> None:
 def silu_mul(dtype, gate, up, out, count, stream=None) -> None:
     check(lib().fth_b200_silu_mul(C.c_int32(dtype), C.c_void_p(ptr(gate)), C.c_void_p(ptr(up)), C.c_void_p(ptr(out)), C.c_int64(count),
                                   stream or current_stream()), "fth_b200_silu_mul")
+
+
+# ---- rotary positions, the 4-bit cache and its attention (include/fth_b200.h) -------------------------------------------
+# The *_desc functions take torch tensors or device addresses.  A tensor must live on a GPU, the same one for all tensors of
+# a descriptor; its row stride is taken from it unless a stride is given.  The calls run on that GPU, on its current stream
+# unless one is given.
+
+def _tensors(desc, **tensors):
+    """Stores the addresses in the descriptor's fields, checks where the tensors are, and keeps them alive with it."""
+    keep, device = [], None
+    for name, t in tensors.items():
+        if hasattr(t, "data_ptr"):
+            if not t.is_cuda:
+                raise ValueError(f"{name} is not on a GPU")
+            if device is not None and t.device.index != device:
+                raise ValueError(f"{name} is on cuda:{t.device.index}, other tensors on cuda:{device}")
+            device = t.device.index
+        keep.append(t)
+        setattr(desc, name, ptr(t))
+    desc._keep = getattr(desc, "_keep", []) + keep
+    if device is not None:
+        if getattr(desc, "_device", device) != device:
+            raise ValueError(f"tensors on cuda:{device} and cuda:{desc._device}")
+        desc._device = device
+    return desc
+
+
+def _dense(**tensors):
+    for name, t in tensors.items():
+        if hasattr(t, "is_contiguous") and not t.is_contiguous():
+            raise ValueError(f"{name} is not contiguous")
+
+
+_SIZES = {FP32: 4, FP16: 2, BF16: 2}
+
+
+def _rows(name, t, dtype, tokens, heads, head_dim, ld):
+    """Row stride of [tokens, heads, head_dim] (or [tokens, heads * head_dim])."""
+    if t is None or not hasattr(t, "stride"):
+        return ld
+    if t.element_size() != _SIZES.get(dtype, t.element_size()):
+        raise ValueError(f"{name} has {t.element_size()}-byte elements")
+    if ld == 0 and t.dim() >= 2:
+        inner = t.stride(-1) == 1 or t.shape[-1] == 1
+        if t.dim() == 3:
+            inner = inner and (t.stride(1) == head_dim or t.shape[1] == 1) and t.shape[1] * t.shape[2] == heads * head_dim
+        else:
+            inner = inner and t.dim() == 2 and t.shape[1] == heads * head_dim
+        if not inner or t.shape[0] < tokens:
+            raise ValueError(f"{name}: expected [{tokens}, {heads}, {head_dim}] with heads {head_dim} apart, got {tuple(t.shape)}, strides {t.stride()}")
+        if t.shape[0] > 1:
+            return t.stride(0)
+    return ld
+
+
+def _count(name, t, count):
+    if hasattr(t, "numel") and t.numel() < count:
+        raise ValueError(f"{name} has {t.numel()} elements, needs {count}")
+    if hasattr(t, "element_size") and t.element_size() != 4:
+        raise ValueError(f"{name} has {t.element_size()}-byte elements, needs 4")
+
+
+def _call(name, desc, stream):
+    """Runs an entry point with the descriptor's GPU current."""
+    fn = getattr(lib(), name)
+    device = getattr(desc, "_device", None)
+    if device is None:
+        check(fn(C.byref(desc), stream or current_stream()), name)
+        return
+    import torch
+    if torch.cuda.current_device() == device:
+        check(fn(C.byref(desc), stream or C.c_void_p(torch.cuda.current_stream().cuda_stream)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(C.byref(desc), stream or C.c_void_p(torch.cuda.current_stream().cuda_stream)), name)
+
+
+def rope_turns(rotary_dim, base=10000.0, scaling="none", factor=1.0, original=0.0, fast=0.0, slow=0.0):
+    """Host table of turns per position (float64, [rotary_dim / 2]) and the amplitude; see fth_b200_rope_turns."""
+    import numpy as np
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling {scaling!r}: one of {sorted(ROPE_SCALINGS)}")
+    s = RopeScaling(rotary_dim, ROPE_SCALINGS[scaling], base, factor, original, fast, slow)
+    turns, amplitude = np.empty(max(rotary_dim // 2, 0), np.float64), C.c_float()
+    check(lib().fth_b200_rope_turns(C.byref(s), C.c_void_p(turns.ctypes.data), C.byref(amplitude)), "fth_b200_rope_turns")
+    return turns, amplitude.value
+
+
+def rope_desc(*, dtype, layout, tokens, head_dim, rotary_dim, positions, turns, amplitude=1.0, q=None, q_out=None, q_heads=0, k=None,
+              k_out=None, k_heads=0, ldq=0, ldq_out=0, ldk=0, ldk_out=0) -> RopeDesc:
+    d = RopeDesc()
+    d.dtype, d.layout, d.tokens, d.head_dim, d.rotary_dim = dtype, layout, tokens, head_dim, rotary_dim
+    d.q_heads, d.k_heads, d.amplitude = q_heads, k_heads, amplitude
+    d.ldq, d.ldq_out = _rows("q", q, dtype, tokens, q_heads, head_dim, ldq), _rows("q_out", q_out, dtype, tokens, q_heads, head_dim, ldq_out)
+    d.ldk, d.ldk_out = _rows("k", k, dtype, tokens, k_heads, head_dim, ldk), _rows("k_out", k_out, dtype, tokens, k_heads, head_dim, ldk_out)
+    _dense(positions=positions, turns=turns)
+    _count("positions", positions, tokens)
+    if hasattr(turns, "element_size") and (turns.element_size() != 8 or turns.numel() < rotary_dim // 2):
+        raise ValueError(f"turns: needs {rotary_dim // 2} float64")
+    return _tensors(d, q=q, q_out=q_out, k=k, k_out=k_out, positions=positions, turns=turns)
+
+
+def rope(desc: RopeDesc, stream=None) -> None:
+    _call("fth_b200_rope", desc, stream)
+
+
+def kv4_cache(*, k_codes, v_codes, k_params, v_params, blocks, block_size, kv_heads, head_dim) -> Kv4Cache:
+    c = Kv4Cache()
+    c.blocks, c.block_size, c.kv_heads, c.head_dim = blocks, block_size, kv_heads, head_dim
+    tensors = dict(k_codes=k_codes, v_codes=v_codes, k_params=k_params, v_params=v_params)
+    _dense(**tensors)
+    tokens = blocks * kv_heads * block_size
+    for name, t in tensors.items():
+        need = tokens * (head_dim // 2 if "codes" in name else 4)
+        if hasattr(t, "numel") and t.numel() * t.element_size() < need:
+            raise ValueError(f"{name} has {t.numel() * t.element_size()} bytes, needs {need}")
+    return _tensors(c, **tensors)
+
+
+def kv4_new_cache(torch, *, blocks, block_size, kv_heads, head_dim, device="cuda") -> Kv4Cache:
+    """Allocates one layer's cache (its contents are arbitrary until they are written)."""
+    codes, params = (blocks, kv_heads, block_size, head_dim // 2), (blocks, kv_heads, block_size)
+    make = lambda shape, dtype: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
+    return kv4_cache(k_codes=make(codes, torch.uint8), v_codes=make(codes, torch.uint8), k_params=make(params, torch.int32),
+                     v_params=make(params, torch.int32), blocks=blocks, block_size=block_size, kv_heads=kv_heads, head_dim=head_dim)
+
+
+def _with_cache(d, cache):
+    d.cache = cache
+    d._keep = [cache]
+    if hasattr(cache, "_device"):
+        d._device = cache._device
+    return d
+
+
+def kv4_assign_desc(*, requests, max_blocks, block_size, blocks, tokens, cached_lens, new_lens, free_blocks, free_count, free_count_out,
+                    block_table, total_lens, query_start, slots, positions, status) -> Kv4AssignDesc:
+    d = Kv4AssignDesc()
+    d.requests, d.max_blocks, d.block_size, d.blocks, d.tokens = requests, max_blocks, block_size, blocks, tokens
+    t = dict(cached_lens=cached_lens, new_lens=new_lens, free_blocks=free_blocks, free_count=free_count, free_count_out=free_count_out,
+             block_table=block_table, total_lens=total_lens, query_start=query_start, slots=slots, positions=positions, status=status)
+    need = dict(cached_lens=requests, new_lens=requests, free_blocks=blocks, free_count=1, free_count_out=1, block_table=requests * max_blocks,
+                total_lens=requests, query_start=requests + 1, slots=tokens, positions=tokens, status=2)
+    _dense(**t)
+    for name in t:
+        _count(name, t[name], need[name])
+    return _tensors(d, **t)
+
+
+def kv4_assign(desc: Kv4AssignDesc, stream=None) -> None:
+    _call("fth_b200_kv4_assign", desc, stream)
+
+
+def kv4_release_desc(*, requests, max_blocks, block_size, blocks, lens, keep_lens, free_blocks, free_count, free_count_out, block_table,
+                     lens_out, status) -> Kv4ReleaseDesc:
+    d = Kv4ReleaseDesc()
+    d.requests, d.max_blocks, d.block_size, d.blocks = requests, max_blocks, block_size, blocks
+    t = dict(lens=lens, keep_lens=keep_lens, free_blocks=free_blocks, free_count=free_count, free_count_out=free_count_out,
+             block_table=block_table, lens_out=lens_out, status=status)
+    need = dict(lens=requests, keep_lens=requests, free_blocks=blocks, free_count=1, free_count_out=1, block_table=requests * max_blocks,
+                lens_out=requests, status=2)
+    _dense(**t)
+    for name in t:
+        _count(name, t[name], need[name])
+    return _tensors(d, **t)
+
+
+def kv4_release(desc: Kv4ReleaseDesc, stream=None) -> None:
+    _call("fth_b200_kv4_release", desc, stream)
+
+
+def kv4_append_desc(*, cache, dtype, tokens, k, v, slots, ldk=0, ldv=0, rope=None) -> Kv4AppendDesc:
+    """rope: a rope_desc of the same k with k_out=None (its q is turned in the same launch)."""
+    d = _with_cache(Kv4AppendDesc(), cache)
+    d.dtype, d.tokens = dtype, tokens
+    d.ldk, d.ldv = _rows("k", k, dtype, tokens, cache.kv_heads, cache.head_dim, ldk), _rows("v", v, dtype, tokens, cache.kv_heads, cache.head_dim, ldv)
+    _dense(slots=slots)
+    _count("slots", slots, tokens)
+    if rope is not None:
+        if getattr(rope, "_device", getattr(d, "_device", None)) != getattr(d, "_device", None):
+            raise ValueError("rope tensors and cache are on different GPUs")
+        d._keep.append(rope)
+        d.rope = C.addressof(rope)
+    return _tensors(d, k=k, v=v, slots=slots)
+
+
+def kv4_append(desc: Kv4AppendDesc, stream=None) -> None:
+    _call("fth_b200_kv4_append", desc, stream)
+
+
+def kv4_gather_desc(*, cache, dtype, tokens, slots, k_out=None, v_out=None, ldk=0, ldv=0) -> Kv4GatherDesc:
+    d = _with_cache(Kv4GatherDesc(), cache)
+    d.dtype, d.tokens = dtype, tokens
+    d.ldk = _rows("k_out", k_out, dtype, tokens, cache.kv_heads, cache.head_dim, ldk)
+    d.ldv = _rows("v_out", v_out, dtype, tokens, cache.kv_heads, cache.head_dim, ldv)
+    _dense(slots=slots)
+    _count("slots", slots, tokens)
+    return _tensors(d, slots=slots, k_out=k_out, v_out=v_out)
+
+
+def kv4_gather(desc: Kv4GatherDesc, stream=None) -> None:
+    _call("fth_b200_kv4_gather", desc, stream)
+
+
+def kv4_attention_desc(*, cache, dtype, requests, tokens, q_heads, q, out, block_table, max_blocks, total_lens, scale, query_start=None,
+                       max_query=1, causal=True, window=0, lse=None, ldq=0, ldo=0, workspace=None, workspace_bytes=0) -> Kv4AttentionDesc:
+    d = _with_cache(Kv4AttentionDesc(), cache)
+    d.dtype, d.requests, d.tokens, d.q_heads, d.max_blocks, d.max_query = dtype, requests, tokens, q_heads, max_blocks, max_query
+    d.causal, d.window, d.scale, d.workspace_bytes = int(causal), window, scale, workspace_bytes
+    d.ldq, d.ldo = _rows("q", q, dtype, tokens, q_heads, cache.head_dim, ldq), _rows("out", out, dtype, tokens, q_heads, cache.head_dim, ldo)
+    _dense(block_table=block_table, total_lens=total_lens, query_start=query_start, lse=lse)
+    _count("block_table", block_table, requests * max_blocks)
+    _count("total_lens", total_lens, requests)
+    _count("query_start", query_start, requests + 1)
+    _count("lse", lse, tokens * q_heads)
+    return _tensors(d, q=q, out=out, lse=lse, block_table=block_table, total_lens=total_lens, query_start=query_start, workspace=workspace)
+
+
+def kv4_attention_workspace(torch, desc: Kv4AttentionDesc):
+    """Allocates and zero-fills the scratch an attention descriptor needs and attaches it; returns the tensor."""
+    need = lib().fth_b200_kv4_attention_workspace_bytes(C.byref(desc))
+    if not need:
+        check(lib().fth_b200_kv4_attention_supported(C.byref(desc)), "fth_b200_kv4_attention_supported")
+        return None
+    ws = torch.zeros(need, dtype=torch.uint8, device=f"cuda:{desc._device}" if getattr(desc, "_device", None) is not None else "cuda")
+    _tensors(desc, workspace=ws)
+    desc.workspace_bytes = need
+    return ws
+
+
+def kv4_attention(desc: Kv4AttentionDesc, stream=None) -> None:
+    _call("fth_b200_kv4_attention", desc, stream)
 
 
 def device_status() -> int:
