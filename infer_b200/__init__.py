@@ -416,19 +416,26 @@ def _count(name, t, count):
         raise ValueError(f"{name} has {t.element_size()}-byte elements, needs 4")
 
 
+def _raw_stream(device):
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 def _call(name, desc, stream):
     """Runs an entry point with the descriptor's GPU current."""
-    fn = getattr(lib(), name)
+    call = getattr(desc, "_call", None)
+    if call is None:  # the foreign function and its argument, looked up once per descriptor
+        import torch
+        call = desc._call = (getattr(lib(), name), C.byref(desc), torch.cuda)
+    fn, arg, cuda = call
     device = getattr(desc, "_device", None)
-    if device is None:
-        check(fn(C.byref(desc), stream or current_stream()), name)
-        return
-    import torch
-    if torch.cuda.current_device() == device:
-        check(fn(C.byref(desc), stream or C.c_void_p(torch.cuda.current_stream().cuda_stream)), name)
+    if device is None or cuda.current_device() == device:
+        code = fn(arg, stream or C.c_void_p(_raw_stream(device)))
     else:
-        with torch.cuda.device(device):
-            check(fn(C.byref(desc), stream or C.c_void_p(torch.cuda.current_stream().cuda_stream)), name)
+        with cuda.device(device):
+            code = fn(arg, stream or C.c_void_p(_raw_stream(device)))
+    if code != OK:
+        raise B200Error(code, name)
 
 
 def rope_turns(rotary_dim, base=10000.0, scaling="none", factor=1.0, original=0.0, fast=0.0, slow=0.0):
