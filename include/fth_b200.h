@@ -457,8 +457,8 @@ int fth_b200_rope(const fth_b200_rope_desc* desc, fth_b200_stream_t stream);
  * attends to it is NaN.
  * A slot is block * block_size + offset. */
 typedef struct {
-    void* k_codes; /* 16-byte aligned */
-    void* v_codes; /* 16-byte aligned */
+    void* k_codes; /* all four 16-byte aligned */
+    void* v_codes;
     void* k_params;
     void* v_params;
     int64_t blocks;     /* blocks * block_size < 2^31 */

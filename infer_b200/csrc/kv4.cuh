@@ -59,7 +59,7 @@ inline int CheckCache(const fth_b200_kv4_cache& c) {
     if (rc != FTH_B200_OK) return rc;
     if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return FTH_B200_ERR_UNSUPPORTED;
     if (c.kv_heads > 4096) return FTH_B200_ERR_UNSUPPORTED;
-    if (!AlignedTo(c.k_codes, 16) || !AlignedTo(c.v_codes, 16) || !AlignedTo(c.k_params, 4) || !AlignedTo(c.v_params, 4)) return FTH_B200_ERR_INVALID;
+    if (!AlignedTo(c.k_codes, 16) || !AlignedTo(c.v_codes, 16) || !AlignedTo(c.k_params, 16) || !AlignedTo(c.v_params, 16)) return FTH_B200_ERR_INVALID;
     return FTH_B200_OK;
 }
 

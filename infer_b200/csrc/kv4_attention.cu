@@ -1,4 +1,4 @@
-// Attention over the 4-bit cache.
+// Attention over the 4-bit cache, few query rows per kv head (single tokens, drafts).
 //
 // The codes go into the matrix instructions as they are.  With value = m + s c per token (one scale and minimum for a
 // whole head),
@@ -6,14 +6,20 @@
 // so scales touch scores and probabilities, never elements.  A four-bit code in the low bits of a half-precision number is
 // the number c * 2^-24 (a subnormal, exact in the matrix units), and four bits higher 16 c * 2^-24: one AND makes two
 // operands out of a packed word, and eight codes take five operations.  The factors go into q (1/16 on the elements in
-// the higher places, a power of two per row that puts its largest element at 2^14) and into the results; all are exact.
+// the higher places, a power of two that puts the largest element of the rows at 2^14) and into the results; all are exact.
 //
 // S^T = K q^T: tokens are the 16 rows of the instruction, query rows its 8 columns, so a group of up to eight query
 // heads fills it and the products of one K word serve all of them.  O^T = V^T P^T likewise: head elements are its rows.
-// P^T comes from S^T by transposing 8 x 8 tiles within the warp.  Every lane loads exactly the words it multiplies (16
-// bytes, neighbouring lanes neighbouring addresses) through a ring of its own in shared memory: no exchange, no barrier.
+// P^T comes from S^T by transposing 8 x 8 tiles within the warp.  A warp streams its tokens, 64 at a time (32 for wide
+// heads), through a ring of its own with bulk copies: a block's codes of one head are contiguous, and every lane finds
+// the words it multiplies 16 bytes apart from its neighbours'.  No barrier between warps.
 //
-// Work is the flat list of (request, kv head, block of 8 or 16 query rows, tile of 128 tokens); every block of threads
+// A weight p s rounded to FP16 (11 bits) stands for the probability in all three sums of the result: the weighted codes, the
+// sum of minima and the sum that divides them (weight / s gives the probability back), so a rounding moves the result by
+// a rounding of that token's share of (v - out), not by one of its code, which is far larger than the value when minimum
+// and code cancel.  The lse is taken from the probabilities before the rounding.
+//
+// Work is the flat list of (request, kv head, block of 8 or 16 query rows, tile of tokens); every block of threads
 // takes an equal, contiguous share, found from the lengths on the device.  A unit cut by shares leaves partial results
 // (maximum, sum, weighted values, FP32) in the workspace; the part that arrives last joins them in order.
 //
@@ -29,61 +35,34 @@ using namespace rowops;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kWarpTokens = 32;
-constexpr int kTile = kWarps * kWarpTokens;
-constexpr float kNoMax = -1e30f;      // below every score, and finite: differences stay numbers
 constexpr float kLazy = 8.0f;         // a running maximum may lag by 2^8 before sums are rescaled
-
-__device__ __forceinline__ void CopyAsync16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void CopyAsync8(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void CopyAsync4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void CopyWait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ void MmaF16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t Transpose8x8(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ float Exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t PackHalf(float low, float high) {
-    const __half2 h = __floats2half2_rn(low, high);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+constexpr float kNotStarted = -3e38f;
 
 template <int D>
 struct Shape {
-    static constexpr int kWords = D / 32;            // packed words a lane holds of a token (K) or of a pair of tokens (V)
-    static constexpr int kStages = D == 256 ? 3 : 4;
-    // a stage of a warp's ring: per 16 tokens two K rows and two V rows of kWords words for each lane, then 32 parameters
-    static constexpr int kSubBytes = 4 * kWords * 4 * 32;
-    static constexpr int kStageBytes = 2 * kSubBytes + 2 * 128;
+    static constexpr int kWords = D / 32;                 // packed words a lane holds of a token (K) or of a pair of tokens (V)
+    static constexpr int kStep = D == 256 ? 32 : 64;      // tokens of a stage
+    static constexpr int kSubs = kStep / 16;
+    static constexpr int kStages = D == 128 ? 2 : 3;
+    static constexpr int kTile = kWarps * kStep;
+    // a stage: K codes, V codes, K parameters, V parameters
+    static constexpr int kCodeBytes = kStep * D / 2;
+    static constexpr int kStageBytes = 2 * kCodeBytes + 2 * kStep * 4;
     static constexpr int kRingBytes = kStages * kStageBytes;
+    static constexpr int kBlocksPerSm = D == 256 ? 2 : 3;
 };
 
 template <int D, int NT>
-constexpr size_t DecodeSmem() {
-    const size_t ring = static_cast<size_t>(kWarps) * Shape<D>::kRingBytes;
-    const size_t join = static_cast<size_t>(kWarps) * 8 * NT * (D + 2) * sizeof(float);
-    return ring > join ? ring : join;
-}
+constexpr bool kQueriesInShared = D == 256 && NT == 2;   // 64 registers of fragments would not fit beside 128 accumulators
+
+// Dynamic shared memory: the warps' rings, in whose place their results are joined, then query operands.
+template <int D, int NT>
+struct Layout {
+    static constexpr size_t kRings = static_cast<size_t>(kWarps) * Shape<D>::kRingBytes;
+    static constexpr size_t kJoin = static_cast<size_t>(kWarps) * 8 * NT * kRow<D> * sizeof(float);
+    static constexpr size_t kQueries = kRings > kJoin ? kRings : (kJoin + 15) / 16 * 16;
+    static constexpr size_t kBytes = kQueries + (kQueriesInShared<D, NT> ? NT * Shape<D>::kWords * 32 * 16 : 0);
+};
 
 // Sum of v over the block, and the sum over the threads before this one.
 __device__ __forceinline__ int64_t ScanWork(int64_t v, int64_t* shared, int64_t* total) {
@@ -98,7 +77,8 @@ __device__ __forceinline__ int64_t ScanWork(int64_t v, int64_t* shared, int64_t*
     if (lane == 31) shared[warp] = s;
     __syncthreads();
     int64_t before = 0, all = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
         if (w < warp) before += shared[w];
         all += shared[w];
     }
@@ -118,68 +98,54 @@ __device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, const 
     return sum;
 }
 
-// One lane's place in the cache for the 16 tokens that start at `token` (a multiple of 16 within a block).
-template <int D>
-__device__ __forceinline__ void IssueSub(const AttentionParams& p, uint32_t ring, int64_t base, int offset, int lane) {
-    constexpr int W = Shape<D>::kWords;
-    const int g = lane >> 2, quad = lane & 3;
-    const uint8_t* k = p.cache.k_codes + (base + offset) * (D / 2);
-    const uint8_t* v = p.cache.v_codes + (base + offset) * (D / 2);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const uint8_t* krow = k + (g + 8 * half) * (D / 2);
-        const uint8_t* vrow = v + (quad + 4 * half) * D;
-        const uint32_t dk = ring + half * (W * 128), dv = ring + (2 + half) * (W * 128);
-        if constexpr (W == 2) {
-            CopyAsync8(dk + lane * 8, krow + quad * 8);
-            CopyAsync8(dv + lane * 8, vrow + g * 8);
-        } else {
-#pragma unroll
-            for (int c = 0; c < W / 4; ++c) {
-                CopyAsync16(dk + c * 512 + lane * 16, krow + c * 64 + quad * 16);
-                CopyAsync16(dv + c * 512 + lane * 16, vrow + c * 128 + g * 16);
-            }
-        }
-    }
-}
-template <int W>
-__device__ __forceinline__ void LoadWords(const uint8_t* at, int lane, uint32_t (&w)[W]) {
+// A lane's packed words of one token row (or row of a pair of tokens): four words every 64 (K) or 128 (V) bytes.
+template <int W, int SPACING>
+__device__ __forceinline__ void LoadChunk(const uint8_t* row, int place, int chunk, uint32_t (&w)[4]) {
     if constexpr (W == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(at + lane * 8);
+        const uint2 x = *reinterpret_cast<const uint2*>(row + place * 8);
         w[0] = x.x;
         w[1] = x.y;
     } else {
-#pragma unroll
-        for (int c = 0; c < W / 4; ++c) {
-            const uint4 x = *reinterpret_cast<const uint4*>(at + c * 512 + lane * 16);
-            w[4 * c] = x.x;
-            w[4 * c + 1] = x.y;
-            w[4 * c + 2] = x.z;
-            w[4 * c + 3] = x.w;
-        }
+        const uint4 x = *reinterpret_cast<const uint4*>(row + chunk * SPACING + place * 16);
+        w[0] = x.x;
+        w[1] = x.y;
+        w[2] = x.z;
+        w[3] = x.w;
     }
 }
 
 template <int D, int DTYPE, int NT>
 __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__ AttentionParams p) {
-    constexpr int W = Shape<D>::kWords;
-    constexpr int S = Shape<D>::kStages;
+    using T = Shape<D>;
+    constexpr int W = T::kWords;
+    constexpr int CW = W == 2 ? 2 : 4;        // words of a chunk
+    constexpr int S = T::kStages;
     constexpr int R = 8 * NT;
+    constexpr bool QS = kQueriesInShared<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan[kWarps];
+    __shared__ Request start_req;
     __shared__ int start_request;
-    __shared__ int64_t start_offset;
+    __shared__ int64_t start_offset, start_per_head;
     __shared__ int join_last;
+    __shared__ __align__(8) uint64_t bars[kWarps * S];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, quad = lane & 3;
+    if (lane < S) MbarInit(&bars[warp * S + lane], 1);
+    FenceBarrierInit();
     WaitForPrevious();
 
     // ---- this block's share of the tiles --------------------------------------------------------------------------------
-    int64_t work = 0, mine = 0, before = 0;
+    int64_t work = 0, mine = 0, before = 0, per_head = 0;
+    Request req;
     for (int base = 0; base < p.requests; base += kThreads) {
         const int b = base + threadIdx.x;
         mine = 0;
-        if (b < p.requests) mine = RequestTiles<kTile>(p, LoadRequest(p, b), R) * p.kv_heads;
+        if (b < p.requests) {
+            req = LoadRequest(p, b);
+            per_head = RequestTiles<T::kTile>(p, req, R);
+            mine = per_head * p.kv_heads;
+        }
         int64_t total;
         before = ScanWork(mine, scan, &total);
         work += total;
@@ -195,12 +161,18 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
         if (p.requests > kThreads) {
             const int b = base + threadIdx.x;
             mine = 0;
-            if (b < p.requests) mine = RequestTiles<kTile>(p, LoadRequest(p, b), R) * p.kv_heads;
+            if (b < p.requests) {
+                req = LoadRequest(p, b);
+                per_head = RequestTiles<T::kTile>(p, req, R);
+                mine = per_head * p.kv_heads;
+            }
             before = ScanWork(mine, scan, &total);
         }
         if (share_begin >= passed + before && share_begin < passed + before + mine) {
             start_request = base + threadIdx.x;
             start_offset = share_begin - passed - before;
+            start_req = req;
+            start_per_head = per_head;
         }
         passed += total;
         if (passed > share_begin) break;
@@ -209,144 +181,69 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
 
     // ---- the first unit: request, head, rows, tiles ---------------------------------------------------------------------
     int b = start_request;
-    Request req = LoadRequest(p, b);
-    const int64_t per_head = RequestTiles<kTile>(p, req, R);
-    int head = static_cast<int>(start_offset / per_head);
+    req = start_req;
+    int head = static_cast<int>(start_offset / start_per_head);
     int row = 0;
-    int64_t into = start_offset % per_head;  // tiles of the unit that other blocks take
+    int64_t into = start_offset - head * start_per_head;  // tiles of the unit that other blocks take
     int tile_first, tile_last;
     for (;;) {
-        UnitTiles<kTile>(p, req, row, R, &tile_first, &tile_last);
+        UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
         if (into < tile_last - tile_first) break;
         into -= tile_last - tile_first;
         row += R;
     }
     int64_t at = share_begin;
-    const uint32_t ring = SmemAddr(smem) + warp * Shape<D>::kRingBytes;
-    uint8_t* ring_ptr = smem + warp * Shape<D>::kRingBytes;
+    uint8_t* ring = smem + warp * T::kRingBytes;
+    uint64_t* bar = bars + warp * S;
+    uint32_t phases = 0;   // parity of each stage's next completion
+    bool failed = false;
 
     for (;;) {
         const int64_t unit_begin = at - into;
         const int64_t unit_end = unit_begin + (tile_last - tile_first);
         const int t0 = tile_first + static_cast<int>(into);
         const int64_t here = (unit_end < share_end ? unit_end : share_end) - at;
-        const int t1 = t0 + static_cast<int>(here);
-
-        // ---- query rows ----------------------------------------------------------------------------------------------------
-        uint32_t qf[NT][2 * W][2];
-        float f[NT][2], qsum[NT][2];   // of the columns 2 * quad, 2 * quad + 1
-        int row_low[NT][2], row_high[NT][2];
-        int all_low = 0, all_high = 0x7fffffff;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = row + n * 8 + g;
-            const bool valid = r < req.rows;
-            const int query = valid ? r / p.group : 0;
-            const int64_t from = valid ? (req.first_row + static_cast<int64_t>(query)) * p.ldq + (static_cast<int64_t>(head) * p.group + r % p.group) * D : 0;
-            float x[W][8];
-            float big = 0.0f, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const int word = W == 2 ? quad * 2 + w : (w >> 2) * 16 + quad * 4 + (w & 3);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[w][i] = valid ? ReadFloat<DTYPE>(p.q, from + word * 8 + i) : 0.0f;
-                    big = fmaxf(big, fabsf(x[w][i]));
-                    sum += x[w][i];
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            }
-            int e = 14 - (static_cast<int>((__float_as_uint(big) >> 23) & 0xffu) - 127);
-            if (big == 0.0f) e = 0;
-            e = e > 120 ? 120 : e < -86 ? -86 : e;
-            const float up = PowerOfTwo(e);
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[w][i] *= (i & 1) ? up * 0.0625f : up;
-                qf[n][2 * w][0] = PackHalf(x[w][0], x[w][4]);
-                qf[n][2 * w][1] = PackHalf(x[w][1], x[w][5]);
-                qf[n][2 * w + 1][0] = PackHalf(x[w][2], x[w][6]);
-                qf[n][2 * w + 1][1] = PackHalf(x[w][3], x[w][7]);
-            }
-            const float back = p.scale_log2 * PowerOfTwo(24 - e), weighted = p.scale_log2 * sum;
-            int low = 0, high = 0;
-            if (valid) Visible(p, req, query, &low, &high);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int from_lane = (quad * 2 + c) * 4;
-                f[n][c] = __shfl_sync(0xffffffffu, back, from_lane);
-                qsum[n][c] = __shfl_sync(0xffffffffu, weighted, from_lane);
-                row_low[n][c] = __shfl_sync(0xffffffffu, low, from_lane);
-                row_high[n][c] = __shfl_sync(0xffffffffu, high, from_lane);
-            }
-            if (valid) {
-                all_low = low > all_low ? low : all_low;
-                all_high = high < all_high ? high : all_high;
-            }
-        }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            const int l = __shfl_xor_sync(0xffffffffu, all_low, o), h = __shfl_xor_sync(0xffffffffu, all_high, o);
-            all_low = l > all_low ? l : all_low;
-            all_high = h < all_high ? h : all_high;
-        }
+        const int steps = static_cast<int>(here);
         int first_low, last_high, unused;
         Visible(p, req, row / p.group, &first_low, &unused);
         Visible(p, req, ((row + R < req.rows ? row + R : req.rows) - 1) / p.group, &unused, &last_high);
 
-        // ---- tokens -----------------------------------------------------------------------------------------------------------
-        float acc[NT][2 * W][4];
-        float top[NT][2], sum[NT][2], offset[NT][2];
-        float shrink = 1.0f;   // value scales are multiplied by this power of two before they become FP16
-        float scale_limit = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int m = 0; m < 2 * W; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                top[n][c] = kNoMax;
-                sum[n][c] = offset[n][c] = 0.0f;
-            }
-        }
-        const int steps = t1 - t0;
+        // ---- copies: lane = 4 * (16 tokens) + (K codes, V codes, K parameters, V parameters) ----------------------------------
+        // Blocks of more than 16 tokens are copied by the lanes of their first 16, up to a whole step at once.
         const int32_t* table = p.table + static_cast<int64_t>(b) * p.max_blocks;
-        uint32_t have = 0;   // two bits per stage: the block of these 16 tokens exists
-        int id[2];
+        const int span_shift = p.cache.block_shift < (T::kStep == 64 ? 6 : 5) ? p.cache.block_shift : (T::kStep == 64 ? 6 : 5);
+        const int sub = lane >> 2;
+        const bool copies = lane < 4 * T::kSubs && ((sub << 4) & ((1 << span_shift) - 1)) == 0;
+        uint32_t have = 0;   // kSubs bits per stage: these 16 tokens are there
+        int id = -2;
         const auto lookup = [&](int step) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int token = (t0 + step) * kTile + warp * kWarpTokens + s * 16;
-                id[s] = -2;
-                if (step < steps && token < last_high && token + 16 > first_low) id[s] = table[token >> p.cache.block_shift];
-            }
+            const int token = (t0 + step) * T::kTile + warp * T::kStep + sub * 16;
+            id = -2;
+            if (copies && step < steps && token < last_high && token + (1 << span_shift) > first_low) id = table[token >> p.cache.block_shift];
         };
         const auto issue = [&](int step) {
             const int stage = step % S;
-            have &= ~(3u << (2 * stage));
+            const bool good = id >= 0 && id < p.cache.blocks;
+            if (id != -2 && !good && quad == 0) ReportTimeout(p.status, kSiteAttention, b);
+            const uint32_t who = __ballot_sync(0xffffffffu, good);
+            uint32_t there = 0;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int token = (t0 + step) * kTile + warp * kWarpTokens + s * 16;
-                if (id[s] >= 0 && id[s] < p.cache.blocks) {
-                    have |= 1u << (2 * stage + s);
-                    const int64_t base = HeadBase(p.cache, id[s], head);
-                    const int off = token & ((1 << p.cache.block_shift) - 1);
-                    const uint32_t dst = ring + stage * Shape<D>::kStageBytes;
-                    IssueSub<D>(p, dst + s * Shape<D>::kSubBytes, base, off, lane);
-                    const uint32_t* params = (lane < 16 ? p.cache.k_params : p.cache.v_params) + base + off + (lane & 15);
-                    CopyAsync4(dst + 2 * Shape<D>::kSubBytes + s * 128 + lane * 4, params);
-                } else if (id[s] != -2 && lane == 0) {
-                    ReportTimeout(p.status, kSiteAttention, b);
+            for (int i = 0; i < T::kSubs; ++i) there |= ((who >> (4 * (((i << 4) >> span_shift) << (span_shift - 4)))) & 1u) << i;
+            have = (have & ~(((1u << T::kSubs) - 1) << (T::kSubs * stage))) | (there << (T::kSubs * stage));
+            if (lane == 0) MbarExpectTx(&bar[stage], static_cast<uint32_t>(__popc(who)) * (1u << span_shift) * (D + 8) / 4);
+            __syncwarp();
+            if (good) {
+                const int token = (t0 + step) * T::kTile + warp * T::kStep + sub * 16;
+                const int64_t from = HeadBase(p.cache, id, head) + (token & ((1 << p.cache.block_shift) - 1));
+                uint8_t* dst = ring + stage * T::kStageBytes;
+                if (quad < 2) {
+                    BulkLoad(dst + quad * T::kCodeBytes + sub * (16 * D / 2), (quad == 0 ? p.cache.k_codes : p.cache.v_codes) + from * (D / 2),
+                             (1u << span_shift) * (D / 2), &bar[stage]);
+                } else {
+                    BulkLoad(dst + 2 * T::kCodeBytes + (quad - 2) * (T::kStep * 4) + sub * 64, (quad == 2 ? p.cache.k_params : p.cache.v_params) + from,
+                             (1u << span_shift) * 4, &bar[stage]);
                 }
             }
-            CopyCommit();
         };
         lookup(0);
 #pragma unroll
@@ -354,156 +251,340 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
             issue(s);
             lookup(s + 1);
         }
-        for (int step = 0; step < steps; ++step) {
-            CopyWait<S - 2>();
-            __syncwarp();
-            issue(step + S - 1);
-            lookup(step + S);
-            const int stage = step % S;
-            const uint8_t* data = ring_ptr + stage * Shape<D>::kStageBytes;
-            const uint32_t* params = reinterpret_cast<const uint32_t*>(data + 2 * Shape<D>::kSubBytes);
-            const uint32_t present = (have >> (2 * stage)) & 3u;
-            if (present == 0) continue;
-            const int token0 = (t0 + step) * kTile + warp * kWarpTokens;
 
-            // scores, as exponents of two
-            float z[2][NT][4];
-            uint32_t kp[2][2], vp[2][2];
+        // ---- query rows ----------------------------------------------------------------------------------------------------
+        uint32_t qf[QS ? 1 : NT][2 * W][2];
+        uint4* const q_shared = reinterpret_cast<uint4*>(smem + Layout<D, NT>::kQueries);
+        float2 qsum[NT];   // of the columns 2 * quad, 2 * quad + 1
+        int row_low[NT][2], row_high[NT][2];
+        int all_low = 0, all_high = 0x7fffffff;
+        float back;
+        {
+            uint32_t raw[NT][W][4];   // eight 16-bit elements per word of codes
+            float big = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint32_t k0[W], k1[W];
-                LoadWords<W>(data + s * Shape<D>::kSubBytes, lane, k0);
-                LoadWords<W>(data + s * Shape<D>::kSubBytes + W * 128, lane, k1);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    kp[s][h] = params[s * 32 + g + 8 * h];
-                    vp[s][h] = params[s * 32 + 16 + g + 8 * h];
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) z[s][n][i] = 0.0f;
+            for (int n = 0; n < NT; ++n) {
+                const int r = row + n * 8 + g;
+                const bool valid = r < req.rows;
+                const int query = valid ? r / p.group : 0;
+                const uint16_t* from = static_cast<const uint16_t*>(p.q) + (req.first_row + static_cast<int64_t>(query)) * p.ldq +
+                                       (static_cast<int64_t>(head) * p.group + r - query * p.group) * D;
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    const uint32_t x0 = k0[w], x1 = k1[w], y0 = x0 >> 8, y1 = x1 >> 8;
+                    const int word = W == 2 ? quad * 2 + w : (w >> 2) * 16 + quad * 4 + (w & 3);
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (valid) {
+                        if (p.q_vec) x = *reinterpret_cast<const uint4*>(from + word * 8);
+                        else x = LoadUnaligned8(from + word * 8);
+                    }
+                    raw[n][w][0] = x.x;
+                    raw[n][w][1] = x.y;
+                    raw[n][w][2] = x.z;
+                    raw[n][w][3] = x.w;
+                }
+                int low = 0, high = 0;
+                if (valid) {
+                    Visible(p, req, query, &low, &high);
+                    all_low = low > all_low ? low : all_low;
+                    all_high = high < all_high ? high : all_high;
+                }
+                float sum = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        MmaF16(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, qf[n][2 * w][0], qf[n][2 * w][1]);
-                        MmaF16(z[s][n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 v = HalfPair<DTYPE>(raw[n][w][i]);
+                        big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+                        sum += v.x + v.y;
+                    }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                qsum[n].x = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8);
+                qsum[n].y = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8 + 4);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    row_low[n][c] = __shfl_sync(0xffffffffu, low, quad * 8 + c * 4);
+                    row_high[n][c] = __shfl_sync(0xffffffffu, high, quad * 8 + c * 4);
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const int l = __shfl_xor_sync(0xffffffffu, all_low, o), h = __shfl_xor_sync(0xffffffffu, all_high, o);
+                all_low = l > all_low ? l : all_low;
+                all_high = h < all_high ? h : all_high;
+            }
+            // one power of two for all rows: what lies 2^28 below the largest element of the largest row keeps FP16's 11 bits
+            const int e = QueryExponent(big);
+            back = p.scale_log2 * PowerOfTwo(24 - e);
+            const float up = PowerOfTwo(e);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    uint32_t f[4];
+                    QueryOperands<DTYPE>(raw[n][w], up, f);
+                    if constexpr (QS) {
+                        if (warp == 0) q_shared[(n * W + w) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
+                    } else {
+                        qf[n][2 * w][0] = f[0];
+                        qf[n][2 * w][1] = f[1];
+                        qf[n][2 * w + 1][0] = f[2];
+                        qf[n][2 * w + 1][1] = f[3];
                     }
                 }
             }
-            const bool inside = token0 >= all_low && token0 + kWarpTokens <= all_high && present == 3u;
-            bool rescale = false;
-            float vs[2][2], vm[2][2];
+            if constexpr (QS) __syncthreads();
+        }
+
+        // ---- tokens -----------------------------------------------------------------------------------------------------------
+        float acc[NT][2 * W][4];
+        float2 top[NT], sum[NT], mass[NT], offset[NT];   // top: the running maximum; scores are kept relative to it
+        float limit[NT][2];                    // a relative score above it moves the maximum
+        float shrink = 1.0f;                   // value scales are multiplied by this power of two before they become FP16
+        float scale_limit = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float ks = ParamScale(kp[s][h]), km = ParamMin(kp[s][h]);
-                    vs[s][h] = ParamScale(vp[s][h]);
-                    vm[s][h] = ParamMin(vp[s][h]);
-                    bool seen_by_any = inside;
+            for (int m = 0; m < 2 * W; ++m)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float& score = z[s][n][2 * h + c];
-                            score = fmaf(ks, score * f[n][c], km * qsum[n][c]);
-                            if (!inside) {
-                                const int token = token0 + s * 16 + h * 8 + g;
-                                const bool seen = ((present >> s) & 1u) != 0 && token >= row_low[n][c] && token < row_high[n][c];
-                                if (!seen) score = -INFINITY;
-                                seen_by_any = seen_by_any || seen;
-                            }
-                            rescale = rescale || score > top[n][c] + kLazy;
-                        }
-                    }
-                    if (!seen_by_any) vs[s][h] = vm[s][h] = 0.0f;  // whatever stands there: 0 * NaN is no zero
-                    rescale = rescale || vs[s][h] > scale_limit;
-                }
-            }
-            if (__any_sync(0xffffffffu, rescale)) {
-                float biggest = scale_limit * 0.5f;
+                for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.0f;
+            top[n] = sum[n] = mass[n] = offset[n] = make_float2(0.0f, 0.0f);
+            limit[n][0] = limit[n][1] = kNotStarted;
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int stage = step % S;
+            if (!failed && !MbarWait(&bar[stage], (phases >> stage) & 1u, p.status, kSiteAttentionWait, stage)) failed = true;
+            phases ^= 1u << stage;
+            __syncwarp();  // every lane is done with the stage that is filled next
+            issue(step + S - 1);
+            lookup(step + S);
+            const uint8_t* data = ring + stage * T::kStageBytes;
+            const uint32_t* k_params = reinterpret_cast<const uint32_t*>(data + 2 * T::kCodeBytes);
+            const uint32_t* v_params = k_params + T::kStep;
+            const uint32_t present_all = (have >> (T::kSubs * stage)) & ((1u << T::kSubs) - 1);
+#pragma unroll 1
+            for (int half = 0; half < T::kSubs / 2; ++half) {   // 32 tokens
+                const uint32_t present = (present_all >> (2 * half)) & 3u;
+                if (present == 0) continue;
+                const int token0 = (t0 + step) * T::kTile + warp * T::kStep + half * 32;
+                const uint8_t* k_rows = data + half * (32 * D / 2);
+                const uint8_t* v_rows = k_rows + T::kCodeBytes;
+
+                // q . c
+                float z[2][NT][4];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (vs[s][h] > biggest) biggest = vs[s][h];
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, o));
-                float change = 1.0f;
-                if (biggest > scale_limit) {
-                    // 2^e > biggest: with probabilities up to 2^8 the products stay below 2^15
-                    int e = static_cast<int>((__float_as_uint(biggest) >> 23) & 0xffu) - 126;
-                    e = e > 120 ? 120 : e < -100 ? -100 : e;
-                    const float next = PowerOfTwo(7 - e);
-                    change = scale_limit == 0.0f ? 0.0f : next / shrink;
-                    shrink = next;
-                    scale_limit = PowerOfTwo(e);
-                }
+                        for (int i = 0; i < 4; ++i) z[s][n][i] = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float factor[2];
+                for (int c = 0; c < W / CW; ++c) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float best = top[n][c];
+                    for (int s = 0; s < 2; ++s) {
+                        uint32_t k0[4], k1[4];
+                        LoadChunk<W, 64>(k_rows + (s * 16 + g) * (D / 2), quad, c, k0);
+                        LoadChunk<W, 64>(k_rows + (s * 16 + 8 + g) * (D / 2), quad, c, k1);
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) best = fmaxf(best, fmaxf(z[s][n][c], z[s][n][2 + c]));
+                        for (int i = 0; i < CW; ++i) {
+                            const int w = c * CW + i;
+                            const uint32_t x0 = k0[i], x1 = k1[i], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-                        const float alpha = Exp2(top[n][c] - best);
-                        top[n][c] = best;
-                        sum[n][c] *= alpha;
-                        offset[n][c] *= alpha;
-                        factor[c] = alpha * change;
-                    }
-#pragma unroll
-                    for (int m = 0; m < 2 * W; ++m) {
-                        acc[n][m][0] *= factor[0];
-                        acc[n][m][1] *= factor[1];
-                        acc[n][m][2] *= factor[0];
-                        acc[n][m][3] *= factor[1];
+                            for (int n = 0; n < NT; ++n) {
+                                uint4 f;
+                                if constexpr (QS) f = q_shared[(n * W + w) * 32 + lane];
+                                else f = make_uint4(qf[n][2 * w][0], qf[n][2 * w][1], qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                                MmaF16(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, f.x, f.y);
+                                MmaF16(z[s][n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, f.z, f.w);
+                            }
+                        }
                     }
                 }
-            }
-            // probabilities and weighted values
+                // scores, exponents of two, relative to the running maximum
+                const bool inside = token0 >= all_low && token0 + 32 <= all_high && present == 3u;
+                float vs[2][2], vm[2][2];
+                bool rescale = false;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                uint32_t pt[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int s = 0; s < 2; ++s) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float weight[2];
+                        const int place = half * 32 + s * 16 + h * 8 + g;
+                        const uint32_t kp = k_params[place], vp = v_params[place];
+                        const float ks = ParamScale(kp) * back, km = ParamMin(kp);
+                        vs[s][h] = ParamScale(vp);
+                        vm[s][h] = ParamMin(vp);
+                        bool seen_by_any = inside;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const float prob = Exp2(z[s][n][2 * h + c] - top[n][c]);
-                            sum[n][c] += prob;
-                            offset[n][c] = fmaf(prob, vm[s][h], offset[n][c]);
-                            weight[c] = prob * (vs[s][h] * shrink);
+                        for (int n = 0; n < NT; ++n) {
+                            float2 t = Fma2(make_float2(km, km), qsum[n], make_float2(-top[n].x, -top[n].y));
+                            t = Fma2(make_float2(ks, ks), make_float2(z[s][n][2 * h], z[s][n][2 * h + 1]), t);
+                            if (!inside) {
+                                const int token = token0 + s * 16 + h * 8 + g;
+                                const bool there = ((present >> s) & 1u) != 0;
+                                const bool seen0 = there && token >= row_low[n][0] && token < row_high[n][0];
+                                const bool seen1 = there && token >= row_low[n][1] && token < row_high[n][1];
+                                if (!seen0) t.x = -INFINITY;
+                                if (!seen1) t.y = -INFINITY;
+                                seen_by_any = seen_by_any || seen0 || seen1;
+                            }
+                            z[s][n][2 * h] = t.x;
+                            z[s][n][2 * h + 1] = t.y;
                         }
-                        pt[n][h] = Transpose8x8(PackHalf(weight[0], weight[1]));
+                        if (!seen_by_any) vs[s][h] = vm[s][h] = 0.0f;  // whatever stands there: 0 * NaN is no zero
+                        rescale = rescale || vs[s][h] > scale_limit;
                     }
                 }
-                uint32_t v0[W], v1[W];
-                LoadWords<W>(data + s * Shape<D>::kSubBytes + 2 * W * 128, lane, v0);
-                LoadWords<W>(data + s * Shape<D>::kSubBytes + 3 * W * 128, lane, v1);
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const uint32_t x0 = v0[w], x1 = v1[w], y0 = x0 >> 8, y1 = x1 >> 8;
+                for (int n = 0; n < NT; ++n) {
+                    const float best0 = fmaxf(fmaxf(z[0][n][0], z[0][n][2]), fmaxf(z[1][n][0], z[1][n][2]));
+                    const float best1 = fmaxf(fmaxf(z[0][n][1], z[0][n][3]), fmaxf(z[1][n][1], z[1][n][3]));
+                    rescale = rescale || best0 > limit[n][0] || best1 > limit[n][1];
+                }
+                if (__any_sync(0xffffffffu, rescale)) {
+                    float biggest = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) biggest = fmaxf(biggest, vs[s][h]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, o));
+                    float change = 1.0f;
+                    if (biggest > scale_limit) {
+                        const int e = ScaleExponent(biggest);
+                        const float next = PowerOfTwo(7 - e);
+                        change = scale_limit == 0.0f ? 0.0f : next / shrink;
+                        shrink = next;
+                        scale_limit = PowerOfTwo(e);
+                    }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        MmaF16(acc[n][2 * w], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, pt[n][0], pt[n][1]);
-                        MmaF16(acc[n][2 * w + 1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, pt[n][0], pt[n][1]);
+                        float2 moved, alpha;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float best = fmaxf(fmaxf(z[0][n][c], z[0][n][2 + c]), fmaxf(z[1][n][c], z[1][n][2 + c]));
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+                            const bool first = limit[n][c] == kNotStarted;
+                            const bool move = first ? best > kNotStarted : best > 0.0f;
+                            const float by = move ? best : 0.0f;
+                            if (move) limit[n][c] = kLazy;
+                            // before the first score the sums are zeros (or NaN, which stay)
+                            (c == 0 ? alpha.x : alpha.y) = first ? 0.0f : Exp2(-by);
+                            (c == 0 ? moved.x : moved.y) = by;
+                        }
+                        top[n].x += moved.x;
+                        top[n].y += moved.y;
+                        sum[n] = Mul2(sum[n], alpha);
+                        mass[n] = Mul2(mass[n], alpha);
+                        offset[n] = Mul2(offset[n], alpha);
+                        const float2 factor = make_float2(alpha.x * change, alpha.y * change);
+#pragma unroll
+                        for (int m = 0; m < 2 * W; ++m) {
+                            acc[n][m][0] *= factor.x;
+                            acc[n][m][1] *= factor.y;
+                            acc[n][m][2] *= factor.x;
+                            acc[n][m][3] *= factor.y;
+                        }
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) z[s][n][i] -= (i & 1) ? moved.y : moved.x;
+                    }
+                }
+                // probabilities, weights, weighted values
+                bool plain = !inside;
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        vs[s][h] *= shrink;
+                        plain = plain || !(vs[s][h] >= 1.0f);
+                    }
+                plain = __any_sync(0xffffffffu, plain);
+                uint32_t pt[2][NT][2];
+                if (!plain) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float inverse = Reciprocal(vs[s][h]);
+                            const float ratio = vm[s][h] * inverse;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                float2 w = make_float2(Exp2(z[s][n][2 * h]), Exp2(z[s][n][2 * h + 1]));
+                                mass[n] = Add2(mass[n], w);
+                                w = Mul2(w, make_float2(vs[s][h], vs[s][h]));
+                                const uint32_t packed = PackHalf(w.x, w.y);
+                                w = HalfPair<FTH_B200_FP16>(packed);
+                                sum[n] = Fma2(w, make_float2(inverse, inverse), sum[n]);
+                                offset[n] = Fma2(w, make_float2(ratio, ratio), offset[n]);
+                                pt[s][n][h] = Transpose8x8(packed);
+                            }
+                        }
+                    }
+                } else {
+                    // masked tokens, and value scales too small beside the largest to give the probability back
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                float w[2];
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    const float zc = z[s][n][2 * h + c];
+                                    const bool hidden = zc == -INFINITY;
+                                    const float prob = Exp2(zc);
+                                    const float weight = hidden ? 0.0f : prob * vs[s][h];
+                                    float& sum_c = c == 0 ? sum[n].x : sum[n].y;
+                                    float& mass_c = c == 0 ? mass[n].x : mass[n].y;
+                                    float& offset_c = c == 0 ? offset[n].x : offset[n].y;
+                                    const float rounded = __half2float(__float2half_rn(weight));
+                                    const float kept = vs[s][h] >= 1.0f ? rounded * Reciprocal(vs[s][h]) : prob;
+                                    if (!hidden) {
+                                        sum_c += kept;
+                                        mass_c += prob;
+                                        offset_c = fmaf(kept, vm[s][h], offset_c);
+                                    }
+                                    w[c] = rounded;
+                                }
+                                pt[s][n][h] = Transpose8x8(PackHalf(w[0], w[1]));
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < W / CW; ++c) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        uint32_t v0[4], v1[4];
+                        LoadChunk<W, 128>(v_rows + (s * 8 + quad) * D, g, c, v0);
+                        LoadChunk<W, 128>(v_rows + (s * 8 + 4 + quad) * D, g, c, v1);
+#pragma unroll
+                        for (int i = 0; i < CW; ++i) {
+                            const int w = c * CW + i;
+                            const uint32_t x0 = v0[i], x1 = v1[i], y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                MmaF16(acc[n][2 * w], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, pt[s][n][0], pt[s][n][1]);
+                                MmaF16(acc[n][2 * w + 1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, pt[s][n][0], pt[s][n][1]);
+                            }
+                        }
                     }
                 }
             }
         }
-        CopyWait<0>();
+        // the stages issued beyond the last step carry no bytes; their phases are passed all the same
+        for (int step = steps; step < steps + S - 1; ++step) {
+            const int stage = step % S;
+            if (!failed && !MbarWait(&bar[stage], (phases >> stage) & 1u, p.status, kSiteAttentionWait, stage)) failed = true;
+            phases ^= 1u << stage;
+        }
 
         // ---- the four warps' results together ---------------------------------------------------------------------------------
-        // [warp][row][D values, maximum, sum], in the rings' memory
+        // [warp][row][D values, maximum, sum, sum for the lse], in the rings' memory
         float* join = reinterpret_cast<float*>(smem);
         __syncthreads();
         {
@@ -511,94 +592,84 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int o = 4; o < 32; o <<= 1) {
+                    sum[n].x += __shfl_xor_sync(0xffffffffu, sum[n].x, o);
+                    sum[n].y += __shfl_xor_sync(0xffffffffu, sum[n].y, o);
+                    mass[n].x += __shfl_xor_sync(0xffffffffu, mass[n].x, o);
+                    mass[n].y += __shfl_xor_sync(0xffffffffu, mass[n].y, o);
+                    offset[n].x += __shfl_xor_sync(0xffffffffu, offset[n].x, o);
+                    offset[n].y += __shfl_xor_sync(0xffffffffu, offset[n].y, o);
+                }
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
-                        offset[n][c] += __shfl_xor_sync(0xffffffffu, offset[n][c], o);
-                    }
-                    float* out = join + static_cast<size_t>(warp * R + n * 8 + quad * 2 + c) * (D + 2);
+                for (int c = 0; c < 2; ++c) {
+                    float* out = join + static_cast<size_t>(warp * R + n * 8 + quad * 2 + c) * kRow<D>;
+                    const float shift = c == 0 ? offset[n].x : offset[n].y;
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
                         const int word = W == 2 ? g * 2 + w : (w >> 2) * 32 + g * 4 + (w & 3);
-                        out[word * 4] = fmaf(acc[n][2 * w][c], unit, offset[n][c]);
-                        out[word * 4 + 1] = fmaf(acc[n][2 * w][2 + c], unit * 0.0625f, offset[n][c]);
-                        out[word * 4 + 2] = fmaf(acc[n][2 * w + 1][c], unit, offset[n][c]);
-                        out[word * 4 + 3] = fmaf(acc[n][2 * w + 1][2 + c], unit * 0.0625f, offset[n][c]);
+                        out[word * 4] = fmaf(acc[n][2 * w][c], unit, shift);
+                        out[word * 4 + 1] = fmaf(acc[n][2 * w][2 + c], unit * 0.0625f, shift);
+                        out[word * 4 + 2] = fmaf(acc[n][2 * w + 1][c], unit, shift);
+                        out[word * 4 + 3] = fmaf(acc[n][2 * w + 1][2 + c], unit * 0.0625f, shift);
                     }
                     if (g == 0) {
-                        out[D] = top[n][c];
-                        out[D + 1] = sum[n][c];
+                        out[D] = limit[n][c] == kNotStarted ? kNoMax : (c == 0 ? top[n].x : top[n].y);
+                        out[D + 1] = c == 0 ? sum[n].x : sum[n].y;
+                        out[D + 2] = c == 0 ? mass[n].x : mass[n].y;
                     }
                 }
             }
         }
         __syncthreads();
-        const int64_t part_first = unit_begin / per, part_last = (unit_end - 1) / per;
+        // blocks of threads that hold the first and the last part of the unit
+        const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : unit_begin / per;
+        const int64_t part_last = unit_end <= share_end ? blockIdx.x : (unit_end - 1) / per;
         const bool whole = part_first == part_last;
         const int valid_rows = req.rows - row < R ? req.rows - row : R;
-        const int64_t slot_floats = static_cast<int64_t>(R) * (D + 2);
+        const int64_t slot_floats = static_cast<int64_t>(R) * kRow<D>;
         float* partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == part_first ? 1 : 0)) * slot_floats;
         for (int i = threadIdx.x; i < valid_rows * D; i += kThreads) {
             const int r = i / D, d = i - r * D;
             float best = kNoMax;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) best = fmaxf(best, join[(w * R + r) * (D + 2) + D]);
-            float total = 0.0f, value = 0.0f;
+            for (int w = 0; w < kWarps; ++w) best = fmaxf(best, join[(w * R + r) * kRow<D> + D]);
+            float total = 0.0f, all = 0.0f, value = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float* from = join + (w * R + r) * (D + 2);
+                const float* from = join + (w * R + r) * kRow<D>;
                 const float weight = Exp2(from[D] - best);
                 total = fmaf(weight, from[D + 1], total);
+                all = fmaf(weight, from[D + 2], all);
                 value = fmaf(weight, from[d], value);
             }
             if (whole) {
-                const int query = (row + r) / p.group;
-                const int64_t q_row = req.first_row + static_cast<int64_t>(query);
-                const int q_head = head * p.group + (row + r) % p.group;
-                WriteFloat<DTYPE>(p.out, q_row * p.ldo + static_cast<int64_t>(q_head) * D + d, total == 0.0f ? 0.0f : value / total);
-                if (d == 0 && p.lse != nullptr)
-                    p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
+                StoreResult<D, DTYPE>(p, req, head, row + r, d, value, total, best, all);
             } else {
-                partial[r * (D + 2) + d] = value;
+                partial[r * kRow<D> + d] = value;
                 if (d == 0) {
-                    partial[r * (D + 2) + D] = best;
-                    partial[r * (D + 2) + D + 1] = total;
+                    partial[r * kRow<D> + D] = best;
+                    partial[r * kRow<D> + D + 1] = total;
+                    partial[r * kRow<D> + D + 2] = all;
                 }
             }
         }
         if (!whole) {
+            const int parts = static_cast<int>(part_last - part_first) + 1;
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
-                const int parts = static_cast<int>(part_last - part_first) + 1;
                 join_last = atomicAdd(&p.counters[part_first], 1) == parts - 1;
                 if (join_last) p.counters[part_first] = 0;
             }
             __syncthreads();
             if (join_last) {
                 __threadfence();
-                for (int i = threadIdx.x; i < valid_rows * D; i += kThreads) {
-                    const int r = i / D, d = i - r * D;
-                    float best = kNoMax, total = 0.0f, value = 0.0f;
-                    for (int64_t c = part_first; c <= part_last; ++c) {
-                        const float* from = p.partials + (c * 2 + (c == part_first ? 1 : 0)) * slot_floats + r * (D + 2);
-                        const float m = __ldcg(from + D), next = fmaxf(best, m);
-                        const float old = Exp2(best - next), now = Exp2(m - next);
-                        total = fmaf(now, __ldcg(from + D + 1), total * old);
-                        value = fmaf(now, __ldcg(from + d), value * old);
-                        best = next;
-                    }
-                    const int query = (row + r) / p.group;
-                    const int64_t q_row = req.first_row + static_cast<int64_t>(query);
-                    const int q_head = head * p.group + (row + r) % p.group;
-                    WriteFloat<DTYPE>(p.out, q_row * p.ldo + static_cast<int64_t>(q_head) * D + d, total == 0.0f ? 0.0f : value / total);
-                    if (d == 0 && p.lse != nullptr)
-                        p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
-                }
+                JoinParts<D, DTYPE, kThreads>(p, req, head, row, valid_rows, static_cast<int>(part_first), parts, slot_floats,
+                                              join, static_cast<int>(Layout<D, NT>::kQueries / sizeof(float)));
             }
         }
-        __syncthreads();  // the rings are free again
+        FenceProxyAsync();  // the rings' memory was written by ordinary stores; copies write it next
+        __syncthreads();
 
         at += here;
         if (at >= share_end) break;
@@ -615,11 +686,9 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                 } while (req.rows == 0);
             }
         }
-        UnitTiles<kTile>(p, req, row, R, &tile_first, &tile_last);
+        UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
     }
 }
-
-bool Aligned16Strided(const void* p, int64_t ld) { return AlignedTo(p, 16) && ld % 8 == 0; }
 
 int CheckAttention(const fth_b200_kv4_attention_desc* d) {
     if (d == nullptr) return FTH_B200_ERR_INVALID;
@@ -640,17 +709,23 @@ int CheckAttention(const fth_b200_kv4_attention_desc* d) {
     return FTH_B200_OK;
 }
 
+constexpr int kMaxGrid = 1024;
+constexpr size_t kCounterBytes = kMaxGrid * sizeof(int);
+
 // Query rows of a unit, in eights: 8 when no request has more.
 int DecodeTiles(const fth_b200_kv4_attention_desc& d) {
     return static_cast<int64_t>(d.max_query) * (d.q_heads / d.cache.kv_heads) <= 8 ? 1 : 2;
 }
 // Blocks of threads that are resident together.
-int DecodeGrid(const fth_b200_kv4_attention_desc& d) { return SmCount() * (d.cache.head_dim == 256 ? 2 : 3); }
+int DecodeGrid(const fth_b200_kv4_attention_desc& d) {
+    const int per_sm = d.cache.head_dim == 64 ? Shape<64>::kBlocksPerSm : d.cache.head_dim == 128 ? Shape<128>::kBlocksPerSm : Shape<256>::kBlocksPerSm;
+    const int grid = SmCount() * per_sm;
+    return grid < kMaxGrid ? grid : kMaxGrid;
+}
 
-constexpr size_t kCounterBytes = 4096;
 
 size_t WorkspaceBytes(const fth_b200_kv4_attention_desc& d) {
-    return kCounterBytes + static_cast<size_t>(DecodeGrid(d)) * 2 * 8 * DecodeTiles(d) * (d.cache.head_dim + 2) * sizeof(float);
+    return kCounterBytes + static_cast<size_t>(DecodeGrid(d)) * 2 * 8 * DecodeTiles(d) * (d.cache.head_dim + 4) * sizeof(float);
 }
 
 template <int D, int DTYPE>
@@ -659,7 +734,7 @@ int LaunchDecode(const AttentionParams& p, int tiles, int grid, cudaStream_t s) 
         if (EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), smem) != FTH_B200_OK) return static_cast<int>(FTH_B200_ERR_CUDA);
         return Launch(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, s, p);
     };
-    return tiles == 1 ? run(DecodeKernel<D, DTYPE, 1>, DecodeSmem<D, 1>()) : run(DecodeKernel<D, DTYPE, 2>, DecodeSmem<D, 2>());
+    return tiles == 1 ? run(DecodeKernel<D, DTYPE, 1>, Layout<D, 1>::kBytes) : run(DecodeKernel<D, DTYPE, 2>, Layout<D, 2>::kBytes);
 }
 
 }  // namespace
@@ -699,6 +774,7 @@ extern "C" int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* d, fth_
     p.group = d->q_heads / d->cache.kv_heads;
     p.causal = d->causal != 0;
     p.window = d->window;
+    p.q_vec = kv4::AlignedTo(d->q, 16) && p.ldq % 8 == 0;
     p.scale_log2 = d->scale * 1.4426950408889634f;
     p.status = DeviceStatusPtr();
     p.counters = static_cast<int*>(d->workspace);

@@ -7,7 +7,8 @@
 namespace fth {
 namespace kv4 {
 
-constexpr int kSiteAttention = 42;
+constexpr int kSiteAttention = 42, kSiteAttentionWait = 43;
+constexpr float kNoMax = -1e30f;  // the maximum of no scores: below all, and finite, so that differences stay numbers
 
 struct AttentionParams {
     Cache cache;
@@ -18,11 +19,11 @@ struct AttentionParams {
     const int32_t* table;
     const int32_t* total_lens;
     const int32_t* query_start;
-    int requests, max_blocks, max_query, kv_heads, group, causal, window;
+    int requests, max_blocks, max_query, kv_heads, group, causal, window, q_vec;
     float scale_log2;  // scale * log2(e): scores are kept as exponents of two
     int* status;
     int* counters;     // one per block of threads: arrivals of the parts of the unit that begins in it
-    float* partials;   // [block of threads][2][rows of a unit][head_dim + 2]
+    float* partials;   // [block of threads][2][rows of a unit][head_dim values, maximum, sum, sum for the lse, unused]
 };
 
 // The rows of one request and what they see.  Row i of n stands at position total - n + i.
@@ -78,6 +79,156 @@ __device__ __forceinline__ void UnitTiles(const AttentionParams& p, const Reques
     *first = l0 / TILE;
     *last = h1 > 0 ? (h1 + TILE - 1) / TILE : 0;
     if (*last <= *first) *last = *first + 1;
+}
+
+// ---- arithmetic -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void MmaF16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t Transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float Exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float Reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two FP32 operations per instruction.
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 Add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ uint32_t PackHalf(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int DTYPE>
+__device__ __forceinline__ float2 HalfPair(uint32_t x) {
+    if constexpr (DTYPE == FTH_B200_BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+__device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// Power of two that brings the largest query element to [2^14, 2^15); 24 - e stays an FP32 exponent.
+__device__ __forceinline__ int QueryExponent(float biggest) {
+    if (biggest == 0.0f) return 0;
+    const int e = 14 - (static_cast<int>((__float_as_uint(biggest) >> 23) & 0xffu) - 127);
+    return e > 120 ? 120 : e < -86 ? -86 : e;
+}
+// 2^e > biggest: shrunk by 2^(7 - e), value scales stay below 2^7 and weights with probabilities up to 2^8 below 2^15.
+__device__ __forceinline__ int ScaleExponent(float biggest) {
+    const int e = static_cast<int>((__float_as_uint(biggest) >> 23) & 0xffu) - 126;
+    return e > 120 ? 120 : e < -100 ? -100 : e;
+}
+// Eight query elements in the order a word of eight codes gives its operands: (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
+template <int DTYPE>
+__device__ __forceinline__ void QueryOperands(const uint32_t (&raw)[4], float up, uint32_t (&f)[4]) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = HalfPair<DTYPE>(raw[i]);
+        x[2 * i] = v.x * up;
+        x[2 * i + 1] = v.y * (up * 0.0625f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = PackHalf(x[i], x[i + 4]);
+}
+__device__ __forceinline__ uint4 LoadUnaligned8(const uint16_t* from) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = from[2 * i] | (static_cast<uint32_t>(from[2 * i + 1]) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Copy of `bytes` (a multiple of 16) contiguous bytes, both addresses 16-byte aligned; the bytes are reported to `bar`.
+__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(SmemAddr(dst)), "l"(src), "r"(bytes), "r"(SmemAddr(bar)) : "memory");
+}
+
+// Floats of a row of partial results.
+template <int D>
+constexpr int kRow = D + 4;
+
+// ---- results ---------------------------------------------------------------------------------------------------------------
+// Element d of row `row` of the request: value / total, and the row's lse (mass: the sum of its probabilities) with its first element.
+template <int D, int DTYPE>
+__device__ __forceinline__ void StoreResult(const AttentionParams& p, const Request& req, int head, int row, int d, float value, float total, float best, float mass) {
+    const int query = row / p.group;
+    const int64_t q_row = req.first_row + static_cast<int64_t>(query);
+    const int q_head = head * p.group + row - query * p.group;
+    rowops::WriteFloat<DTYPE>(p.out, q_row * p.ldo + static_cast<int64_t>(q_head) * D + d, total == 0.0f ? 0.0f : __fdividef(value, total));
+    if (d == 0 && p.lse != nullptr)
+        p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(mass)) * 0.6931471805599453f;
+}
+// Joins the parts of a unit, in order: part i is slot 1 of block `first` for i = 0 and slot 0 of block first + i behind it.
+// Every part's weight is computed once into shared memory; the values are then read with nothing waiting for another.
+template <int D, int DTYPE, int THREADS>
+__device__ __forceinline__ void JoinParts(const AttentionParams& p, const Request& req, int head, int row, int rows, int first, int parts,
+                                          int64_t slot_floats, float* shared, int shared_floats) {
+    const float* base = p.partials + (static_cast<int64_t>(first) * 2 + 1) * slot_floats;  // part i > 0 lies 2 i - 1 slots behind
+    const auto slot = [&](int i) { return base + (i == 0 ? 0 : 2 * static_cast<int64_t>(i) - 1) * slot_floats; };
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float* weights = shared;                    // [rows][parts]
+    float* best_of = shared + rows * parts;     // [rows] maximum, [rows] sum, [rows] sum for the lse
+    if (static_cast<int64_t>(rows) * (parts + 3) > shared_floats) return;  // cannot be: the host sizes shared memory for it
+    __syncthreads();
+    for (int r = warp; r < rows; r += THREADS / 32) {
+        float best = kNoMax;
+        for (int i = lane; i < parts; i += 32) best = fmaxf(best, __ldcg(slot(i) + r * kRow<D> + D));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+        float total = 0.0f, mass = 0.0f;
+        for (int i = lane; i < parts; i += 32) {
+            const float w = Exp2(__ldcg(slot(i) + r * kRow<D> + D) - best);
+            weights[r * parts + i] = w;
+            total = fmaf(w, __ldcg(slot(i) + r * kRow<D> + D + 1), total);
+            mass = fmaf(w, __ldcg(slot(i) + r * kRow<D> + D + 2), mass);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, o);
+            mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        }
+        if (lane == 0) {
+            best_of[r] = best;
+            best_of[rows + r] = total;
+            best_of[2 * rows + r] = mass;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * D; i += THREADS) {
+        const int r = i / D, d = i - r * D;
+        float value = 0.0f;
+#pragma unroll 8
+        for (int c = 0; c < parts; ++c) value = fmaf(weights[r * parts + c], __ldcg(slot(c) + r * kRow<D> + d), value);
+        StoreResult<D, DTYPE>(p, req, head, row + r, d, value, best_of[rows + r], best_of[r], best_of[2 * rows + r]);
+    }
 }
 
 }  // namespace kv4
