@@ -10,9 +10,10 @@
 //
 // S^T = K q^T: tokens are the 16 rows of the instruction, query rows its 8 columns, so a group of up to eight query
 // heads fills it and the products of one K word serve all of them.  O^T = V^T P^T likewise: head elements are its rows.
-// P^T comes from S^T by transposing 8 x 8 tiles within the warp.  A warp streams its tokens, 64 at a time (32 for wide
-// heads), through a ring of its own with bulk copies: a block's codes of one head are contiguous, and every lane finds
-// the words it multiplies 16 bytes apart from its neighbours'.  No barrier between warps.
+// P^T comes from S^T by transposing 8 x 8 tiles within the warp.  One warp of a block of threads streams the tokens of its
+// share through a ring in shared memory with bulk copies (a block's codes of one head are contiguous), also across units,
+// so that the next unit's tokens fly while this one's results are joined; four warps compute, each on its 32 or 64 tokens
+// of every tile, and every lane finds the words it multiplies 16 bytes apart from its neighbours'.
 //
 // A weight p s rounded to FP16 (11 bits) stands for the probability in all three sums of the result: the weighted codes, the
 // sum of minima and the sum that divides them (weight / s gives the probability back), so a rounding moves the result by
@@ -25,6 +26,7 @@
 //
 // Bound: cache bytes, tokens * (head_dim + 8) per kv head.
 #include "kv4_attention.cuh"
+#include "kv4_prefill.h"
 
 namespace fth {
 namespace kv4 {
@@ -33,36 +35,39 @@ namespace {
 
 using namespace rowops;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr float kLazy = 8.0f;         // a running maximum may lag by 2^8 before sums are rescaled
-constexpr float kNotStarted = -3e38f;
+constexpr int kWarps = 4;                         // that compute; one more copies
+constexpr int kCompute = kWarps * 32;
+constexpr int kThreads = kCompute + 32;
+constexpr int kMinShare = 4;                      // tiles; below, cutting a unit costs more than it saves
 
 template <int D>
 struct Shape {
     static constexpr int kWords = D / 32;                 // packed words a lane holds of a token (K) or of a pair of tokens (V)
-    static constexpr int kStep = D == 256 ? 32 : 64;      // tokens of a stage
+    static constexpr int kStep = D == 64 ? 64 : 32;       // tokens of a warp
     static constexpr int kSubs = kStep / 16;
-    static constexpr int kStages = D == 128 ? 2 : 3;
-    static constexpr int kTile = kWarps * kStep;
-    // a stage: K codes, V codes, K parameters, V parameters
-    static constexpr int kCodeBytes = kStep * D / 2;
-    static constexpr int kStageBytes = 2 * kCodeBytes + 2 * kStep * 4;
-    static constexpr int kRingBytes = kStages * kStageBytes;
-    static constexpr int kBlocksPerSm = D == 256 ? 2 : 3;
+    static constexpr int kStages = D == 256 ? 2 : 3;
+    static constexpr int kTile = kWarps * kStep;          // tokens of a stage: K codes, V codes, K parameters, V parameters
+    static constexpr int kCodeBytes = kTile * D / 2;
+    static constexpr int kStageBytes = 2 * kCodeBytes + 2 * kTile * 4;
 };
+// Blocks of threads that share an SM; registers per thread follow from it.
+template <int D, int NT>
+constexpr int kBlocksPerSm = D == 256 || NT == 2 ? 2 : 3;
 
 template <int D, int NT>
 constexpr bool kQueriesInShared = D == 256 && NT == 2;   // 64 registers of fragments would not fit beside 128 accumulators
 
-// Dynamic shared memory: the warps' rings, in whose place their results are joined, then query operands.
+// Dynamic shared memory: the ring, the place where the warps' results are joined, then query operands.
 template <int D, int NT>
 struct Layout {
-    static constexpr size_t kRings = static_cast<size_t>(kWarps) * Shape<D>::kRingBytes;
-    static constexpr size_t kJoin = static_cast<size_t>(kWarps) * 8 * NT * kRow<D> * sizeof(float);
-    static constexpr size_t kQueries = kRings > kJoin ? kRings : (kJoin + 15) / 16 * 16;
+    static constexpr size_t kJoin = static_cast<size_t>(Shape<D>::kStages) * Shape<D>::kStageBytes;
+    static constexpr size_t kJoinFloats = static_cast<size_t>(kWarps) * 8 * NT * kRow<D>;
+    static constexpr size_t kQueries = kJoin + kJoinFloats * sizeof(float);
     static constexpr size_t kBytes = kQueries + (kQueriesInShared<D, NT> ? NT * Shape<D>::kWords * 32 * 16 : 0);
 };
+
+// Barrier of the warps that compute.
+__device__ __forceinline__ void ComputeSync() { asm volatile("bar.sync 1, %0;" ::"n"(kCompute) : "memory"); }
 
 // Sum of v over the block, and the sum over the threads before this one.
 __device__ __forceinline__ int64_t ScanWork(int64_t v, int64_t* shared, int64_t* total) {
@@ -78,7 +83,7 @@ __device__ __forceinline__ int64_t ScanWork(int64_t v, int64_t* shared, int64_t*
     __syncthreads();
     int64_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) before += shared[w];
         all += shared[w];
     }
@@ -115,24 +120,31 @@ __device__ __forceinline__ void LoadChunk(const uint8_t* row, int place, int chu
 }
 
 template <int D, int DTYPE, int NT>
-__global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(const __grid_constant__ AttentionParams p) {
     using T = Shape<D>;
     constexpr int W = T::kWords;
     constexpr int CW = W == 2 ? 2 : 4;        // words of a chunk
     constexpr int S = T::kStages;
     constexpr int R = 8 * NT;
     constexpr bool QS = kQueriesInShared<D, NT>;
+    constexpr int I = 2;   // sixteens of tokens worked on together
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scan[kWarps];
+    __shared__ int64_t scan[kThreads / 32];
     __shared__ Request start_req;
     __shared__ int start_request;
     __shared__ int64_t start_offset, start_per_head;
     __shared__ int join_last;
-    __shared__ __align__(8) uint64_t bars[kWarps * S];
+    __shared__ __align__(8) uint64_t full[S], empty[S];
+    __shared__ uint32_t stage_present[S];   // a bit for every 16 tokens of the stage that are there
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, quad = lane & 3;
-    if (lane < S) MbarInit(&bars[warp * S + lane], 1);
-    FenceBarrierInit();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            MbarInit(&full[i], 1);
+            MbarInit(&empty[i], kWarps);
+        }
+        FenceBarrierInit();
+    }
     WaitForPrevious();
 
     // ---- this block's share of the tiles --------------------------------------------------------------------------------
@@ -151,7 +163,7 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
         work += total;
     }
     int64_t per = (work + gridDim.x - 1) / gridDim.x;
-    if (per < 2) per = 2;
+    if (per < kMinShare) per = kMinShare;
     const int64_t share_begin = blockIdx.x * per;
     const int64_t share_end = share_begin + per < work ? share_begin + per : work;
     if (share_begin >= share_end) return;
@@ -193,69 +205,115 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
         row += R;
     }
     int64_t at = share_begin;
-    uint8_t* ring = smem + warp * T::kRingBytes;
-    uint64_t* bar = bars + warp * S;
-    uint32_t phases = 0;   // parity of each stage's next completion
+    int t0, steps, first_low, last_high;   // of this block's part of the unit
+    const auto place = [&] {
+        const int64_t left = share_end - at, tiles = tile_last - tile_first - into;
+        t0 = tile_first + static_cast<int>(into);
+        steps = static_cast<int>(tiles < left ? tiles : left);
+        int unused;
+        Visible(p, req, row / p.group, &first_low, &unused);
+        Visible(p, req, ((row + R < req.rows ? row + R : req.rows) - 1) / p.group, &unused, &last_high);
+    };
+    const auto next_unit = [&] {   // false: the share is done
+        at += steps;
+        if (at >= share_end) return false;
+        into = 0;
+        row += R;
+        if (row >= req.rows) {
+            row = 0;
+            if (++head == p.kv_heads) {
+                head = 0;
+                do {
+                    ++b;
+                    req = LoadRequest(p, b);
+                } while (req.rows == 0);
+            }
+        }
+        UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
+        place();
+        return true;
+    };
+    place();
+    int stage = 0;
+    uint32_t phase = 0;
     bool failed = false;
+
+    if (warp == kWarps) {
+        // ---- copies: lane = 4 * (16 tokens) + (K codes, V codes, K parameters, V parameters) ----------------------------------
+        // Blocks of more than 16 tokens are copied by the lanes of their first 16, up to a whole tile at once.
+        constexpr int kRounds = T::kTile / 128;
+        constexpr int kTileShift = T::kTile == 256 ? 8 : 7;
+        const int span_shift = p.cache.block_shift < kTileShift ? p.cache.block_shift : kTileShift;
+        const int span = 1 << span_shift;
+        int id[kRounds];
+        int64_t issued = 0;
+        do {
+            const int32_t* table = p.table + static_cast<int64_t>(b) * p.max_blocks;
+            const auto lookup = [&](int step) {
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) {
+                    const int in_tile = r * 128 + (lane >> 2) * 16;
+                    const int token = (t0 + step) * T::kTile + in_tile;
+                    id[r] = -2;
+                    if (step < steps && (in_tile & (span - 1)) == 0 && token < last_high && token + span > first_low)
+                        id[r] = table[token >> p.cache.block_shift];
+                }
+            };
+            lookup(0);
+            for (int step = 0; step < steps; ++step) {
+                if (issued >= S && !failed && !MbarWait(&empty[stage], phase ^ 1u, p.status, kSiteAttentionWait, stage)) failed = true;
+                uint32_t there = 0;
+                int copies = 0;
+                bool good[kRounds];
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) {
+                    good[r] = id[r] >= 0 && id[r] < p.cache.blocks;
+                    if (id[r] != -2 && !good[r] && quad == 0) ReportTimeout(p.status, kSiteAttention, b);
+                    const uint32_t who = __ballot_sync(0xffffffffu, good[r]);
+                    copies += __popc(who & 0x11111111u);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) there |= ((who >> (4 * i)) & 1u) << (r * 8 + i);
+                }
+                for (int sh = 1; sh < (span >> 4); sh <<= 1) there |= there << sh;   // a span's later sixteens
+                if (lane == 0) {
+                    stage_present[stage] = there;
+                    MbarExpectTx(&full[stage], static_cast<uint32_t>(copies) * span * (D + 8));
+                }
+                __syncwarp();
+                uint8_t* dst = smem + stage * T::kStageBytes;
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) {
+                    if (good[r] && !failed) {
+                        const int in_tile = r * 128 + (lane >> 2) * 16;
+                        const int64_t from = HeadBase(p.cache, id[r], head) + (((t0 + step) * T::kTile + in_tile) & ((1 << p.cache.block_shift) - 1));
+                        if (quad < 2) {
+                            BulkLoad(dst + quad * T::kCodeBytes + in_tile * (D / 2), (quad == 0 ? p.cache.k_codes : p.cache.v_codes) + from * (D / 2),
+                                     span * (D / 2), &full[stage]);
+                        } else {
+                            BulkLoad(dst + 2 * T::kCodeBytes + (quad - 2) * (T::kTile * 4) + in_tile * 4,
+                                     (quad == 2 ? p.cache.k_params : p.cache.v_params) + from, span * 4, &full[stage]);
+                        }
+                    }
+                }
+                lookup(step + 1);
+                ++issued;
+                if (++stage == S) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        } while (next_unit());
+        return;
+    }
 
     for (;;) {
         const int64_t unit_begin = at - into;
         const int64_t unit_end = unit_begin + (tile_last - tile_first);
-        const int t0 = tile_first + static_cast<int>(into);
-        const int64_t here = (unit_end < share_end ? unit_end : share_end) - at;
-        const int steps = static_cast<int>(here);
-        int first_low, last_high, unused;
-        Visible(p, req, row / p.group, &first_low, &unused);
-        Visible(p, req, ((row + R < req.rows ? row + R : req.rows) - 1) / p.group, &unused, &last_high);
-
-        // ---- copies: lane = 4 * (16 tokens) + (K codes, V codes, K parameters, V parameters) ----------------------------------
-        // Blocks of more than 16 tokens are copied by the lanes of their first 16, up to a whole step at once.
-        const int32_t* table = p.table + static_cast<int64_t>(b) * p.max_blocks;
-        const int span_shift = p.cache.block_shift < (T::kStep == 64 ? 6 : 5) ? p.cache.block_shift : (T::kStep == 64 ? 6 : 5);
-        const int sub = lane >> 2;
-        const bool copies = lane < 4 * T::kSubs && ((sub << 4) & ((1 << span_shift) - 1)) == 0;
-        uint32_t have = 0;   // kSubs bits per stage: these 16 tokens are there
-        int id = -2;
-        const auto lookup = [&](int step) {
-            const int token = (t0 + step) * T::kTile + warp * T::kStep + sub * 16;
-            id = -2;
-            if (copies && step < steps && token < last_high && token + (1 << span_shift) > first_low) id = table[token >> p.cache.block_shift];
-        };
-        const auto issue = [&](int step) {
-            const int stage = step % S;
-            const bool good = id >= 0 && id < p.cache.blocks;
-            if (id != -2 && !good && quad == 0) ReportTimeout(p.status, kSiteAttention, b);
-            const uint32_t who = __ballot_sync(0xffffffffu, good);
-            uint32_t there = 0;
-#pragma unroll
-            for (int i = 0; i < T::kSubs; ++i) there |= ((who >> (4 * (((i << 4) >> span_shift) << (span_shift - 4)))) & 1u) << i;
-            have = (have & ~(((1u << T::kSubs) - 1) << (T::kSubs * stage))) | (there << (T::kSubs * stage));
-            if (lane == 0) MbarExpectTx(&bar[stage], static_cast<uint32_t>(__popc(who)) * (1u << span_shift) * (D + 8) / 4);
-            __syncwarp();
-            if (good) {
-                const int token = (t0 + step) * T::kTile + warp * T::kStep + sub * 16;
-                const int64_t from = HeadBase(p.cache, id, head) + (token & ((1 << p.cache.block_shift) - 1));
-                uint8_t* dst = ring + stage * T::kStageBytes;
-                if (quad < 2) {
-                    BulkLoad(dst + quad * T::kCodeBytes + sub * (16 * D / 2), (quad == 0 ? p.cache.k_codes : p.cache.v_codes) + from * (D / 2),
-                             (1u << span_shift) * (D / 2), &bar[stage]);
-                } else {
-                    BulkLoad(dst + 2 * T::kCodeBytes + (quad - 2) * (T::kStep * 4) + sub * 64, (quad == 2 ? p.cache.k_params : p.cache.v_params) + from,
-                             (1u << span_shift) * 4, &bar[stage]);
-                }
-            }
-        };
-        lookup(0);
-#pragma unroll
-        for (int s = 0; s < S - 1; ++s) {
-            issue(s);
-            lookup(s + 1);
-        }
 
         // ---- query rows ----------------------------------------------------------------------------------------------------
         uint32_t qf[QS ? 1 : NT][2 * W][2];
         uint4* const q_shared = reinterpret_cast<uint4*>(smem + Layout<D, NT>::kQueries);
-        float2 qsum[NT];   // of the columns 2 * quad, 2 * quad + 1
+        float qsum[NT][2];   // of the columns 2 * quad, 2 * quad + 1
         int row_low[NT][2], row_high[NT][2];
         int all_low = 0, all_high = 0x7fffffff;
         float back;
@@ -299,8 +357,8 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                     }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qsum[n].x = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8);
-                qsum[n].y = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8 + 4);
+                qsum[n][0] = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8);
+                qsum[n][1] = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8 + 4);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     row_low[n][c] = __shfl_sync(0xffffffffu, low, quad * 8 + c * 4);
@@ -334,12 +392,12 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                     }
                 }
             }
-            if constexpr (QS) __syncthreads();
+            if constexpr (QS) ComputeSync();
         }
 
         // ---- tokens -----------------------------------------------------------------------------------------------------------
         float acc[NT][2 * W][4];
-        float2 top[NT], sum[NT], mass[NT], offset[NT];   // top: the running maximum; scores are kept relative to it
+        float top[NT][2], sum[NT][2], mass[NT][2], offset[NT][2];   // top: the running maximum; scores are kept relative to it
         float limit[NT][2];                    // a relative score above it moves the maximum
         float shrink = 1.0f;                   // value scales are multiplied by this power of two before they become FP16
         float scale_limit = 0.0f;
@@ -349,40 +407,33 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
             for (int m = 0; m < 2 * W; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.0f;
-            top[n] = sum[n] = mass[n] = offset[n] = make_float2(0.0f, 0.0f);
-            limit[n][0] = limit[n][1] = kNotStarted;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                top[n][c] = sum[n][c] = mass[n][c] = offset[n][c] = 0.0f;
+                limit[n][c] = kNotStarted;
+            }
         }
         for (int step = 0; step < steps; ++step) {
-            const int stage = step % S;
-            if (!failed && !MbarWait(&bar[stage], (phases >> stage) & 1u, p.status, kSiteAttentionWait, stage)) failed = true;
-            phases ^= 1u << stage;
-            __syncwarp();  // every lane is done with the stage that is filled next
-            issue(step + S - 1);
-            lookup(step + S);
-            const uint8_t* data = ring + stage * T::kStageBytes;
-            const uint32_t* k_params = reinterpret_cast<const uint32_t*>(data + 2 * T::kCodeBytes);
-            const uint32_t* v_params = k_params + T::kStep;
-            const uint32_t present_all = (have >> (T::kSubs * stage)) & ((1u << T::kSubs) - 1);
+            if (!failed && !MbarWait(&full[stage], phase, p.status, kSiteAttentionWait, S + stage)) failed = true;
+            const uint8_t* data = smem + stage * T::kStageBytes + warp * (T::kStep * D / 2);
+            const uint32_t* k_params = reinterpret_cast<const uint32_t*>(smem + stage * T::kStageBytes + 2 * T::kCodeBytes) + warp * T::kStep;
+            const uint32_t* v_params = k_params + T::kTile;
+            const uint32_t present_all = failed ? 0u : stage_present[stage] >> (T::kSubs * warp);
 #pragma unroll 1
-            for (int half = 0; half < T::kSubs / 2; ++half) {   // 32 tokens
-                const uint32_t present = (present_all >> (2 * half)) & 3u;
+            for (int part = 0; part < T::kSubs / I; ++part) {   // 16 * I tokens
+                const uint32_t present = (present_all >> (I * part)) & ((1u << I) - 1);
                 if (present == 0) continue;
-                const int token0 = (t0 + step) * T::kTile + warp * T::kStep + half * 32;
-                const uint8_t* k_rows = data + half * (32 * D / 2);
+                const int place0 = part * (16 * I);
+                const int token0 = (t0 + step) * T::kTile + warp * T::kStep + place0;
+                const uint8_t* k_rows = data + place0 * (D / 2);
                 const uint8_t* v_rows = k_rows + T::kCodeBytes;
 
                 // q . c
-                float z[2][NT][4];
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) z[s][n][i] = 0.0f;
+                float z[I][NT][4];
 #pragma unroll
                 for (int c = 0; c < W / CW; ++c) {
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
+                    for (int s = 0; s < I; ++s) {
                         uint32_t k0[4], k1[4];
                         LoadChunk<W, 64>(k_rows + (s * 16 + g) * (D / 2), quad, c, k0);
                         LoadChunk<W, 64>(k_rows + (s * 16 + 8 + g) * (D / 2), quad, c, k1);
@@ -395,60 +446,75 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                                 uint4 f;
                                 if constexpr (QS) f = q_shared[(n * W + w) * 32 + lane];
                                 else f = make_uint4(qf[n][2 * w][0], qf[n][2 * w][1], qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
-                                MmaF16(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, f.x, f.y);
+                                if (w == 0) MmaF16First(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, f.x, f.y);
+                                else MmaF16(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, f.x, f.y);
                                 MmaF16(z[s][n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, f.z, f.w);
                             }
                         }
                     }
                 }
                 // scores, exponents of two, relative to the running maximum
-                const bool inside = token0 >= all_low && token0 + 32 <= all_high && present == 3u;
-                float vs[2][2], vm[2][2];
-                bool rescale = false;
+                const bool inside = token0 >= all_low && token0 + 16 * I <= all_high && present == (1u << I) - 1;
+                float best[NT][2];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
+                for (int n = 0; n < NT; ++n) best[n][0] = best[n][1] = -INFINITY;
+#pragma unroll
+                for (int s = 0; s < I; ++s) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int place = half * 32 + s * 16 + h * 8 + g;
-                        const uint32_t kp = k_params[place], vp = v_params[place];
+                        const uint32_t kp = k_params[place0 + s * 16 + h * 8 + g];
                         const float ks = ParamScale(kp) * back, km = ParamMin(kp);
-                        vs[s][h] = ParamScale(vp);
-                        vm[s][h] = ParamMin(vp);
-                        bool seen_by_any = inside;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            float2 t = Fma2(make_float2(km, km), qsum[n], make_float2(-top[n].x, -top[n].y));
-                            t = Fma2(make_float2(ks, ks), make_float2(z[s][n][2 * h], z[s][n][2 * h + 1]), t);
-                            if (!inside) {
-                                const int token = token0 + s * 16 + h * 8 + g;
-                                const bool there = ((present >> s) & 1u) != 0;
-                                const bool seen0 = there && token >= row_low[n][0] && token < row_high[n][0];
-                                const bool seen1 = there && token >= row_low[n][1] && token < row_high[n][1];
-                                if (!seen0) t.x = -INFINITY;
-                                if (!seen1) t.y = -INFINITY;
-                                seen_by_any = seen_by_any || seen0 || seen1;
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                float& score = z[s][n][2 * h + c];
+                                score = fmaf(ks, score, fmaf(km, qsum[n][c], -top[n][c]));
                             }
-                            z[s][n][2 * h] = t.x;
-                            z[s][n][2 * h + 1] = t.y;
                         }
-                        if (!seen_by_any) vs[s][h] = vm[s][h] = 0.0f;  // whatever stands there: 0 * NaN is no zero
-                        rescale = rescale || vs[s][h] > scale_limit;
                     }
                 }
+                // value scales of these tokens, as bits (positive numbers order like their bits; NaN counts as the largest)
+                uint32_t scale_bits = v_params[place0 + lane] << 16;
+                if (!inside) {
+                    bool lane_seen = false;   // of the token whose scale this lane holds
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float best0 = fmaxf(fmaxf(z[0][n][0], z[0][n][2]), fmaxf(z[1][n][0], z[1][n][2]));
-                    const float best1 = fmaxf(fmaxf(z[0][n][1], z[0][n][3]), fmaxf(z[1][n][1], z[1][n][3]));
-                    rescale = rescale || best0 > limit[n][0] || best1 > limit[n][1];
+                    for (int s = 0; s < I; ++s) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int token = token0 + s * 16 + h * 8 + g;
+                            const bool there = ((present >> s) & 1u) != 0;
+                            bool any = false;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    const bool seen = there && token >= row_low[n][c] && token < row_high[n][c];
+                                    if (!seen) z[s][n][2 * h + c] = -INFINITY;
+                                    any = any || seen;
+                                }
+                            }
+                            // columns of all four lanes of a token, then bit = token within these 32
+                            const uint32_t who = __ballot_sync(0xffffffffu, any);
+                            const int mine_at = lane - (s * 16 + h * 8);
+                            if (mine_at >= 0 && mine_at < 8) lane_seen = ((who >> (4 * mine_at)) & 15u) != 0;
+                        }
+                    }
+                    if (!lane_seen) scale_bits = 0;
                 }
+                const uint32_t scale_top = __reduce_max_sync(0xffffffffu, scale_bits), scale_low = __reduce_min_sync(0xffffffffu, scale_bits);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int s = 0; s < I; ++s) best[n][c] = fmaxf(best[n][c], fmaxf(z[s][n][c], z[s][n][2 + c]));
+                float biggest = __uint_as_float(scale_top);
+                if (!(biggest < INFINITY)) biggest = scale_limit;   // NaN: the weights show it
+                bool rescale = biggest > scale_limit;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) rescale = rescale || best[n][0] > limit[n][0] || best[n][1] > limit[n][1];
                 if (__any_sync(0xffffffffu, rescale)) {
-                    float biggest = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) biggest = fmaxf(biggest, vs[s][h]);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) biggest = fmaxf(biggest, __shfl_xor_sync(0xffffffffu, biggest, o));
                     float change = 1.0f;
                     if (biggest > scale_limit) {
                         const int e = ScaleExponent(biggest);
@@ -459,74 +525,70 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float2 moved, alpha;
+                        float moved[2], factor[2];
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float best = fmaxf(fmaxf(z[0][n][c], z[0][n][2 + c]), fmaxf(z[1][n][c], z[1][n][2 + c]));
+                            float m = best[n][c];
 #pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+                            for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                             const bool first = limit[n][c] == kNotStarted;
-                            const bool move = first ? best > kNotStarted : best > 0.0f;
-                            const float by = move ? best : 0.0f;
+                            const bool move = first ? m > kNotStarted : m > 0.0f;
+                            moved[c] = move ? m : 0.0f;
                             if (move) limit[n][c] = kLazy;
                             // before the first score the sums are zeros (or NaN, which stay)
-                            (c == 0 ? alpha.x : alpha.y) = first ? 0.0f : Exp2(-by);
-                            (c == 0 ? moved.x : moved.y) = by;
+                            const float alpha = first ? 0.0f : Exp2(-moved[c]);
+                            factor[c] = alpha * change;
+                            top[n][c] += moved[c];
+                            sum[n][c] *= alpha;
+                            mass[n][c] *= alpha;
+                            offset[n][c] *= alpha;
                         }
-                        top[n].x += moved.x;
-                        top[n].y += moved.y;
-                        sum[n] = Mul2(sum[n], alpha);
-                        mass[n] = Mul2(mass[n], alpha);
-                        offset[n] = Mul2(offset[n], alpha);
-                        const float2 factor = make_float2(alpha.x * change, alpha.y * change);
 #pragma unroll
                         for (int m = 0; m < 2 * W; ++m) {
-                            acc[n][m][0] *= factor.x;
-                            acc[n][m][1] *= factor.y;
-                            acc[n][m][2] *= factor.x;
-                            acc[n][m][3] *= factor.y;
+                            acc[n][m][0] *= factor[0];
+                            acc[n][m][1] *= factor[1];
+                            acc[n][m][2] *= factor[0];
+                            acc[n][m][3] *= factor[1];
                         }
 #pragma unroll
-                        for (int s = 0; s < 2; ++s)
+                        for (int s = 0; s < I; ++s)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) z[s][n][i] -= (i & 1) ? moved.y : moved.x;
+                            for (int i = 0; i < 4; ++i) z[s][n][i] -= moved[i & 1];
                     }
                 }
                 // probabilities, weights, weighted values
-                bool plain = !inside;
+                const bool plain = !inside || !(__uint_as_float(scale_low) * shrink >= 1.0f) || !(__uint_as_float(scale_top) < INFINITY);
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                for (int s = 0; s < I; ++s) {
+                    uint32_t pt[NT][2];
+                    float vs[2], vm[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        vs[s][h] *= shrink;
-                        plain = plain || !(vs[s][h] >= 1.0f);
+                        const uint32_t vp = v_params[place0 + s * 16 + h * 8 + g];
+                        vs[h] = ParamScale(vp) * shrink;
+                        vm[h] = ParamMin(vp);
                     }
-                plain = __any_sync(0xffffffffu, plain);
-                uint32_t pt[2][NT][2];
-                if (!plain) {
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
+                    if (!plain) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float inverse = Reciprocal(vs[s][h]);
-                            const float ratio = vm[s][h] * inverse;
+                            const float inverse = Reciprocal(vs[h]), ratio = vm[h] * inverse;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                float2 w = make_float2(Exp2(z[s][n][2 * h]), Exp2(z[s][n][2 * h + 1]));
-                                mass[n] = Add2(mass[n], w);
-                                w = Mul2(w, make_float2(vs[s][h], vs[s][h]));
-                                const uint32_t packed = PackHalf(w.x, w.y);
-                                w = HalfPair<FTH_B200_FP16>(packed);
-                                sum[n] = Fma2(w, make_float2(inverse, inverse), sum[n]);
-                                offset[n] = Fma2(w, make_float2(ratio, ratio), offset[n]);
-                                pt[s][n][h] = Transpose8x8(packed);
+                                const float p0 = Exp2(z[s][n][2 * h]), p1 = Exp2(z[s][n][2 * h + 1]);
+                                mass[n][0] += p0;
+                                mass[n][1] += p1;
+                                const uint32_t packed = PackHalf(p0 * vs[h], p1 * vs[h]);
+                                const float2 w = HalfPair<FTH_B200_FP16>(packed);
+                                sum[n][0] = fmaf(w.x, inverse, sum[n][0]);
+                                sum[n][1] = fmaf(w.y, inverse, sum[n][1]);
+                                offset[n][0] = fmaf(w.x, ratio, offset[n][0]);
+                                offset[n][1] = fmaf(w.y, ratio, offset[n][1]);
+                                pt[n][h] = Transpose8x8(packed);
                             }
                         }
-                    }
-                } else {
-                    // masked tokens, and value scales too small beside the largest to give the probability back
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
+                    } else {
+                        // hidden tokens (whatever stands there: 0 * NaN is no zero), and value scales too small beside the
+                        // largest for a weight to give the probability back
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -534,31 +596,23 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                                 float w[2];
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    const float zc = z[s][n][2 * h + c];
-                                    const bool hidden = zc == -INFINITY;
-                                    const float prob = Exp2(zc);
-                                    const float weight = hidden ? 0.0f : prob * vs[s][h];
-                                    float& sum_c = c == 0 ? sum[n].x : sum[n].y;
-                                    float& mass_c = c == 0 ? mass[n].x : mass[n].y;
-                                    float& offset_c = c == 0 ? offset[n].x : offset[n].y;
-                                    const float rounded = __half2float(__float2half_rn(weight));
-                                    const float kept = vs[s][h] >= 1.0f ? rounded * Reciprocal(vs[s][h]) : prob;
+                                    const float score = z[s][n][2 * h + c];
+                                    const bool hidden = score == -INFINITY;
+                                    const float prob = Exp2(score);
+                                    w[c] = hidden ? 0.0f : __half2float(__float2half_rn(prob * vs[h]));
+                                    const float kept = vs[h] >= 1.0f ? w[c] * Reciprocal(vs[h]) : prob;
                                     if (!hidden) {
-                                        sum_c += kept;
-                                        mass_c += prob;
-                                        offset_c = fmaf(kept, vm[s][h], offset_c);
+                                        mass[n][c] += prob;
+                                        sum[n][c] += kept;
+                                        offset[n][c] = fmaf(kept, vm[h], offset[n][c]);
                                     }
-                                    w[c] = rounded;
                                 }
-                                pt[s][n][h] = Transpose8x8(PackHalf(w[0], w[1]));
+                                pt[n][h] = Transpose8x8(PackHalf(w[0], w[1]));
                             }
                         }
                     }
-                }
 #pragma unroll
-                for (int c = 0; c < W / CW; ++c) {
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
+                    for (int c = 0; c < W / CW; ++c) {
                         uint32_t v0[4], v1[4];
                         LoadChunk<W, 128>(v_rows + (s * 8 + quad) * D, g, c, v0);
                         LoadChunk<W, 128>(v_rows + (s * 8 + 4 + quad) * D, g, c, v1);
@@ -568,42 +622,38 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                             const uint32_t x0 = v0[i], x1 = v1[i], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                MmaF16(acc[n][2 * w], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, pt[s][n][0], pt[s][n][1]);
-                                MmaF16(acc[n][2 * w + 1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, pt[s][n][0], pt[s][n][1]);
+                                MmaF16(acc[n][2 * w], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu, x1 & 0x00f000f0u, pt[n][0], pt[n][1]);
+                                MmaF16(acc[n][2 * w + 1], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u, pt[n][0], pt[n][1]);
                             }
                         }
                     }
                 }
             }
-        }
-        // the stages issued beyond the last step carry no bytes; their phases are passed all the same
-        for (int step = steps; step < steps + S - 1; ++step) {
-            const int stage = step % S;
-            if (!failed && !MbarWait(&bar[stage], (phases >> stage) & 1u, p.status, kSiteAttentionWait, stage)) failed = true;
-            phases ^= 1u << stage;
+            __syncwarp();
+            if (lane == 0) MbarArrive(&empty[stage]);
+            if (++stage == S) {
+                stage = 0;
+                phase ^= 1u;
+            }
         }
 
-        // ---- the four warps' results together ---------------------------------------------------------------------------------
-        // [warp][row][D values, maximum, sum, sum for the lse], in the rings' memory
-        float* join = reinterpret_cast<float*>(smem);
-        __syncthreads();
+        // ---- the four warps' results together: [warp][row][D values, maximum, unused, sum, sum for the lse] ---------------------------
+        float* join = reinterpret_cast<float*>(smem + Layout<D, NT>::kJoin);
+        ComputeSync();
         {
             const float unit = PowerOfTwo(24) / shrink;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    sum[n].x += __shfl_xor_sync(0xffffffffu, sum[n].x, o);
-                    sum[n].y += __shfl_xor_sync(0xffffffffu, sum[n].y, o);
-                    mass[n].x += __shfl_xor_sync(0xffffffffu, mass[n].x, o);
-                    mass[n].y += __shfl_xor_sync(0xffffffffu, mass[n].y, o);
-                    offset[n].x += __shfl_xor_sync(0xffffffffu, offset[n].x, o);
-                    offset[n].y += __shfl_xor_sync(0xffffffffu, offset[n].y, o);
-                }
-#pragma unroll
                 for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
+                        mass[n][c] += __shfl_xor_sync(0xffffffffu, mass[n][c], o);
+                        offset[n][c] += __shfl_xor_sync(0xffffffffu, offset[n][c], o);
+                    }
                     float* out = join + static_cast<size_t>(warp * R + n * 8 + quad * 2 + c) * kRow<D>;
-                    const float shift = c == 0 ? offset[n].x : offset[n].y;
+                    const float shift = offset[n][c];
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
                         const int word = W == 2 ? g * 2 + w : (w >> 2) * 32 + g * 4 + (w & 3);
@@ -613,14 +663,14 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
                         out[word * 4 + 3] = fmaf(acc[n][2 * w + 1][2 + c], unit * 0.0625f, shift);
                     }
                     if (g == 0) {
-                        out[D] = limit[n][c] == kNotStarted ? kNoMax : (c == 0 ? top[n].x : top[n].y);
-                        out[D + 1] = c == 0 ? sum[n].x : sum[n].y;
-                        out[D + 2] = c == 0 ? mass[n].x : mass[n].y;
+                        out[D] = limit[n][c] == kNotStarted ? kNoMax : top[n][c];
+                        out[D + 2] = sum[n][c];
+                        out[D + 3] = mass[n][c];
                     }
                 }
             }
         }
-        __syncthreads();
+        ComputeSync();
         // blocks of threads that hold the first and the last part of the unit
         const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : unit_begin / per;
         const int64_t part_last = unit_end <= share_end ? blockIdx.x : (unit_end - 1) / per;
@@ -628,65 +678,44 @@ __global__ void __launch_bounds__(kThreads) DecodeKernel(const __grid_constant__
         const int valid_rows = req.rows - row < R ? req.rows - row : R;
         const int64_t slot_floats = static_cast<int64_t>(R) * kRow<D>;
         float* partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == part_first ? 1 : 0)) * slot_floats;
-        for (int i = threadIdx.x; i < valid_rows * D; i += kThreads) {
-            const int r = i / D, d = i - r * D;
+        for (int i = threadIdx.x; i < valid_rows * (D / 4); i += kCompute) {
+            const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
             float best = kNoMax;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) best = fmaxf(best, join[(w * R + r) * kRow<D> + D]);
-            float total = 0.0f, all = 0.0f, value = 0.0f;
+            float total = 0.0f, all = 0.0f;
+            float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float* from = join + (w * R + r) * kRow<D>;
                 const float weight = Exp2(from[D] - best);
-                total = fmaf(weight, from[D + 1], total);
-                all = fmaf(weight, from[D + 2], all);
-                value = fmaf(weight, from[d], value);
+                total = fmaf(weight, from[D + 2], total);
+                all = fmaf(weight, from[D + 3], all);
+                FmaFour(value, weight, *reinterpret_cast<const float4*>(from + d));
             }
             if (whole) {
-                StoreResult<D, DTYPE>(p, req, head, row + r, d, value, total, best, all);
+                StoreFour<D, DTYPE>(p, req, head, row + r, d, value, total, best, all);
             } else {
-                partial[r * kRow<D> + d] = value;
-                if (d == 0) {
-                    partial[r * kRow<D> + D] = best;
-                    partial[r * kRow<D> + D + 1] = total;
-                    partial[r * kRow<D> + D + 2] = all;
-                }
+                *reinterpret_cast<float4*>(partial + r * kRow<D> + d) = value;
+                if (d == 0) *reinterpret_cast<float4*>(partial + r * kRow<D> + D) = make_float4(best, 0.0f, total, all);
             }
         }
         if (!whole) {
             const int parts = static_cast<int>(part_last - part_first) + 1;
             __threadfence();
-            __syncthreads();
+            ComputeSync();
             if (threadIdx.x == 0) {
                 join_last = atomicAdd(&p.counters[part_first], 1) == parts - 1;
                 if (join_last) p.counters[part_first] = 0;
             }
-            __syncthreads();
+            ComputeSync();
             if (join_last) {
                 __threadfence();
-                JoinParts<D, DTYPE, kThreads>(p, req, head, row, valid_rows, static_cast<int>(part_first), parts, slot_floats,
-                                              join, static_cast<int>(Layout<D, NT>::kQueries / sizeof(float)));
+                JoinParts<D, DTYPE, kCompute>(p, req, head, row, valid_rows, static_cast<int>(part_first), parts, slot_floats, join,
+                                              static_cast<int>(Layout<D, NT>::kJoinFloats), threadIdx.x, ComputeSync);
             }
         }
-        FenceProxyAsync();  // the rings' memory was written by ordinary stores; copies write it next
-        __syncthreads();
-
-        at += here;
-        if (at >= share_end) break;
-        // the next unit
-        into = 0;
-        row += R;
-        if (row >= req.rows) {
-            row = 0;
-            if (++head == p.kv_heads) {
-                head = 0;
-                do {
-                    ++b;
-                    req = LoadRequest(p, b);
-                } while (req.rows == 0);
-            }
-        }
-        UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
+        if (!next_unit()) break;
     }
 }
 
@@ -718,13 +747,17 @@ int DecodeTiles(const fth_b200_kv4_attention_desc& d) {
 }
 // Blocks of threads that are resident together.
 int DecodeGrid(const fth_b200_kv4_attention_desc& d) {
-    const int per_sm = d.cache.head_dim == 64 ? Shape<64>::kBlocksPerSm : d.cache.head_dim == 128 ? Shape<128>::kBlocksPerSm : Shape<256>::kBlocksPerSm;
+    const int per_sm = d.cache.head_dim == 256 || DecodeTiles(d) == 2 ? kBlocksPerSm<256, 1> : kBlocksPerSm<128, 1>;
     const int grid = SmCount() * per_sm;
     return grid < kMaxGrid ? grid : kMaxGrid;
 }
 
 
+// More query rows per kv head than two eights: the kernel with 128-row tiles.
+bool ManyRows(const fth_b200_kv4_attention_desc& d) { return static_cast<int64_t>(d.max_query) * (d.q_heads / d.cache.kv_heads) > 16; }
+
 size_t WorkspaceBytes(const fth_b200_kv4_attention_desc& d) {
+    if (ManyRows(d)) return kCounterBytes + static_cast<size_t>(PrefillPartialFloats(d.cache.head_dim)) * sizeof(float);
     return kCounterBytes + static_cast<size_t>(DecodeGrid(d)) * 2 * 8 * DecodeTiles(d) * (d.cache.head_dim + 4) * sizeof(float);
 }
 
@@ -775,13 +808,20 @@ extern "C" int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* d, fth_
     p.causal = d->causal != 0;
     p.window = d->window;
     p.q_vec = kv4::AlignedTo(d->q, 16) && p.ldq % 8 == 0;
+    p.out_vec = kv4::AlignedTo(d->out, 8) && p.ldo % 4 == 0;
     p.scale_log2 = d->scale * 1.4426950408889634f;
     p.status = DeviceStatusPtr();
     p.counters = static_cast<int*>(d->workspace);
     p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + kv4::kCounterBytes);
     auto s = static_cast<cudaStream_t>(stream);
-    const int tiles = kv4::DecodeTiles(*d), grid = kv4::DecodeGrid(*d);
     int status;
+    if (kv4::ManyRows(*d)) {
+        p.few_units = static_cast<int64_t>(d->max_query) * p.group <= 512;
+        status = kv4::LaunchPrefill(p, d->cache.head_dim, d->dtype, s);
+        if (status == FTH_B200_OK) NoteLaunch("kv4_attention_rows");
+        return status;
+    }
+    const int tiles = kv4::DecodeTiles(*d), grid = kv4::DecodeGrid(*d);
     if (d->dtype == FTH_B200_BF16) {
         if (d->cache.head_dim == 64) status = kv4::LaunchDecode<64, FTH_B200_BF16>(p, tiles, grid, s);
         else if (d->cache.head_dim == 128) status = kv4::LaunchDecode<128, FTH_B200_BF16>(p, tiles, grid, s);

@@ -8,6 +8,8 @@ namespace fth {
 namespace kv4 {
 
 constexpr int kSiteAttention = 42, kSiteAttentionWait = 43;
+constexpr float kLazy = 8.0f;     // a running maximum may lag by 2^8 before sums are rescaled
+constexpr float kNotStarted = -3e38f;
 constexpr float kNoMax = -1e30f;  // the maximum of no scores: below all, and finite, so that differences stay numbers
 
 struct AttentionParams {
@@ -19,11 +21,12 @@ struct AttentionParams {
     const int32_t* table;
     const int32_t* total_lens;
     const int32_t* query_start;
-    int requests, max_blocks, max_query, kv_heads, group, causal, window, q_vec;
+    int requests, max_blocks, max_query, kv_heads, group, causal, window, q_vec, out_vec;
+    int few_units;     // no request has more than a few units of rows
     float scale_log2;  // scale * log2(e): scores are kept as exponents of two
     int* status;
     int* counters;     // one per block of threads: arrivals of the parts of the unit that begins in it
-    float* partials;   // [block of threads][2][rows of a unit][head_dim values, maximum, sum, sum for the lse, unused]
+    float* partials;   // [block of threads][2][rows of a unit][head_dim values, maximum, unused, sum, sum for the lse]
 };
 
 // The rows of one request and what they see.  Row i of n stands at position total - n + i.
@@ -83,13 +86,19 @@ __device__ __forceinline__ void UnitTiles(const AttentionParams& p, const Reques
 
 // ---- arithmetic -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void MmaF16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The first of a sum: c is written, not read.
+__device__ __forceinline__ void MmaF16First(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t Transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ float Exp2(float x) {
@@ -176,58 +185,91 @@ template <int D>
 constexpr int kRow = D + 4;
 
 // ---- results ---------------------------------------------------------------------------------------------------------------
-// Element d of row `row` of the request: value / total, and the row's lse (mass: the sum of its probabilities) with its first element.
+// Elements d .. d + 3 of row `row` of the request: value / total, and the row's lse (mass: the sum of its probabilities)
+// with its first elements.
 template <int D, int DTYPE>
-__device__ __forceinline__ void StoreResult(const AttentionParams& p, const Request& req, int head, int row, int d, float value, float total, float best, float mass) {
+__device__ __forceinline__ void StoreFour(const AttentionParams& p, const Request& req, int head, int row, int d, float4 v, float total, float best, float mass) {
     const int query = row / p.group;
     const int64_t q_row = req.first_row + static_cast<int64_t>(query);
     const int q_head = head * p.group + row - query * p.group;
-    rowops::WriteFloat<DTYPE>(p.out, q_row * p.ldo + static_cast<int64_t>(q_head) * D + d, total == 0.0f ? 0.0f : __fdividef(value, total));
+    const float scale = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+    const float x[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+    const int64_t at = q_row * p.ldo + static_cast<int64_t>(q_head) * D + d;
+    if (p.out_vec) {
+        uint2 packed;
+        if constexpr (DTYPE == FTH_B200_BF16) {
+            packed.x = EncodeBf16Cast(x[0]) | (static_cast<uint32_t>(EncodeBf16Cast(x[1])) << 16);
+            packed.y = EncodeBf16Cast(x[2]) | (static_cast<uint32_t>(EncodeBf16Cast(x[3])) << 16);
+        } else {
+            packed.x = PackHalf(x[0], x[1]);
+            packed.y = PackHalf(x[2], x[3]);
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = packed;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rowops::WriteFloat<DTYPE>(p.out, at + i, x[i]);
+    }
     if (d == 0 && p.lse != nullptr)
         p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(mass)) * 0.6931471805599453f;
 }
+__device__ __forceinline__ void FmaFour(float4& a, float w, float4 x) {
+    a.x = fmaf(w, x.x, a.x);
+    a.y = fmaf(w, x.y, a.y);
+    a.z = fmaf(w, x.z, a.z);
+    a.w = fmaf(w, x.w, a.w);
+}
 // Joins the parts of a unit, in order: part i is slot 1 of block `first` for i = 0 and slot 0 of block first + i behind it.
-// Every part's weight is computed once into shared memory; the values are then read with nothing waiting for another.
-template <int D, int DTYPE, int THREADS>
+// Every part's weight is computed once into shared memory; the values are then read sixteen bytes at a time with no load
+// waiting for another.  `sync` is a barrier of the THREADS threads (thread = 0 .. THREADS - 1) that call this.
+template <int D, int DTYPE, int THREADS, typename Sync>
 __device__ __forceinline__ void JoinParts(const AttentionParams& p, const Request& req, int head, int row, int rows, int first, int parts,
-                                          int64_t slot_floats, float* shared, int shared_floats) {
+                                          int64_t slot_floats, float* shared, int shared_floats, int thread, Sync sync) {
     const float* base = p.partials + (static_cast<int64_t>(first) * 2 + 1) * slot_floats;  // part i > 0 lies 2 i - 1 slots behind
     const auto slot = [&](int i) { return base + (i == 0 ? 0 : 2 * static_cast<int64_t>(i) - 1) * slot_floats; };
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float* weights = shared;                    // [rows][parts]
-    float* best_of = shared + rows * parts;     // [rows] maximum, [rows] sum, [rows] sum for the lse
-    if (static_cast<int64_t>(rows) * (parts + 3) > shared_floats) return;  // cannot be: the host sizes shared memory for it
-    __syncthreads();
-    for (int r = warp; r < rows; r += THREADS / 32) {
-        float best = kNoMax;
-        for (int i = lane; i < parts; i += 32) best = fmaxf(best, __ldcg(slot(i) + r * kRow<D> + D));
+    int at_once = shared_floats / (parts + 3);   // rows
+    if (at_once > rows) at_once = rows;
+    if (at_once < 1) return;                     // cannot be: shared memory is sized for it
+    float* best_of = shared;                     // [at_once] maximum, sum, sum for the lse
+    float* weights = shared + 3 * at_once;       // [at_once][parts]
+    const int lane = thread & 31, warp = thread >> 5;
+    for (int r0 = 0; r0 < rows; r0 += at_once) {
+        const int count = rows - r0 < at_once ? rows - r0 : at_once;
+        sync();
+        for (int r = warp; r < count; r += THREADS / 32) {
+            float best = kNoMax, total = 0.0f, mass = 0.0f;
+#pragma unroll 4
+            for (int i = lane; i < parts; i += 32) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (r0 + r) * kRow<D> + D));
+                weights[r * parts + i] = v.x;
+                const float next = fmaxf(best, v.x), old = Exp2(best - next), now = Exp2(v.x - next);
+                total = fmaf(now, v.z, total * old);
+                mass = fmaf(now, v.w, mass * old);
+                best = next;
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-        float total = 0.0f, mass = 0.0f;
-        for (int i = lane; i < parts; i += 32) {
-            const float w = Exp2(__ldcg(slot(i) + r * kRow<D> + D) - best);
-            weights[r * parts + i] = w;
-            total = fmaf(w, __ldcg(slot(i) + r * kRow<D> + D + 1), total);
-            mass = fmaf(w, __ldcg(slot(i) + r * kRow<D> + D + 2), mass);
+            for (int o = 16; o > 0; o >>= 1) {
+                const float b = __shfl_xor_sync(0xffffffffu, best, o), t = __shfl_xor_sync(0xffffffffu, total, o), m = __shfl_xor_sync(0xffffffffu, mass, o);
+                const float next = fmaxf(best, b), old = Exp2(best - next), now = Exp2(b - next);
+                total = fmaf(now, t, total * old);
+                mass = fmaf(now, m, mass * old);
+                best = next;
+            }
+            for (int i = lane; i < parts; i += 32) weights[r * parts + i] = Exp2(weights[r * parts + i] - best);
+            if (lane == 0) {
+                best_of[r] = best;
+                best_of[at_once + r] = total;
+                best_of[2 * at_once + r] = mass;
+            }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            total += __shfl_xor_sync(0xffffffffu, total, o);
-            mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        sync();
+        for (int i = thread; i < count * (D / 4); i += THREADS) {
+            const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+            float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 16
+            for (int c = 0; c < parts; ++c)
+                FmaFour(value, weights[r * parts + c], __ldcg(reinterpret_cast<const float4*>(slot(c) + (r0 + r) * kRow<D> + d)));
+            StoreFour<D, DTYPE>(p, req, head, row + r0 + r, d, value, best_of[at_once + r], best_of[r], best_of[2 * at_once + r]);
         }
-        if (lane == 0) {
-            best_of[r] = best;
-            best_of[rows + r] = total;
-            best_of[2 * rows + r] = mass;
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * D; i += THREADS) {
-        const int r = i / D, d = i - r * D;
-        float value = 0.0f;
-#pragma unroll 8
-        for (int c = 0; c < parts; ++c) value = fmaf(weights[r * parts + c], __ldcg(slot(c) + r * kRow<D> + d), value);
-        StoreResult<D, DTYPE>(p, req, head, row + r, d, value, best_of[rows + r], best_of[r], best_of[2 * rows + r]);
     }
 }
 

@@ -1,0 +1,742 @@
+// Attention over the 4-bit cache, many query rows per kv head (prompts, chunks of them, long drafts).
+//
+// The same arithmetic as in kv4_attention.cu on the tensor cores of sm_100: a tile of 128 query rows (queries x heads of
+// the group, so a group shares every key) against tiles of 128 tokens,
+//     S = Q C_k^T   tcgen05.mma kind::f16, both operands in shared memory, accumulator in tensor memory
+//     P = exp2(s_k S + m_k sum(q) - maximum) s_v, rounded to FP16, written over S in tensor memory
+//     O = O + P C_v   the probabilities read from tensor memory
+// with the codes as half-precision numbers: c * 2^-24 in the low four bits, 16 c * 2^-24 four bits higher, both exact
+// (kv4_attention.cu).  Four warps unpack: a word of eight K codes is five operations and one 16-byte store (q has its
+// elements in the order this gives), a word of V codes eight operations (a byte spread to two halves and one AND each), in
+// natural order with every second element times 16, which the results are divided by.  K tiles are K-major operands, V
+// tiles MN-major ones (a row per token), both with the 128-byte swizzle; the unpacking warps hold the next tile's words in
+// registers while the matrix unit still reads the present one.  Four more warps own a query row per thread: scores out of
+// tensor memory 32 at a time, two FMAs each on pairs, one exp2, and the sums.  One thread issues the matrix instructions.
+// Nothing of this is double-buffered within a block of threads: two blocks share an SM (one for 256-wide heads), and one's
+// softmax runs beside the other's products.
+//
+// Work is dealt out as in the decode kernel: the flat list of (request, kv head, 128 query rows, tile of tokens the
+// rows see) in equal contiguous shares, cut units joined by the part that arrives last.
+//
+// Bound: 4 * rows * tokens * head_dim operations on the matrix units; one exponential per score (16 a clock and SM) takes as
+// long as the products of 128-wide heads do.
+#include "kv4_attention.cuh"
+#include "kv4_prefill.h"
+#include "tcgen05.cuh"
+
+namespace fth {
+namespace kv4 {
+
+namespace {
+
+constexpr int kRows = 128;          // query rows of a unit
+constexpr int kTokens = 128;        // tokens of a tile
+constexpr int kThreads = 288;       // 4 softmax warps, 4 unpacking warps, 1 that issues
+constexpr int kBoundThreads = 320;  // ten warps: registers are handed out by quarters of an SM, five warps to one with two blocks
+constexpr int kSite = kSiteAttentionWait;
+
+template <int D>
+struct Tiles {
+    static constexpr int kBlocks64 = D / 64;                       // 128-byte wide pieces of a row
+    static constexpr int kPieceBytes = 128 * 128;
+    static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V
+    static constexpr int kParams = 3 * kOperandBytes;
+    static constexpr int kParamBytes = 6 * kTokens * 4;            // of one tile; two tiles' worth
+    static constexpr size_t kBytes = kParams + 2 * kParamBytes + 1024;  // 1024: alignment
+    static constexpr uint32_t kTmemColumns = D == 256 ? 512 : 256;
+    static constexpr int kBlocksPerSm = D == 256 ? 1 : 2;
+};
+// Arrays of a tile's parameters.
+enum { kScaleK = 0, kMinK = 1, kScaleV = 2, kMinV = 3, kInverseV = 4, kRatioV = 5 };
+
+__device__ __forceinline__ void MmaShared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void MmaTensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void TmemLoad32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+    umma::TmemLoadWait();
+}
+__device__ __forceinline__ void TmemStore16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                   "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int BAR>
+__device__ __forceinline__ void WarpsSync() { asm volatile("bar.sync %0, 128;" ::"n"(BAR) : "memory"); }
+
+__device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
+    return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// Sum of v over the warp.
+__device__ __forceinline__ int64_t WarpSum(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Token tiles of all units of one kv head of a request, by a whole warp.
+__device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, const Request& r) {
+    int64_t sum = 0;
+    for (int row = (threadIdx.x & 31) * kRows; row < r.rows; row += 32 * kRows) {
+        int a, b;
+        UnitTiles<kTokens>(p, r, row, kRows, &a, &b);
+        sum += b - a;
+    }
+    return WarpSum(sum);
+}
+
+// What a block of threads works on: a place in the list of units.
+struct Place {
+    int b, head, row;
+    int tile_first, tile_last;  // of the unit
+    int64_t into;               // tiles of the unit that other blocks take
+    int64_t at;                 // in the flat list
+    int t0, steps;              // this block's tiles of it
+    Request req;
+};
+__device__ __forceinline__ void Settle(const AttentionParams& p, int64_t share_end, Place& u) {
+    const int64_t left = share_end - u.at, tiles = u.tile_last - u.tile_first - u.into;
+    u.t0 = u.tile_first + static_cast<int>(u.into);
+    u.steps = static_cast<int>(tiles < left ? tiles : left);
+}
+__device__ __forceinline__ bool Advance(const AttentionParams& p, int64_t share_end, Place& u) {
+    u.at += u.steps;
+    if (u.at >= share_end) return false;
+    u.into = 0;
+    u.row += kRows;
+    if (u.row >= u.req.rows) {
+        u.row = 0;
+        if (++u.head == p.kv_heads) {
+            u.head = 0;
+            do {
+                ++u.b;
+                u.req = LoadRequest(p, u.b);
+            } while (u.req.rows == 0);
+        }
+    }
+    UnitTiles<kTokens>(p, u.req, u.row, kRows, &u.tile_first, &u.tile_last);
+    Settle(p, share_end, u);
+    return true;
+}
+
+template <int D, int DTYPE>
+__global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) PrefillKernel(const __grid_constant__ AttentionParams p) {
+    using T = Tiles<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    __shared__ uint32_t tmem_slot;
+    __shared__ __align__(8) uint64_t bars[8];
+    uint64_t &q_full = bars[0], &k_full = bars[1], &k_empty = bars[2], &v_full = bars[3], &v_empty = bars[4], &s_full = bars[5], &p_full = bars[6], &o_full = bars[7];
+    __shared__ int64_t unit_work[kThreads];
+    __shared__ int64_t work_total, longest;
+    __shared__ Place start;
+    __shared__ uint32_t present[2][4];     // a bit per token of a tile that some row may see
+    __shared__ float scale_range[2][4][2]; // smallest and largest value scale of those tokens, by unpacking warp
+    __shared__ float q_big[4];
+    __shared__ int join_last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        MbarInit(&q_full, 128);
+        MbarInit(&k_full, 128);
+        MbarInit(&k_empty, 1);
+        MbarInit(&v_full, 128);
+        MbarInit(&v_empty, 1);
+        MbarInit(&s_full, 1);
+        MbarInit(&p_full, 128);
+        MbarInit(&o_full, 1);
+        FenceBarrierInit();
+    }
+    // tensor memory is taken before the next kernel of the stream may start on this SM and take it
+    if (warp == 8) umma::TmemAlloc(&tmem_slot, T::kTmemColumns);
+    umma::FenceBeforeThreadSync();
+    __syncthreads();
+    umma::FenceAfterThreadSync();
+    const uint32_t tmem = tmem_slot;
+    WaitForPrevious();
+
+    // ---- this block's share ----------------------------------------------------------------------------------------------
+    // A warp takes a request at a time; thread 0 adds.  Few requests have many rows.
+    if (threadIdx.x == 0) work_total = longest = 0;
+    __syncthreads();
+    for (int base = 0; base < p.requests; base += kThreads) {
+        const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
+        if (p.few_units) {
+            if (threadIdx.x < count) {
+                const Request r = LoadRequest(p, base + threadIdx.x);
+                int64_t sum = 0;
+                for (int row = 0; row < r.rows; row += kRows) {
+                    int a, b;
+                    UnitTiles<kTokens>(p, r, row, kRows, &a, &b);
+                    sum += b - a;
+                }
+                unit_work[threadIdx.x] = sum;
+            }
+        } else {
+            for (int i = warp; i < count; i += kThreads / 32) {
+                const int64_t sum = RequestTiles(p, LoadRequest(p, base + i));
+                if (lane == 0) unit_work[i] = sum;
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int64_t sum = 0;
+            for (int i = lane; i < count; i += 32) sum += unit_work[i];
+            sum = WarpSum(sum);
+            if (lane == 0) work_total += sum * p.kv_heads;
+        }
+        __syncthreads();
+    }
+    const int64_t work = work_total;
+    const int64_t per = work > 0 ? Divide(work + gridDim.x - 1, gridDim.x) : 1;
+    const int64_t share_begin = blockIdx.x * per;
+    const int64_t share_end = share_begin + per < work ? share_begin + per : work;
+    const bool busy = share_begin < share_end;
+    if (busy) {
+        // the request, then the head, then the rows that share_begin falls into
+        int64_t passed = 0;
+        for (int base = 0; base < p.requests; base += kThreads) {
+            const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
+            if (p.requests > kThreads) {
+                __syncthreads();
+                for (int i = warp; i < count; i += kThreads / 32) {
+                    const int64_t sum = RequestTiles(p, LoadRequest(p, base + i));
+                    if (lane == 0) unit_work[i] = sum;
+                }
+                __syncthreads();
+            }
+            bool found = false;
+            if (warp == 0) {
+                for (int i = 0; i < count && !found; i += 32) {
+                    int64_t mine = i + lane < count ? unit_work[i + lane] * p.kv_heads : 0, sum = mine;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int64_t n = __shfl_up_sync(0xffffffffu, sum, o);
+                        if (lane >= o) sum += n;
+                    }
+                    const int64_t all = __shfl_sync(0xffffffffu, sum, 31);
+                    const int64_t before = passed + sum - mine;
+                    const uint32_t who = __ballot_sync(0xffffffffu, share_begin >= before && share_begin < before + mine);
+                    if (who != 0) {
+                        found = true;
+                        const int src = __ffs(who) - 1;
+                        int64_t off = share_begin - __shfl_sync(0xffffffffu, before, src);
+                        const int64_t per_head = unit_work[i + src];
+                        Place u;
+                        u.b = base + i + src;
+                        u.req = LoadRequest(p, u.b);
+                        u.head = static_cast<int>(Divide(off, per_head));
+                        off -= u.head * per_head;
+                        // rows, 32 units at a time
+                        for (int row = 0;; row += 32 * kRows) {
+                            const int my_row = row + lane * kRows;
+                            int a = 0, c = 0;
+                            if (my_row < u.req.rows) UnitTiles<kTokens>(p, u.req, my_row, kRows, &a, &c);
+                            int64_t upto = c - a;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const int64_t n = __shfl_up_sync(0xffffffffu, upto, o);
+                                if (lane >= o) upto += n;
+                            }
+                            const uint32_t here = __ballot_sync(0xffffffffu, off < upto);
+                            if (here != 0) {
+                                if (lane == __ffs(here) - 1) {
+                                    u.row = my_row;
+                                    u.tile_first = a;
+                                    u.tile_last = c;
+                                    u.into = off - (upto - (c - a));
+                                    u.at = share_begin;
+                                    Settle(p, share_end, u);
+                                    start = u;
+                                }
+                                break;
+                            }
+                            off -= __shfl_sync(0xffffffffu, upto, 31);
+                        }
+                    }
+                    passed += all;
+                }
+            }
+            if (__syncthreads_or(found ? 1 : 0)) break;
+        }
+        __syncthreads();
+    }
+
+    uint8_t* const q_smem = smem;
+    uint8_t* const k_smem = smem + T::kOperandBytes;
+    uint8_t* const v_smem = smem + 2 * T::kOperandBytes;
+    float* const params = reinterpret_cast<float*>(smem + T::kParams);
+    bool failed = false;
+    const auto wait = [&](uint64_t* bar, uint32_t parity, int detail) {
+        if (!failed && !MbarWait(bar, parity, p.status, kSite, 16 + detail)) failed = true;
+    };
+
+    if (busy && warp >= 4 && warp < 8) {
+        // ================================================ unpacking ==================================================
+        const int tid = threadIdx.x - 128;
+        Place u = start;
+        int64_t tile_count = 0;
+        // this thread's 16-byte pieces: K piece j is 32 elements of a token, V piece j four words of a pair of tokens
+        constexpr int kPieces = D / 32;
+        uint4 kw[kPieces], vw[kPieces];
+        uint32_t kp, vp;
+        bool there;
+        do {
+            int first_low, last_high, unused;
+            Visible(p, u.req, u.row / p.group, &first_low, &unused);
+            Visible(p, u.req, ((u.row + kRows < u.req.rows ? u.row + kRows : u.req.rows) - 1) / p.group, &unused, &last_high);
+            const int32_t* table = p.table + static_cast<int64_t>(u.b) * p.max_blocks;
+            // index of token `token` within its head, or -1 when no row sees it or its block does not exist
+            const auto locate = [&](int token) -> int64_t {
+                if (token >= last_high || token < (first_low & ~15)) return -1;
+                const int id = table[token >> p.cache.block_shift];
+                if (id < 0 || id >= p.cache.blocks) {
+                    ReportTimeout(p.status, kSiteAttention, u.b);
+                    return -1;
+                }
+                return HeadBase(p.cache, id, u.head) + (token & ((1 << p.cache.block_shift) - 1));
+            };
+            // K: neighbouring lanes take the halves of 64 bytes of four tokens, then further 64-byte pieces, so that the eight
+            // lanes of a store phase hit eight different 16-byte columns
+            const auto k_token = [&](int j) { return ((tid + 128 * j) >> 1 & 3) | ((tid + 128 * j) / (4 * kPieces) << 2); };
+            const auto k_piece = [&](int j) { return ((tid + 128 * j) & 1) | (((tid + 128 * j) >> 3) % (kPieces / 2) << 1); };
+            const auto load_k = [&](int step) {
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const int64_t at = locate((u.t0 + step) * kTokens + k_token(j));
+                    kw[j] = make_uint4(0, 0, 0, 0);
+                    if (at >= 0) kw[j] = LoadStream16(p.cache.k_codes + at * (D / 2) + k_piece(j) * 16);
+                }
+                const int token = (u.t0 + step) * kTokens + tid;
+                const int64_t at = locate(token);
+                there = at >= 0 && token >= first_low;
+                kp = vp = 0;
+                if (there) {
+                    kp = p.cache.k_params[at];
+                    vp = p.cache.v_params[at];
+                }
+            };
+            // V: neighbouring lanes take 64 bytes of one pair of tokens, then of the next
+            const auto v_pair = [&](int j) { return ((tid + 128 * j) >> 2 & 1) | ((tid + 128 * j) / (8 * T::kBlocks64) << 1); };
+            const auto v_piece = [&](int j) { return ((tid + 128 * j) & 3) | (((tid + 128 * j) >> 3) % T::kBlocks64 << 2); };
+            const auto load_v = [&](int step) {
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const int pair = v_pair(j), piece = v_piece(j);
+                    const int64_t at = locate((u.t0 + step) * kTokens + 2 * pair);
+                    vw[j] = make_uint4(0, 0, 0, 0);
+                    if (at >= 0) vw[j] = LoadStream16(p.cache.v_codes + at * (D / 2) + piece * 16);
+                }
+            };
+            load_k(0);
+            load_v(0);
+            for (int step = 0; step < u.steps; ++step, ++tile_count) {
+                const uint32_t par = static_cast<uint32_t>(tile_count & 1);
+                if (tile_count > 0) wait(&k_empty, par ^ 1u, 0);
+                // parameters, and the token's bit
+                {
+                    float* a = params + par * (T::kParamBytes / 4) + tid;
+                    const float vs = ParamScale(vp), vm = ParamMin(vp), inverse = Reciprocal(vs);
+                    a[kScaleK * kTokens] = ParamScale(kp);
+                    a[kMinK * kTokens] = ParamMin(kp);
+                    a[kScaleV * kTokens] = vs;
+                    a[kMinV * kTokens] = vm;
+                    if constexpr (DTYPE == FTH_B200_FP16) {
+                        a[kInverseV * kTokens] = inverse;
+                        a[kRatioV * kTokens] = vm * inverse;
+                    }
+                    const uint32_t bits = __ballot_sync(0xffffffffu, there);
+                    const uint32_t scale = there ? vp << 16 : 0u;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, scale), low = __reduce_min_sync(0xffffffffu, there ? scale : 0x7f800000u);
+                    if (lane == 0) {
+                        present[par][warp - 4] = bits;
+                        scale_range[par][warp - 4][0] = __uint_as_float(low);
+                        scale_range[par][warp - 4][1] = __uint_as_float(top);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const int token = k_token(j), piece = k_piece(j);
+                    uint8_t* row = k_smem + (piece >> 1) * T::kPieceBytes + token * 128;
+                    const uint32_t w[4] = {kw[j].x, kw[j].y, kw[j].z, kw[j].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t x = w[i], y = x >> 8;
+                        *reinterpret_cast<uint4*>(row + ((((piece & 1) * 4 + i) ^ (token & 7)) << 4)) =
+                            make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
+                    }
+                }
+                FenceProxyAsync();
+                MbarArrive(&k_full);
+                if (step + 1 < u.steps) load_k(step + 1);
+                if (tile_count > 0) wait(&v_empty, par ^ 1u, 1);
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const int pair = v_pair(j), piece = v_piece(j);
+                    const uint32_t w[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        // half v of the sixteen elements, of token 2 * pair + odd; the order of the halves alternates with the
+                        // pair, so that a store phase hits eight different 16-byte columns
+                        const int odd = s & 1, v = (s >> 1) ^ (pair & 1);
+                        const uint32_t x0 = v ? w[2] : w[0], x1 = v ? w[3] : w[1];
+                        const uint32_t low = odd ? 0x4242u : 0x4040u, high = odd ? 0x4343u : 0x4141u;
+                        const int token = 2 * pair + odd, column = 2 * (piece & 3) + v;
+                        *reinterpret_cast<uint4*>(v_smem + (piece >> 2) * T::kPieceBytes + token * 128 + ((column ^ (token & 7)) << 4)) =
+                            make_uint4(__byte_perm(x0, 0, low) & 0x00f0000fu, __byte_perm(x0, 0, high) & 0x00f0000fu,
+                                       __byte_perm(x1, 0, low) & 0x00f0000fu, __byte_perm(x1, 0, high) & 0x00f0000fu);
+                    }
+                }
+                FenceProxyAsync();
+                MbarArrive(&v_full);
+                if (step + 1 < u.steps) load_v(step + 1);
+            }
+        } while (Advance(p, share_end, u));
+    } else if (busy && warp == 8) {
+        // ================================================ products ===================================================
+        if (lane == 0) {
+            Place u = start;
+            const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, true, kRows, D);
+            const uint32_t q_addr = SmemAddr(q_smem), k_addr = SmemAddr(k_smem), v_addr = SmemAddr(v_smem);
+            const uint32_t s_tmem = tmem, o_tmem = tmem + 128;
+            int64_t tile_count = 0;
+            uint32_t unit_count = 0;
+            do {
+                wait(&q_full, unit_count & 1u, 2);
+                for (int step = 0; step < u.steps; ++step, ++tile_count) {
+                    const uint32_t par = static_cast<uint32_t>(tile_count & 1);
+                    wait(&k_full, par, 3);
+                    if (tile_count > 0) wait(&v_empty, par ^ 1u, 8);  // S is written where the last tile's P was read
+                    umma::FenceAfterThreadSync();
+                    if (failed) break;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t at = (i >> 2) * T::kPieceBytes + (i & 3) * 32;
+                        MmaShared(s_tmem, umma::SmemDesc(q_addr + at, 0, 1024), umma::SmemDesc(k_addr + at, 0, 1024), s_desc, i > 0);
+                    }
+                    umma::Commit(&s_full);
+                    umma::Commit(&k_empty);
+                    wait(&p_full, par, 4);
+                    wait(&v_full, par, 5);
+                    umma::FenceAfterThreadSync();
+                    if (failed) break;
+#pragma unroll
+                    for (int i = 0; i < kTokens / 16; ++i)
+                        MmaTensor(o_tmem, s_tmem + i * 8, umma::SmemDesc(v_addr + i * 2048, T::kPieceBytes, 1024), o_desc, step > 0 || i > 0);
+                    umma::Commit(&v_empty);
+                    if (step + 1 == u.steps) umma::Commit(&o_full);
+                }
+                ++unit_count;
+            } while (!failed && Advance(p, share_end, u));
+        }
+    } else if (busy && warp < 4) {
+        // ================================================ softmax ====================================================
+        const int r = threadIdx.x;             // row of the unit, lane of tensor memory
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+        const uint32_t s_tmem = tmem + lanes, o_tmem = tmem + 128 + lanes;
+        Place u = start;
+        int64_t tile_count = 0;
+        uint32_t unit_count = 0;
+        for (;;) {
+            // ---- the unit's queries, as operands
+            const bool valid = u.row + r < u.req.rows;
+            const int query = valid ? (u.row + r) / p.group : 0;
+            const uint16_t* from = static_cast<const uint16_t*>(p.q) + (u.req.first_row + static_cast<int64_t>(query)) * p.ldq +
+                                   (static_cast<int64_t>(u.head) * p.group + (u.row + r - query * p.group)) * D;
+            float big = 0.0f, qsum = 0.0f;
+            if (valid) {
+#pragma unroll 4
+                for (int w = 0; w < D / 8; ++w) {
+                    const uint4 x = p.q_vec ? *reinterpret_cast<const uint4*>(from + w * 8) : LoadUnaligned8(from + w * 8);
+                    const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 v = HalfPair<DTYPE>(raw[i]);
+                        big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+                        qsum += v.x + v.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            if (lane == 0) q_big[warp] = big;
+            WarpsSync<1>();
+            big = fmaxf(fmaxf(q_big[0], q_big[1]), fmaxf(q_big[2], q_big[3]));
+            const int e = QueryExponent(big);
+            const float up = PowerOfTwo(e), back = p.scale_log2 * PowerOfTwo(24 - e);
+            qsum *= p.scale_log2;
+#pragma unroll 4
+            for (int w = 0; w < D / 8; ++w) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (valid) x = p.q_vec ? *reinterpret_cast<const uint4*>(from + w * 8) : LoadUnaligned8(from + w * 8);
+                const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
+                uint32_t f[4];
+                QueryOperands<DTYPE>(raw, up, f);
+                *reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + r * 128 + (((w & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            }
+            FenceProxyAsync();
+            MbarArrive(&q_full);
+            int low = 0, high = 0;
+            if (valid) Visible(p, u.req, query, &low, &high);
+
+            // ---- tiles.  Scores are kept relative to ref = maximum - k, where 2^k brings the value scales below 2^7: all sums
+            // and the weights carry the same factor 2^k, which the division at the end takes out.
+            float ref = 0.0f, limit = kNotStarted, scale_limit = 0.0f;
+            int k = 0;
+            float2 sum = make_float2(0.0f, 0.0f), mass = sum, offset = sum;
+            for (int step = 0; step < u.steps; ++step, ++tile_count) {
+                const uint32_t par = static_cast<uint32_t>(tile_count & 1);
+                wait(&s_full, par, 6);
+                umma::FenceAfterThreadSync();
+                const float* a = params + par * (T::kParamBytes / 4);
+                const int token0 = (u.t0 + step) * kTokens;
+                const uint32_t pr[4] = {present[par][0], present[par][1], present[par][2], present[par][3]};
+                const bool all_there = (pr[0] & pr[1] & pr[2] & pr[3]) == 0xffffffffu;
+                const bool inside = all_there && __all_sync(0xffffffffu, !valid || (token0 >= low && token0 + kTokens <= high));
+                float biggest = 0.0f, smallest = INFINITY;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    smallest = fminf(smallest, scale_range[par][w][0]);
+                    biggest = fmaxf(biggest, scale_range[par][w][1]);   // NaN drops out; the weights show it
+                }
+                int new_k = k;
+                if (biggest > scale_limit) {
+                    const int se = ScaleExponent(biggest);
+                    new_k = 7 - se;
+                    scale_limit = PowerOfTwo(se);
+                }
+                const bool exact_weights = DTYPE == FTH_B200_FP16 && inside && smallest * PowerOfTwo(new_k) >= 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32];
+                    TmemLoad32(s_tmem + c * 32, s);
+                    float2 z[16];
+                    float best = -INFINITY;
+                    const float4* ks = reinterpret_cast<const float4*>(a + kScaleK * kTokens + c * 32);
+                    const float4* km = reinterpret_cast<const float4*>(a + kMinK * kTokens + c * 32);
+                    const float2 qq = make_float2(qsum, qsum), rr = make_float2(-ref, -ref), bb = make_float2(back, back);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 s4 = ks[i], m4 = km[i];
+                        float2 t0 = Fma2(make_float2(m4.x, m4.y), qq, rr), t1 = Fma2(make_float2(m4.z, m4.w), qq, rr);
+                        const float2 v0 = Mul2(make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), bb);
+                        const float2 v1 = Mul2(make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), bb);
+                        z[2 * i] = Fma2(make_float2(s4.x, s4.y), v0, t0);
+                        z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), v1, t1);
+                    }
+                    if (!inside) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int token = token0 + c * 32 + i;
+                            if (token < low || token >= high || ((pr[c] >> i) & 1u) == 0) {
+                                if (i & 1) z[i >> 1].y = -INFINITY;
+                                else z[i >> 1].x = -INFINITY;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) best = fmaxf(best, fmaxf(z[i].x, z[i].y));
+                    if (__any_sync(0xffffffffu, best > limit || new_k != k)) {
+                        // move the maximum: scores of this chunk, the weights of the tile's earlier ones, sums and results
+                        const bool first = limit == kNotStarted;
+                        const float over = best - static_cast<float>(k);   // above the old maximum
+                        float moved = 0.0f;
+                        if (first ? over > kNotStarted : over > 0.0f) {
+                            moved = over;
+                            if (!first) moved = ceilf(moved);   // a whole number of doublings keeps earlier weights exact
+                        }
+                        const float shift = moved + static_cast<float>(k - new_k);
+                        if (!first || moved != 0.0f || over > kNotStarted) limit = first && !(over > kNotStarted) ? kNotStarted : kLazy + static_cast<float>(new_k);
+                        const float alpha = first ? 0.0f : Exp2(-shift);
+                        ref += shift;
+                        sum = Mul2(sum, make_float2(alpha, alpha));
+                        mass = Mul2(mass, make_float2(alpha, alpha));
+                        offset = Mul2(offset, make_float2(alpha, alpha));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[i] = make_float2(z[i].x - shift, z[i].y - shift);
+                        TmemStoreWait();
+                        for (int b = 0; b < c; ++b) {
+                            uint32_t w[16];
+                            umma::TmemLoad16(s_tmem + b * 16, w);
+                            umma::TmemLoadWait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 v = HalfPair<FTH_B200_FP16>(w[i]);
+                                w[i] = PackHalf(v.x * alpha, v.y * alpha);
+                            }
+                            TmemStore16(s_tmem + b * 16, w);
+                        }
+                        if (step > 0) {
+                            for (int b = 0; b < D / 16; ++b) {
+                                uint32_t w[16];
+                                umma::TmemLoad16(o_tmem + b * 16, w);
+                                umma::TmemLoadWait();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
+                                TmemStore16(o_tmem + b * 16, w);
+                            }
+                        }
+                        TmemStoreWait();
+                        k = new_k;
+                    }
+                    uint32_t packed[16];
+                    const float4* vs = reinterpret_cast<const float4*>(a + kScaleV * kTokens + c * 32);
+                    const float4* vm = reinterpret_cast<const float4*>(a + kMinV * kTokens + c * 32);
+                    if (exact_weights) {
+                        const float4* vi = reinterpret_cast<const float4*>(a + kInverseV * kTokens + c * 32);
+                        const float4* vr = reinterpret_cast<const float4*>(a + kRatioV * kTokens + c * 32);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 s4 = vs[i], i4 = vi[i], r4 = vr[i];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float2 prob = make_float2(Exp2(z[2 * i + h].x), Exp2(z[2 * i + h].y));
+                                mass = Add2(mass, prob);
+                                const float2 w = Mul2(prob, h ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y));
+                                packed[2 * i + h] = PackHalf(w.x, w.y);
+                                const float2 kept = HalfPair<FTH_B200_FP16>(packed[2 * i + h]);
+                                sum = Fma2(kept, h ? make_float2(i4.z, i4.w) : make_float2(i4.x, i4.y), sum);
+                                offset = Fma2(kept, h ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y), offset);
+                            }
+                        }
+                    } else if (DTYPE == FTH_B200_BF16 && inside) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 s4 = vs[i], m4 = vm[i];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float2 prob = make_float2(Exp2(z[2 * i + h].x), Exp2(z[2 * i + h].y));
+                                mass = Add2(mass, prob);
+                                offset = Fma2(prob, h ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y), offset);
+                                const float2 w = Mul2(prob, h ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y));
+                                packed[2 * i + h] = PackHalf(w.x, w.y);
+                            }
+                        }
+                    } else {
+                        // hidden tokens (whatever stands there: 0 * NaN is no zero), or value scales too small beside the largest
+                        // for a weight to give the probability back
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float w[2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float score = h ? z[i].y : z[i].x;
+                                const bool hidden = score == -INFINITY;
+                                const float prob = Exp2(score);
+                                const float scale = a[kScaleV * kTokens + c * 32 + 2 * i + h], minimum = a[kMinV * kTokens + c * 32 + 2 * i + h];
+                                w[h] = hidden ? 0.0f : __half2float(__float2half_rn(prob * scale));
+                                float kept = prob;
+                                if (DTYPE == FTH_B200_FP16 && scale * PowerOfTwo(k) >= 1.0f) kept = w[h] * a[kInverseV * kTokens + c * 32 + 2 * i + h];
+                                if (!hidden) {
+                                    mass.x += prob;
+                                    if (DTYPE == FTH_B200_FP16) sum.x += kept;
+                                    offset.x = fmaf(kept, minimum, offset.x);
+                                }
+                            }
+                            packed[i] = PackHalf(w[0], w[1]);
+                        }
+                    }
+                    TmemStore16(s_tmem + c * 16, packed);
+                }
+                TmemStoreWait();
+                umma::FenceBeforeThreadSync();
+                MbarArrive(&p_full);
+            }
+
+            // ---- the unit's results
+            wait(&o_full, unit_count & 1u, 7);
+            umma::FenceAfterThreadSync();
+            const float all = mass.x + mass.y, total = DTYPE == FTH_B200_FP16 ? sum.x + sum.y : all, shift = offset.x + offset.y;
+            const int64_t unit_begin = u.at - u.into, unit_end = unit_begin + (u.tile_last - u.tile_first);
+            const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : Divide(unit_begin, per);
+            const int64_t part_last = unit_end <= share_end ? blockIdx.x : Divide(unit_end - 1, per);
+            const bool whole = part_first == part_last;
+            const int64_t slot_floats = static_cast<int64_t>(kRows) * kRow<D>;
+            float* partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == part_first ? 1 : 0)) * slot_floats + r * kRow<D>;
+            const float best = limit == kNotStarted ? kNoMax : ref;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+                uint32_t w[16];
+                __syncwarp();
+                umma::TmemLoad16(o_tmem + c * 16, w);
+                umma::TmemLoadWait();
+                if (!valid || failed) continue;   // a wait that gave up is in the status word; nothing is stored then
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float unit = 16777216.0f;
+                    const float4 v = make_float4(fmaf(__uint_as_float(w[i]), unit, shift), fmaf(__uint_as_float(w[i + 1]), unit * 0.0625f, shift),
+                                                 fmaf(__uint_as_float(w[i + 2]), unit, shift), fmaf(__uint_as_float(w[i + 3]), unit * 0.0625f, shift));
+                    if (whole) StoreFour<D, DTYPE>(p, u.req, u.head, u.row + r, c * 16 + i, v, total, best, all);
+                    else *reinterpret_cast<float4*>(partial + c * 16 + i) = v;
+                }
+            }
+            if (!whole) {
+                if (valid) *reinterpret_cast<float4*>(partial + D) = make_float4(best, 0.0f, total, all);
+                const int parts = static_cast<int>(part_last - part_first) + 1;
+                __threadfence();
+                WarpsSync<1>();
+                if (threadIdx.x == 0) {
+                    join_last = atomicAdd(&p.counters[part_first], 1) == parts - 1;
+                    if (join_last) p.counters[part_first] = 0;
+                }
+                WarpsSync<1>();
+                if (join_last) {
+                    __threadfence();
+                    const int rows = u.req.rows - u.row < kRows ? u.req.rows - u.row : kRows;
+                    // the query operands' memory: every product that read it is done
+                    JoinParts<D, DTYPE, 128>(p, u.req, u.head, u.row, rows, static_cast<int>(part_first), parts, slot_floats,
+                                             reinterpret_cast<float*>(q_smem), T::kOperandBytes / 4, threadIdx.x, WarpsSync<1>);
+                }
+            }
+            ++unit_count;
+            umma::FenceBeforeThreadSync();
+            if (!Advance(p, share_end, u)) break;
+        }
+    }
+    __syncwarp();
+    umma::FenceBeforeThreadSync();
+    __syncthreads();
+    umma::FenceAfterThreadSync();
+    if (warp == 8) umma::TmemDealloc(tmem, T::kTmemColumns);
+}
+
+template <int D, int DTYPE>
+int LaunchTyped(const AttentionParams& p, int grid, cudaStream_t s) {
+    const auto kernel = PrefillKernel<D, DTYPE>;
+    if (EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), Tiles<D>::kBytes) != FTH_B200_OK) return FTH_B200_ERR_CUDA;
+    return Launch(kernel, dim3(static_cast<unsigned>(grid)), kThreads, Tiles<D>::kBytes, s, p);
+}
+
+}  // namespace
+
+int PrefillGrid(int head_dim) { return SmCount() * (head_dim == 256 ? Tiles<256>::kBlocksPerSm : Tiles<128>::kBlocksPerSm); }
+
+int64_t PrefillPartialFloats(int head_dim) { return static_cast<int64_t>(PrefillGrid(head_dim)) * 2 * kRows * (head_dim + 4); }
+
+int LaunchPrefill(const AttentionParams& p, int head_dim, int dtype, cudaStream_t s) {
+    const int grid = PrefillGrid(head_dim);
+    if (dtype == FTH_B200_BF16) {
+        if (head_dim == 64) return LaunchTyped<64, FTH_B200_BF16>(p, grid, s);
+        if (head_dim == 128) return LaunchTyped<128, FTH_B200_BF16>(p, grid, s);
+        return LaunchTyped<256, FTH_B200_BF16>(p, grid, s);
+    }
+    if (head_dim == 64) return LaunchTyped<64, FTH_B200_FP16>(p, grid, s);
+    if (head_dim == 128) return LaunchTyped<128, FTH_B200_FP16>(p, grid, s);
+    return LaunchTyped<256, FTH_B200_FP16>(p, grid, s);
+}
+
+}  // namespace kv4
+}  // namespace fth
