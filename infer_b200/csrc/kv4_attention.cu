@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
             ComputeSync();
             if (join_last) {
                 __threadfence();
-                JoinParts<D, DTYPE, kCompute>(p, req, head, row, valid_rows, static_cast<int>(part_first), parts, slot_floats, join,
+                JoinParts<D, DTYPE, kCompute>(p, req, head, row, valid_rows, p.partials, static_cast<int>(part_first), parts, slot_floats, join,
                                               static_cast<int>(Layout<D, NT>::kJoinFloats), threadIdx.x, ComputeSync);
             }
         }

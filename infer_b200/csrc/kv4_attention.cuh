@@ -222,9 +222,9 @@ __device__ __forceinline__ void FmaFour(float4& a, float w, float4 x) {
 // Every part's weight is computed once into shared memory; the values are then read sixteen bytes at a time with no load
 // waiting for another.  `sync` is a barrier of the THREADS threads (thread = 0 .. THREADS - 1) that call this.
 template <int D, int DTYPE, int THREADS, typename Sync>
-__device__ __forceinline__ void JoinParts(const AttentionParams& p, const Request& req, int head, int row, int rows, int first, int parts,
+__device__ __forceinline__ void JoinParts(const AttentionParams& p, const Request& req, int head, int row, int rows, const float* partials, int first, int parts,
                                           int64_t slot_floats, float* shared, int shared_floats, int thread, Sync sync) {
-    const float* base = p.partials + (static_cast<int64_t>(first) * 2 + 1) * slot_floats;  // part i > 0 lies 2 i - 1 slots behind
+    const float* base = partials + (static_cast<int64_t>(first) * 2 + 1) * slot_floats;  // part i > 0 lies 2 i - 1 slots behind
     const auto slot = [&](int i) { return base + (i == 0 ? 0 : 2 * static_cast<int64_t>(i) - 1) * slot_floats; };
     int at_once = shared_floats / (parts + 3);   // rows
     if (at_once > rows) at_once = rows;

@@ -12,8 +12,9 @@
 // tiles MN-major ones (a row per token), both with the 128-byte swizzle; the unpacking warps hold the next tile's words in
 // registers while the matrix unit still reads the present one.  Four more warps own a query row per thread: scores out of
 // tensor memory 32 at a time, two FMAs each on pairs, one exp2, and the sums.  One thread issues the matrix instructions.
-// Nothing of this is double-buffered within a block of threads: two blocks share an SM (one for 256-wide heads), and one's
-// softmax runs beside the other's products.
+// A block of threads has two tiles of query rows (one for 256-wide heads, whose results fill tensor memory) that share the
+// unpacked tokens: while one's scores become probabilities the matrix unit works for the other.  Unpacked tiles are
+// double-buffered (not for 256-wide heads, where shared memory holds one).
 //
 // Work is dealt out as in the decode kernel: the flat list of (request, kv head, 128 query rows, tile of tokens the
 // rows see) in equal contiguous shares, cut units joined by the part that arrives last.
@@ -29,22 +30,25 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kRows = 128;          // query rows of a unit
+constexpr int kRows = 128;          // query rows of a tile
 constexpr int kTokens = 128;        // tokens of a tile
-constexpr int kThreads = 288;       // 4 softmax warps, 4 unpacking warps, 1 that issues
-constexpr int kBoundThreads = 320;  // ten warps: registers are handed out by quarters of an SM, five warps to one with two blocks
 constexpr int kSite = kSiteAttentionWait;
 
 template <int D>
 struct Tiles {
+    static constexpr int kQueryTiles = D == 256 ? 1 : 2;
+    static constexpr int kUnitRows = kQueryTiles * kRows;
+    static constexpr int kStages = D == 256 ? 1 : 2;               // unpacked tiles of tokens
+    static constexpr int kSoftmax = kQueryTiles * 128;             // threads: softmax, unpacking, the warp that issues
+    static constexpr int kThreads = kSoftmax + 128 + 32;
     static constexpr int kBlocks64 = D / 64;                       // 128-byte wide pieces of a row
     static constexpr int kPieceBytes = 128 * 128;
-    static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V
-    static constexpr int kParams = 3 * kOperandBytes;
+    static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V of one tile
+    static constexpr int kKeys = kQueryTiles * kOperandBytes;      // stages of K, then of V
+    static constexpr int kParams = kKeys + 2 * kStages * kOperandBytes;
     static constexpr int kParamBytes = 6 * kTokens * 4;            // of one tile; two tiles' worth
     static constexpr size_t kBytes = kParams + 2 * kParamBytes + 1024;  // 1024: alignment
-    static constexpr uint32_t kTmemColumns = D == 256 ? 512 : 256;
-    static constexpr int kBlocksPerSm = D == 256 ? 1 : 2;
+    static constexpr uint32_t kTmemColumns = 512;
 };
 // Arrays of a tile's parameters.
 enum { kScaleK = 0, kMinK = 1, kScaleV = 2, kMinV = 3, kInverseV = 4, kRatioV = 5 };
@@ -75,8 +79,12 @@ __device__ __forceinline__ void TmemStore16(uint32_t addr, const uint32_t* r) {
                  : "memory");
 }
 __device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <int BAR>
-__device__ __forceinline__ void WarpsSync() { asm volatile("bar.sync %0, 128;" ::"n"(BAR) : "memory"); }
+__device__ __forceinline__ void WarpsSync(int barrier, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory"); }
+__device__ __forceinline__ float Max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 __device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
     return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
@@ -89,11 +97,12 @@ __device__ __forceinline__ int64_t WarpSum(int64_t v) {
     return v;
 }
 // Token tiles of all units of one kv head of a request, by a whole warp.
+template <int UNIT>
 __device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, const Request& r) {
     int64_t sum = 0;
-    for (int row = (threadIdx.x & 31) * kRows; row < r.rows; row += 32 * kRows) {
+    for (int row = (threadIdx.x & 31) * UNIT; row < r.rows; row += 32 * UNIT) {
         int a, b;
-        UnitTiles<kTokens>(p, r, row, kRows, &a, &b);
+        UnitTiles<kTokens>(p, r, row, UNIT, &a, &b);
         sum += b - a;
     }
     return WarpSum(sum);
@@ -108,16 +117,17 @@ struct Place {
     int t0, steps;              // this block's tiles of it
     Request req;
 };
-__device__ __forceinline__ void Settle(const AttentionParams& p, int64_t share_end, Place& u) {
+__device__ __forceinline__ void Settle(int64_t share_end, Place& u) {
     const int64_t left = share_end - u.at, tiles = u.tile_last - u.tile_first - u.into;
     u.t0 = u.tile_first + static_cast<int>(u.into);
     u.steps = static_cast<int>(tiles < left ? tiles : left);
 }
+template <int UNIT>
 __device__ __forceinline__ bool Advance(const AttentionParams& p, int64_t share_end, Place& u) {
     u.at += u.steps;
     if (u.at >= share_end) return false;
     u.into = 0;
-    u.row += kRows;
+    u.row += UNIT;
     if (u.row >= u.req.rows) {
         u.row = 0;
         if (++u.head == p.kv_heads) {
@@ -128,40 +138,48 @@ __device__ __forceinline__ bool Advance(const AttentionParams& p, int64_t share_
             } while (u.req.rows == 0);
         }
     }
-    UnitTiles<kTokens>(p, u.req, u.row, kRows, &u.tile_first, &u.tile_last);
-    Settle(p, share_end, u);
+    UnitTiles<kTokens>(p, u.req, u.row, UNIT, &u.tile_first, &u.tile_last);
+    Settle(share_end, u);
     return true;
 }
 
 template <int D, int DTYPE>
-__global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) PrefillKernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __grid_constant__ AttentionParams p) {
     using T = Tiles<D>;
+    constexpr int kThreads = T::kThreads, G = T::kQueryTiles, S = T::kStages, kUnit = T::kUnitRows;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(8) uint64_t bars[8];
-    uint64_t &q_full = bars[0], &k_full = bars[1], &k_empty = bars[2], &v_full = bars[3], &v_empty = bars[4], &s_full = bars[5], &p_full = bars[6], &o_full = bars[7];
+    __shared__ __align__(8) uint64_t q_full[G], s_full[G], p_full[G], o_done[G], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[2], back_full;
     __shared__ int64_t unit_work[kThreads];
-    __shared__ int64_t work_total, longest;
+    __shared__ int64_t work_total;
     __shared__ Place start;
     __shared__ uint32_t present[2][4];     // a bit per token of a tile that some row may see
     __shared__ float scale_range[2][4][2]; // smallest and largest value scale of those tokens, by unpacking warp
-    __shared__ float q_big[4];
-    __shared__ int join_last;
+    __shared__ float q_big[4 * G], unit_back;
+    __shared__ int join_last[G];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kUnpackWarp = T::kSoftmax / 32, kIssueWarp = kUnpackWarp + 4;
     if (threadIdx.x == 0) {
-        MbarInit(&q_full, 128);
-        MbarInit(&k_full, 128);
-        MbarInit(&k_empty, 1);
-        MbarInit(&v_full, 128);
-        MbarInit(&v_empty, 1);
-        MbarInit(&s_full, 1);
-        MbarInit(&p_full, 128);
-        MbarInit(&o_full, 1);
+        for (int g = 0; g < G; ++g) {
+            MbarInit(&q_full[g], 128);
+            MbarInit(&s_full[g], 1);
+            MbarInit(&p_full[g], 128);
+            MbarInit(&o_done[g], 1);
+        }
+        for (int s = 0; s < S; ++s) {
+            MbarInit(&k_full[s], 128);
+            MbarInit(&k_empty[s], 1);
+            MbarInit(&v_full[s], 128);
+            MbarInit(&v_empty[s], 1);
+        }
+        MbarInit(&params_full[0], 128);
+        MbarInit(&params_full[1], 128);
+        MbarInit(&back_full, 1);
         FenceBarrierInit();
     }
     // tensor memory is taken before the next kernel of the stream may start on this SM and take it
-    if (warp == 8) umma::TmemAlloc(&tmem_slot, T::kTmemColumns);
+    if (warp == kIssueWarp) umma::TmemAlloc(&tmem_slot, T::kTmemColumns);
     umma::FenceBeforeThreadSync();
     __syncthreads();
     umma::FenceAfterThreadSync();
@@ -170,7 +188,7 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
 
     // ---- this block's share ----------------------------------------------------------------------------------------------
     // A warp takes a request at a time; thread 0 adds.  Few requests have many rows.
-    if (threadIdx.x == 0) work_total = longest = 0;
+    if (threadIdx.x == 0) work_total = 0;
     __syncthreads();
     for (int base = 0; base < p.requests; base += kThreads) {
         const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
@@ -178,16 +196,16 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
             if (threadIdx.x < count) {
                 const Request r = LoadRequest(p, base + threadIdx.x);
                 int64_t sum = 0;
-                for (int row = 0; row < r.rows; row += kRows) {
+                for (int row = 0; row < r.rows; row += kUnit) {
                     int a, b;
-                    UnitTiles<kTokens>(p, r, row, kRows, &a, &b);
+                    UnitTiles<kTokens>(p, r, row, kUnit, &a, &b);
                     sum += b - a;
                 }
                 unit_work[threadIdx.x] = sum;
             }
         } else {
             for (int i = warp; i < count; i += kThreads / 32) {
-                const int64_t sum = RequestTiles(p, LoadRequest(p, base + i));
+                const int64_t sum = RequestTiles<kUnit>(p, LoadRequest(p, base + i));
                 if (lane == 0) unit_work[i] = sum;
             }
         }
@@ -213,7 +231,7 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
             if (p.requests > kThreads) {
                 __syncthreads();
                 for (int i = warp; i < count; i += kThreads / 32) {
-                    const int64_t sum = RequestTiles(p, LoadRequest(p, base + i));
+                    const int64_t sum = RequestTiles<kUnit>(p, LoadRequest(p, base + i));
                     if (lane == 0) unit_work[i] = sum;
                 }
                 __syncthreads();
@@ -241,10 +259,10 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                         u.head = static_cast<int>(Divide(off, per_head));
                         off -= u.head * per_head;
                         // rows, 32 units at a time
-                        for (int row = 0;; row += 32 * kRows) {
-                            const int my_row = row + lane * kRows;
+                        for (int row = 0;; row += 32 * kUnit) {
+                            const int my_row = row + lane * kUnit;
                             int a = 0, c = 0;
-                            if (my_row < u.req.rows) UnitTiles<kTokens>(p, u.req, my_row, kRows, &a, &c);
+                            if (my_row < u.req.rows) UnitTiles<kTokens>(p, u.req, my_row, kUnit, &a, &c);
                             int64_t upto = c - a;
 #pragma unroll
                             for (int o = 1; o < 32; o <<= 1) {
@@ -259,7 +277,7 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                                     u.tile_last = c;
                                     u.into = off - (upto - (c - a));
                                     u.at = share_begin;
-                                    Settle(p, share_end, u);
+                                    Settle(share_end, u);
                                     start = u;
                                 }
                                 break;
@@ -275,20 +293,17 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
         __syncthreads();
     }
 
-    uint8_t* const q_smem = smem;
-    uint8_t* const k_smem = smem + T::kOperandBytes;
-    uint8_t* const v_smem = smem + 2 * T::kOperandBytes;
     float* const params = reinterpret_cast<float*>(smem + T::kParams);
     bool failed = false;
     const auto wait = [&](uint64_t* bar, uint32_t parity, int detail) {
         if (!failed && !MbarWait(bar, parity, p.status, kSite, 16 + detail)) failed = true;
     };
 
-    if (busy && warp >= 4 && warp < 8) {
+    if (busy && warp >= kUnpackWarp && warp < kIssueWarp) {
         // ================================================ unpacking ==================================================
-        const int tid = threadIdx.x - 128;
+        const int tid = threadIdx.x - T::kSoftmax;
         Place u = start;
-        int64_t tile_count = 0;
+        uint32_t tile_count = 0, unit_count = 0;
         // this thread's 16-byte pieces: K piece j is 32 elements of a token, V piece j four words of a pair of tokens
         constexpr int kPieces = D / 32;
         uint4 kw[kPieces], vw[kPieces];
@@ -297,7 +312,7 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
         do {
             int first_low, last_high, unused;
             Visible(p, u.req, u.row / p.group, &first_low, &unused);
-            Visible(p, u.req, ((u.row + kRows < u.req.rows ? u.row + kRows : u.req.rows) - 1) / p.group, &unused, &last_high);
+            Visible(p, u.req, ((u.row + kUnit < u.req.rows ? u.row + kUnit : u.req.rows) - 1) / p.group, &unused, &last_high);
             const int32_t* table = p.table + static_cast<int64_t>(u.b) * p.max_blocks;
             // index of token `token` within its head, or -1 when no row sees it or its block does not exist
             const auto locate = [&](int token) -> int64_t {
@@ -344,29 +359,10 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
             load_k(0);
             load_v(0);
             for (int step = 0; step < u.steps; ++step, ++tile_count) {
-                const uint32_t par = static_cast<uint32_t>(tile_count & 1);
-                if (tile_count > 0) wait(&k_empty, par ^ 1u, 0);
-                // parameters, and the token's bit
-                {
-                    float* a = params + par * (T::kParamBytes / 4) + tid;
-                    const float vs = ParamScale(vp), vm = ParamMin(vp), inverse = Reciprocal(vs);
-                    a[kScaleK * kTokens] = ParamScale(kp);
-                    a[kMinK * kTokens] = ParamMin(kp);
-                    a[kScaleV * kTokens] = vs;
-                    a[kMinV * kTokens] = vm;
-                    if constexpr (DTYPE == FTH_B200_FP16) {
-                        a[kInverseV * kTokens] = inverse;
-                        a[kRatioV * kTokens] = vm * inverse;
-                    }
-                    const uint32_t bits = __ballot_sync(0xffffffffu, there);
-                    const uint32_t scale = there ? vp << 16 : 0u;
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, scale), low = __reduce_min_sync(0xffffffffu, there ? scale : 0x7f800000u);
-                    if (lane == 0) {
-                        present[par][warp - 4] = bits;
-                        scale_range[par][warp - 4][0] = __uint_as_float(low);
-                        scale_range[par][warp - 4][1] = __uint_as_float(top);
-                    }
-                }
+                const uint32_t stage = tile_count % S, turn = (tile_count / S) & 1u, par = tile_count & 1u;
+                uint8_t* const k_smem = smem + T::kKeys + stage * T::kOperandBytes;
+                uint8_t* const v_smem = smem + T::kKeys + (S + stage) * T::kOperandBytes;
+                if (tile_count >= S) wait(&k_empty[stage], turn ^ 1u, 0);
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
                     const int token = k_token(j), piece = k_piece(j);
@@ -380,9 +376,32 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                     }
                 }
                 FenceProxyAsync();
-                MbarArrive(&k_full);
+                MbarArrive(&k_full[stage]);
+                // parameters, and the token's bit; the tile two before is done with their place when its V is
+                if (tile_count >= S) wait(&v_empty[stage], turn ^ 1u, 1);
+                if (step == 0) wait(&back_full, unit_count & 1u, 9);
+                {
+                    float* a = params + par * (T::kParamBytes / 4) + tid;
+                    const float vs = ParamScale(vp), vm = ParamMin(vp);
+                    a[kScaleK * kTokens] = ParamScale(kp) * unit_back;
+                    a[kMinK * kTokens] = ParamMin(kp);
+                    a[kScaleV * kTokens] = vs;
+                    a[kMinV * kTokens] = vm;
+                    if constexpr (DTYPE == FTH_B200_FP16) {
+                        const float inverse = Reciprocal(vs);
+                        a[kInverseV * kTokens] = inverse;
+                        a[kRatioV * kTokens] = vm * inverse;
+                    }
+                    const uint32_t bits = __ballot_sync(0xffffffffu, there);
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, there ? vp << 16 : 0u), low = __reduce_min_sync(0xffffffffu, there ? vp << 16 : 0x7f800000u);
+                    if (lane == 0) {
+                        present[par][warp - kUnpackWarp] = bits;
+                        scale_range[par][warp - kUnpackWarp][0] = __uint_as_float(low);
+                        scale_range[par][warp - kUnpackWarp][1] = __uint_as_float(top);
+                    }
+                }
+                MbarArrive(&params_full[par]);
                 if (step + 1 < u.steps) load_k(step + 1);
-                if (tile_count > 0) wait(&v_empty, par ^ 1u, 1);
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
                     const int pair = v_pair(j), piece = v_piece(j);
@@ -401,61 +420,83 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                     }
                 }
                 FenceProxyAsync();
-                MbarArrive(&v_full);
+                MbarArrive(&v_full[stage]);
                 if (step + 1 < u.steps) load_v(step + 1);
             }
-        } while (Advance(p, share_end, u));
-    } else if (busy && warp == 8) {
+            ++unit_count;
+        } while (Advance<kUnit>(p, share_end, u));
+    } else if (busy && warp == kIssueWarp) {
         // ================================================ products ===================================================
         if (lane == 0) {
             Place u = start;
             const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, true, kRows, D);
-            const uint32_t q_addr = SmemAddr(q_smem), k_addr = SmemAddr(k_smem), v_addr = SmemAddr(v_smem);
-            const uint32_t s_tmem = tmem, o_tmem = tmem + 128;
-            int64_t tile_count = 0;
-            uint32_t unit_count = 0;
+            const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
+            uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
+            const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
+                // S is written where the last tile's P was read
+                if (used[g] > 0) wait(&o_done[g], (used[g] - 1) & 1u, 8);
+                umma::FenceAfterThreadSync();
+                if (failed) return;
+                const uint32_t q = q_addr + g * T::kOperandBytes, k = k_addr + (tile % S) * T::kOperandBytes;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t at = (i >> 2) * T::kPieceBytes + (i & 3) * 32;
+                    MmaShared(tmem + g * 256, umma::SmemDesc(q + at, 0, 1024), umma::SmemDesc(k + at, 0, 1024), s_desc, i > 0);
+                }
+                umma::Commit(&s_full[g]);
+            };
+            const auto values = [&](int g, uint32_t tile, bool first) {
+                wait(&p_full[g], used[g] & 1u, 4);
+                umma::FenceAfterThreadSync();
+                if (failed) return;
+                const uint32_t v = v_addr + (tile % S) * T::kOperandBytes;
+#pragma unroll
+                for (int i = 0; i < kTokens / 16; ++i)
+                    MmaTensor(tmem + g * 256 + 128, tmem + g * 256 + i * 8, umma::SmemDesc(v + i * 2048, T::kPieceBytes, 1024), o_desc, !first || i > 0);
+                umma::Commit(&o_done[g]);
+                ++used[g];
+            };
             do {
-                wait(&q_full, unit_count & 1u, 2);
-                for (int step = 0; step < u.steps; ++step, ++tile_count) {
-                    const uint32_t par = static_cast<uint32_t>(tile_count & 1);
-                    wait(&k_full, par, 3);
-                    if (tile_count > 0) wait(&v_empty, par ^ 1u, 8);  // S is written where the last tile's P was read
-                    umma::FenceAfterThreadSync();
-                    if (failed) break;
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t at = (i >> 2) * T::kPieceBytes + (i & 3) * 32;
-                        MmaShared(s_tmem, umma::SmemDesc(q_addr + at, 0, 1024), umma::SmemDesc(k_addr + at, 0, 1024), s_desc, i > 0);
+                const int active = u.req.rows - u.row > kRows ? G : 1;   // tiles of rows that have any
+                wait(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+                for (int g = 0; g < active; ++g) {
+                    wait(&q_full[g], unit_count & 1u, 2);
+                    scores(g, tile_count);
+                }
+                umma::Commit(&k_empty[tile_count % S]);
+                for (int step = 0; step < u.steps && !failed; ++step, ++tile_count) {
+                    const bool more = step + 1 < u.steps;
+                    const uint32_t next = tile_count + 1;
+                    wait(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
+                    for (int g = 0; g < active; ++g) {
+                        values(g, tile_count, step == 0);
+                        if (g + 1 == active) umma::Commit(&v_empty[tile_count % S]);
+                        if (more) {
+                            if (g == 0) wait(&k_full[next % S], (next / S) & 1u, 3);
+                            scores(g, next);
+                            if (g + 1 == active) umma::Commit(&k_empty[next % S]);
+                        }
                     }
-                    umma::Commit(&s_full);
-                    umma::Commit(&k_empty);
-                    wait(&p_full, par, 4);
-                    wait(&v_full, par, 5);
-                    umma::FenceAfterThreadSync();
-                    if (failed) break;
-#pragma unroll
-                    for (int i = 0; i < kTokens / 16; ++i)
-                        MmaTensor(o_tmem, s_tmem + i * 8, umma::SmemDesc(v_addr + i * 2048, T::kPieceBytes, 1024), o_desc, step > 0 || i > 0);
-                    umma::Commit(&v_empty);
-                    if (step + 1 == u.steps) umma::Commit(&o_full);
                 }
                 ++unit_count;
-            } while (!failed && Advance(p, share_end, u));
+            } while (!failed && Advance<kUnit>(p, share_end, u));
         }
-    } else if (busy && warp < 4) {
+    } else if (busy && warp < kUnpackWarp) {
         // ================================================ softmax ====================================================
-        const int r = threadIdx.x;             // row of the unit, lane of tensor memory
-        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-        const uint32_t s_tmem = tmem + lanes, o_tmem = tmem + 128 + lanes;
+        const int g = warp >> 2;                   // tile of rows
+        const int r = threadIdx.x & 127;           // row of the tile, lane of tensor memory
+        const uint32_t s_tmem = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * 256, o_tmem = s_tmem + 128;
+        uint8_t* const q_smem = smem + g * T::kOperandBytes;
         Place u = start;
-        int64_t tile_count = 0;
-        uint32_t unit_count = 0;
+        uint32_t tile_count = 0, unit_count = 0, used = 0;
         for (;;) {
             // ---- the unit's queries, as operands
-            const bool valid = u.row + r < u.req.rows;
-            const int query = valid ? (u.row + r) / p.group : 0;
+            const int row = u.row + g * kRows + r;
+            const bool active = g == 0 || u.req.rows - u.row > kRows;
+            const bool valid = row < u.req.rows;
+            const int query = valid ? row / p.group : 0;
             const uint16_t* from = static_cast<const uint16_t*>(p.q) + (u.req.first_row + static_cast<int64_t>(query)) * p.ldq +
-                                   (static_cast<int64_t>(u.head) * p.group + (u.row + r - query * p.group)) * D;
+                                   (static_cast<int64_t>(u.head) * p.group + (row - query * p.group)) * D;
             float big = 0.0f, qsum = 0.0f;
             if (valid) {
 #pragma unroll 4
@@ -473,10 +514,15 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             if (lane == 0) q_big[warp] = big;
-            WarpsSync<1>();
-            big = fmaxf(fmaxf(q_big[0], q_big[1]), fmaxf(q_big[2], q_big[3]));
+            WarpsSync(3, T::kSoftmax);
+#pragma unroll
+            for (int w = 0; w < 4 * G; ++w) big = fmaxf(big, q_big[w]);
             const int e = QueryExponent(big);
-            const float up = PowerOfTwo(e), back = p.scale_log2 * PowerOfTwo(24 - e);
+            const float up = PowerOfTwo(e);
+            if (threadIdx.x == 0) {
+                unit_back = p.scale_log2 * PowerOfTwo(24 - e);
+                MbarArrive(&back_full);
+            }
             qsum *= p.scale_log2;
 #pragma unroll 4
             for (int w = 0; w < D / 8; ++w) {
@@ -488,7 +534,7 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                 *reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + r * 128 + (((w & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
             }
             FenceProxyAsync();
-            MbarArrive(&q_full);
+            MbarArrive(&q_full[g]);
             int low = 0, high = 0;
             if (valid) Visible(p, u.req, query, &low, &high);
 
@@ -497,9 +543,11 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
             float ref = 0.0f, limit = kNotStarted, scale_limit = 0.0f;
             int k = 0;
             float2 sum = make_float2(0.0f, 0.0f), mass = sum, offset = sum;
-            for (int step = 0; step < u.steps; ++step, ++tile_count) {
-                const uint32_t par = static_cast<uint32_t>(tile_count & 1);
-                wait(&s_full, par, 6);
+            if (!active) tile_count += u.steps;   // no rows
+            for (int step = 0; active && step < u.steps; ++step, ++tile_count, ++used) {
+                const uint32_t par = tile_count & 1u;
+                wait(&params_full[par], (tile_count >> 1) & 1u, 10);
+                wait(&s_full[g], used & 1u, 6);
                 umma::FenceAfterThreadSync();
                 const float* a = params + par * (T::kParamBytes / 4);
                 const int token0 = (u.t0 + step) * kTokens;
@@ -527,15 +575,12 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                     float best = -INFINITY;
                     const float4* ks = reinterpret_cast<const float4*>(a + kScaleK * kTokens + c * 32);
                     const float4* km = reinterpret_cast<const float4*>(a + kMinK * kTokens + c * 32);
-                    const float2 qq = make_float2(qsum, qsum), rr = make_float2(-ref, -ref), bb = make_float2(back, back);
+                    const float2 qq = make_float2(qsum, qsum), rr = make_float2(-ref, -ref);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float4 s4 = ks[i], m4 = km[i];
-                        float2 t0 = Fma2(make_float2(m4.x, m4.y), qq, rr), t1 = Fma2(make_float2(m4.z, m4.w), qq, rr);
-                        const float2 v0 = Mul2(make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), bb);
-                        const float2 v1 = Mul2(make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), bb);
-                        z[2 * i] = Fma2(make_float2(s4.x, s4.y), v0, t0);
-                        z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), v1, t1);
+                        z[2 * i] = Fma2(make_float2(s4.x, s4.y), make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), Fma2(make_float2(m4.x, m4.y), qq, rr));
+                        z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), Fma2(make_float2(m4.z, m4.w), qq, rr));
                     }
                     if (!inside) {
 #pragma unroll
@@ -548,7 +593,7 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) best = fmaxf(best, fmaxf(z[i].x, z[i].y));
+                    for (int i = 0; i < 16; ++i) best = Max3(best, z[i].x, z[i].y);
                     if (__any_sync(0xffffffffu, best > limit || new_k != k)) {
                         // move the maximum: scores of this chunk, the weights of the tile's earlier ones, sums and results
                         const bool first = limit == kNotStarted;
@@ -653,22 +698,23 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                 }
                 TmemStoreWait();
                 umma::FenceBeforeThreadSync();
-                MbarArrive(&p_full);
+                MbarArrive(&p_full[g]);
             }
 
             // ---- the unit's results
-            wait(&o_full, unit_count & 1u, 7);
+            if (active) wait(&o_done[g], (used - 1) & 1u, 7);
             umma::FenceAfterThreadSync();
             const float all = mass.x + mass.y, total = DTYPE == FTH_B200_FP16 ? sum.x + sum.y : all, shift = offset.x + offset.y;
             const int64_t unit_begin = u.at - u.into, unit_end = unit_begin + (u.tile_last - u.tile_first);
             const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : Divide(unit_begin, per);
             const int64_t part_last = unit_end <= share_end ? blockIdx.x : Divide(unit_end - 1, per);
             const bool whole = part_first == part_last;
-            const int64_t slot_floats = static_cast<int64_t>(kRows) * kRow<D>;
-            float* partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == part_first ? 1 : 0)) * slot_floats + r * kRow<D>;
+            const int64_t slot_floats = static_cast<int64_t>(kUnit) * kRow<D>;
+            float* const tile_partials = p.partials + g * kRows * kRow<D>;
+            float* partial = tile_partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == part_first ? 1 : 0)) * slot_floats + r * kRow<D>;
             const float best = limit == kNotStarted ? kNoMax : ref;
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
+            for (int c = 0; active && c < D / 16; ++c) {
                 uint32_t w[16];
                 __syncwarp();
                 umma::TmemLoad16(o_tmem + c * 16, w);
@@ -679,55 +725,57 @@ __global__ void __launch_bounds__(kBoundThreads, Tiles<D>::kBlocksPerSm) Prefill
                     const float unit = 16777216.0f;
                     const float4 v = make_float4(fmaf(__uint_as_float(w[i]), unit, shift), fmaf(__uint_as_float(w[i + 1]), unit * 0.0625f, shift),
                                                  fmaf(__uint_as_float(w[i + 2]), unit, shift), fmaf(__uint_as_float(w[i + 3]), unit * 0.0625f, shift));
-                    if (whole) StoreFour<D, DTYPE>(p, u.req, u.head, u.row + r, c * 16 + i, v, total, best, all);
+                    if (whole) StoreFour<D, DTYPE>(p, u.req, u.head, row, c * 16 + i, v, total, best, all);
                     else *reinterpret_cast<float4*>(partial + c * 16 + i) = v;
                 }
             }
-            if (!whole) {
+            if (active && !whole) {
                 if (valid) *reinterpret_cast<float4*>(partial + D) = make_float4(best, 0.0f, total, all);
                 const int parts = static_cast<int>(part_last - part_first) + 1;
+                const auto sync = [&] { WarpsSync(1 + g, 128); };
                 __threadfence();
-                WarpsSync<1>();
-                if (threadIdx.x == 0) {
-                    join_last = atomicAdd(&p.counters[part_first], 1) == parts - 1;
-                    if (join_last) p.counters[part_first] = 0;
+                sync();
+                if (r == 0) {
+                    int* const counter = &p.counters[part_first * G + g];
+                    join_last[g] = atomicAdd(counter, 1) == parts - 1;
+                    if (join_last[g]) *counter = 0;
                 }
-                WarpsSync<1>();
-                if (join_last) {
+                sync();
+                if (join_last[g]) {
                     __threadfence();
-                    const int rows = u.req.rows - u.row < kRows ? u.req.rows - u.row : kRows;
+                    const int rows = u.req.rows - u.row - g * kRows < kRows ? u.req.rows - u.row - g * kRows : kRows;
                     // the query operands' memory: every product that read it is done
-                    JoinParts<D, DTYPE, 128>(p, u.req, u.head, u.row, rows, static_cast<int>(part_first), parts, slot_floats,
-                                             reinterpret_cast<float*>(q_smem), T::kOperandBytes / 4, threadIdx.x, WarpsSync<1>);
+                    JoinParts<D, DTYPE, 128>(p, u.req, u.head, u.row + g * kRows, rows, tile_partials, static_cast<int>(part_first), parts, slot_floats,
+                                             reinterpret_cast<float*>(q_smem), T::kOperandBytes / 4, r, sync);
                 }
             }
             ++unit_count;
             umma::FenceBeforeThreadSync();
-            if (!Advance(p, share_end, u)) break;
+            if (!Advance<kUnit>(p, share_end, u)) break;
         }
     }
     __syncwarp();
     umma::FenceBeforeThreadSync();
     __syncthreads();
     umma::FenceAfterThreadSync();
-    if (warp == 8) umma::TmemDealloc(tmem, T::kTmemColumns);
+    if (warp == kIssueWarp) umma::TmemDealloc(tmem, T::kTmemColumns);
 }
 
 template <int D, int DTYPE>
 int LaunchTyped(const AttentionParams& p, int grid, cudaStream_t s) {
     const auto kernel = PrefillKernel<D, DTYPE>;
     if (EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), Tiles<D>::kBytes) != FTH_B200_OK) return FTH_B200_ERR_CUDA;
-    return Launch(kernel, dim3(static_cast<unsigned>(grid)), kThreads, Tiles<D>::kBytes, s, p);
+    return Launch(kernel, dim3(static_cast<unsigned>(grid)), Tiles<D>::kThreads, Tiles<D>::kBytes, s, p);
 }
 
 }  // namespace
 
-int PrefillGrid(int head_dim) { return SmCount() * (head_dim == 256 ? Tiles<256>::kBlocksPerSm : Tiles<128>::kBlocksPerSm); }
+int PrefillGrid() { return SmCount(); }
 
-int64_t PrefillPartialFloats(int head_dim) { return static_cast<int64_t>(PrefillGrid(head_dim)) * 2 * kRows * (head_dim + 4); }
+int64_t PrefillPartialFloats(int head_dim) { return static_cast<int64_t>(PrefillGrid()) * 2 * (head_dim == 256 ? 1 : 2) * kRows * (head_dim + 4); }
 
 int LaunchPrefill(const AttentionParams& p, int head_dim, int dtype, cudaStream_t s) {
-    const int grid = PrefillGrid(head_dim);
+    const int grid = PrefillGrid();
     if (dtype == FTH_B200_BF16) {
         if (head_dim == 64) return LaunchTyped<64, FTH_B200_BF16>(p, grid, s);
         if (head_dim == 128) return LaunchTyped<128, FTH_B200_BF16>(p, grid, s);

@@ -6,7 +6,7 @@
 namespace fth {
 namespace kv4 {
 
-int PrefillGrid(int head_dim);              // blocks of threads
+int PrefillGrid();                          // blocks of threads; two arrival counters each
 int64_t PrefillPartialFloats(int head_dim); // room for partial results
 int LaunchPrefill(const AttentionParams& p, int head_dim, int dtype, cudaStream_t s);
 
