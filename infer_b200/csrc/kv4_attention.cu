@@ -808,7 +808,7 @@ extern "C" int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* d, fth_
     p.causal = d->causal != 0;
     p.window = d->window;
     p.q_vec = kv4::AlignedTo(d->q, 16) && p.ldq % 8 == 0;
-    p.out_vec = kv4::AlignedTo(d->out, 8) && p.ldo % 4 == 0;
+    p.out_vec = kv4::AlignedTo(d->out, 16) && p.ldo % 8 == 0;
     p.scale_log2 = d->scale * 1.4426950408889634f;
     p.status = DeviceStatusPtr();
     p.counters = static_cast<int*>(d->workspace);

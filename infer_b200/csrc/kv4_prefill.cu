@@ -314,32 +314,39 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             Visible(p, u.req, u.row / p.group, &first_low, &unused);
             Visible(p, u.req, ((u.row + kUnit < u.req.rows ? u.row + kUnit : u.req.rows) - 1) / p.group, &unused, &last_high);
             const int32_t* table = p.table + static_cast<int64_t>(u.b) * p.max_blocks;
-            // index of token `token` within its head, or -1 when no row sees it or its block does not exist
-            const auto locate = [&](int token) -> int64_t {
-                if (token >= last_high || token < (first_low & ~15)) return -1;
-                const int id = table[token >> p.cache.block_shift];
-                if (id < 0 || id >= p.cache.blocks) {
-                    ReportTimeout(p.status, kSiteAttention, u.b);
-                    return -1;
-                }
-                return HeadBase(p.cache, id, u.head) + (token & ((1 << p.cache.block_shift) - 1));
-            };
             // K: neighbouring lanes take the halves of 64 bytes of four tokens, then further 64-byte pieces, so that the eight
             // lanes of a store phase hit eight different 16-byte columns
             const auto k_token = [&](int j) { return ((tid + 128 * j) >> 1 & 3) | ((tid + 128 * j) / (4 * kPieces) << 2); };
             const auto k_piece = [&](int j) { return ((tid + 128 * j) & 1) | (((tid + 128 * j) >> 3) % (kPieces / 2) << 1); };
+            // block numbers of the tokens of this thread's pieces (both kinds lie in the same sixteen tokens) and of its own
+            // token, fetched a tile before they are needed; -1: no row sees the tokens
+            int ids[kPieces], own_id;
+            const auto lookup = [&](int step) {
+                const auto at = [&](int in_tile) {
+                    const int token = (u.t0 + step) * kTokens + (in_tile & ~15);
+                    return step < u.steps && token < last_high && token + 16 > first_low ? table[token >> p.cache.block_shift] : -1;
+                };
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) ids[j] = at(k_token(j));
+                own_id = at(tid);
+            };
+            // a number that is no block hides its tokens
+            const auto exists = [&](int id) { return id >= 0 && id < p.cache.blocks; };
+            const auto index = [&](int id, int step, int in_tile) {
+                return HeadBase(p.cache, id, u.head) + (((u.t0 + step) * kTokens + in_tile) & ((1 << p.cache.block_shift) - 1));
+            };
             const auto load_k = [&](int step) {
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
-                    const int64_t at = locate((u.t0 + step) * kTokens + k_token(j));
                     kw[j] = make_uint4(0, 0, 0, 0);
-                    if (at >= 0) kw[j] = LoadStream16(p.cache.k_codes + at * (D / 2) + k_piece(j) * 16);
+                    if (exists(ids[j])) kw[j] = LoadStream16(p.cache.k_codes + index(ids[j], step, k_token(j)) * (D / 2) + k_piece(j) * 16);
                 }
                 const int token = (u.t0 + step) * kTokens + tid;
-                const int64_t at = locate(token);
-                there = at >= 0 && token >= first_low;
+                there = exists(own_id) && token >= first_low && token < last_high;
+                if (!exists(own_id) && token >= first_low && token < last_high) ReportTimeout(p.status, kSiteAttention, u.b);
                 kp = vp = 0;
                 if (there) {
+                    const int64_t at = index(own_id, step, tid);
                     kp = p.cache.k_params[at];
                     vp = p.cache.v_params[at];
                 }
@@ -350,14 +357,15 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const auto load_v = [&](int step) {
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
-                    const int pair = v_pair(j), piece = v_piece(j);
-                    const int64_t at = locate((u.t0 + step) * kTokens + 2 * pair);
                     vw[j] = make_uint4(0, 0, 0, 0);
-                    if (at >= 0) vw[j] = LoadStream16(p.cache.v_codes + at * (D / 2) + piece * 16);
+                    if (exists(ids[j])) vw[j] = LoadStream16(p.cache.v_codes + index(ids[j], step, 2 * v_pair(j)) * (D / 2) + v_piece(j) * 16);
                 }
             };
+            static_assert(kTokens == 128, "piece j of K and of V lie in the same sixteen tokens");
+            lookup(0);
             load_k(0);
             load_v(0);
+            lookup(1);
             for (int step = 0; step < u.steps; ++step, ++tile_count) {
                 const uint32_t stage = tile_count % S, turn = (tile_count / S) & 1u, par = tile_count & 1u;
                 uint8_t* const k_smem = smem + T::kKeys + stage * T::kOperandBytes;
@@ -421,7 +429,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 }
                 FenceProxyAsync();
                 MbarArrive(&v_full[stage]);
-                if (step + 1 < u.steps) load_v(step + 1);
+                if (step + 1 < u.steps) {
+                    load_v(step + 1);
+                    lookup(step + 2);
+                }
             }
             ++unit_count;
         } while (Advance<kUnit>(p, share_end, u));
@@ -497,19 +508,31 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const int query = valid ? row / p.group : 0;
             const uint16_t* from = static_cast<const uint16_t*>(p.q) + (u.req.first_row + static_cast<int64_t>(query)) * p.ldq +
                                    (static_cast<int64_t>(u.head) * p.group + (row - query * p.group)) * D;
+            // the row stays in registers between the two passes when it fits (all its loads in flight together)
+            constexpr int kHeld = D <= 128 ? D / 8 : 1;
+            uint4 held[kHeld];
+            const auto fetch = [&](int w) {
+                if (!valid) return make_uint4(0, 0, 0, 0);
+                return p.q_vec ? *reinterpret_cast<const uint4*>(from + w * 8) : LoadUnaligned8(from + w * 8);
+            };
             float big = 0.0f, qsum = 0.0f;
-            if (valid) {
-#pragma unroll 4
-                for (int w = 0; w < D / 8; ++w) {
-                    const uint4 x = p.q_vec ? *reinterpret_cast<const uint4*>(from + w * 8) : LoadUnaligned8(from + w * 8);
-                    const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
+            const auto measure = [&](uint4 x) {
+                const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 v = HalfPair<DTYPE>(raw[i]);
-                        big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
-                        qsum += v.x + v.y;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = HalfPair<DTYPE>(raw[i]);
+                    big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+                    qsum += v.x + v.y;
                 }
+            };
+            if constexpr (D <= 128) {
+#pragma unroll
+                for (int w = 0; w < D / 8; ++w) held[w] = fetch(w);
+#pragma unroll
+                for (int w = 0; w < D / 8; ++w) measure(held[w]);
+            } else {
+#pragma unroll 8
+                for (int w = 0; w < D / 8; ++w) measure(fetch(w));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
@@ -524,14 +547,18 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 MbarArrive(&back_full);
             }
             qsum *= p.scale_log2;
-#pragma unroll 4
-            for (int w = 0; w < D / 8; ++w) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (valid) x = p.q_vec ? *reinterpret_cast<const uint4*>(from + w * 8) : LoadUnaligned8(from + w * 8);
+            const auto place = [&](int w, uint4 x) {
                 const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
                 uint32_t f[4];
                 QueryOperands<DTYPE>(raw, up, f);
                 *reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + r * 128 + (((w & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            };
+            if constexpr (D <= 128) {
+#pragma unroll
+                for (int w = 0; w < D / 8; ++w) place(w, held[w]);
+            } else {
+#pragma unroll 8
+                for (int w = 0; w < D / 8; ++w) place(w, fetch(w));
             }
             FenceProxyAsync();
             MbarArrive(&q_full[g]);
@@ -713,6 +740,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             float* const tile_partials = p.partials + g * kRows * kRow<D>;
             float* partial = tile_partials + (static_cast<int64_t>(blockIdx.x) * 2 + (blockIdx.x == part_first ? 1 : 0)) * slot_floats + r * kRow<D>;
             const float best = limit == kNotStarted ? kNoMax : ref;
+            const int q_head = u.head * p.group + row - query * p.group;
+            const int64_t q_row = u.req.first_row + static_cast<int64_t>(query);
+            uint16_t* const out = static_cast<uint16_t*>(p.out) + q_row * p.ldo + static_cast<int64_t>(q_head) * D;
+            const float scale = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+            const float even = 16777216.0f, odd = 1048576.0f;   // 2^24, 2^20: what the codes' places make of them
 #pragma unroll 1
             for (int c = 0; active && c < D / 16; ++c) {
                 uint32_t w[16];
@@ -720,15 +752,24 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 umma::TmemLoad16(o_tmem + c * 16, w);
                 umma::TmemLoadWait();
                 if (!valid || failed) continue;   // a wait that gave up is in the status word; nothing is stored then
+                float v[16];
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float unit = 16777216.0f;
-                    const float4 v = make_float4(fmaf(__uint_as_float(w[i]), unit, shift), fmaf(__uint_as_float(w[i + 1]), unit * 0.0625f, shift),
-                                                 fmaf(__uint_as_float(w[i + 2]), unit, shift), fmaf(__uint_as_float(w[i + 3]), unit * 0.0625f, shift));
-                    if (whole) StoreFour<D, DTYPE>(p, u.req, u.head, row, c * 16 + i, v, total, best, all);
-                    else *reinterpret_cast<float4*>(partial + c * 16 + i) = v;
+                for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(w[i]), (i & 1) ? odd : even, shift);
+                if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        float eight[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) eight[j] = total == 0.0f ? 0.0f : v[i + j] * scale;
+                        rowops::WriteEight<DTYPE>(out, c * 16 + i, p.out_vec != 0, eight);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(partial + c * 16 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 }
             }
+            if (active && whole && valid && !failed && p.lse != nullptr)
+                p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(all)) * 0.6931471805599453f;
             if (active && !whole) {
                 if (valid) *reinterpret_cast<float4*>(partial + D) = make_float4(best, 0.0f, total, all);
                 const int parts = static_cast<int>(part_last - part_first) + 1;
