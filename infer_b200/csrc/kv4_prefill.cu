@@ -1,17 +1,19 @@
 // Attention over the 4-bit cache, many query rows per kv head (prompts, chunks of them, long drafts).
 //
-// The same arithmetic as in kv4_attention.cu on the tensor cores of sm_100: a tile of 128 query rows (queries x heads of
-// the group, so a group shares every key) against tiles of 128 tokens,
+// A tile of 128 query rows (queries x heads of the group, so a group shares every key) against tiles of 128 tokens,
 //     S = Q C_k^T   tcgen05.mma kind::f16, both operands in shared memory, accumulator in tensor memory
-//     P = exp2(s_k S + m_k sum(q) - maximum) s_v, rounded to FP16, written over S in tensor memory
-//     O = O + P C_v   the probabilities read from tensor memory
-// with the codes as half-precision numbers: c * 2^-24 in the low four bits, 16 c * 2^-24 four bits higher, both exact
-// (kv4_attention.cu).  Four warps unpack: a word of eight K codes is five operations and one 16-byte store (q has its
-// elements in the order this gives), a word of V codes eight operations (a byte spread to two halves and one AND each), in
-// natural order with every second element times 16, which the results are divided by.  K tiles are K-major operands, V
-// tiles MN-major ones (a row per token), both with the 128-byte swizzle; the unpacking warps hold the next tile's words in
-// registers while the matrix unit still reads the present one.  Four more warps own a query row per thread: scores out of
-// tensor memory 32 at a time, two FMAs each on pairs, one exp2, and the sums.  One thread issues the matrix instructions.
+//     P = exp2(s_k S + m_k sum(q) - maximum), rounded to FP16, written over S in tensor memory
+//     O = O + P V   the probabilities read from tensor memory
+// Keys enter as their codes: c * 2^-24 in the low four bits of a half-precision number and 16 c * 2^-24 four bits higher,
+// both exact (kv4_attention.cu), eight codes in five operations and one 16-byte store; q has its elements in the order
+// this gives.  Values enter as numbers, minimum + scale * code rounded once to FP16 (11 bits) after a power of two that
+// brings the largest of the tokens so far to 2^14: a scale and a minimum per token would have to be handed to every row of
+// probabilities, and what a warp reads from shared memory for all its lanes costs as much as 32 different words.  The
+// rounding moves a result by at most 2^-12 of the values it averages, as the rounding of the probabilities does.
+// Four warps unpack, holding the next tile's words in registers while the matrix unit still reads the present one.  Four
+// more per tile of rows own a row per thread: scores out of tensor memory 32 at a time, two FMAs on pairs, one exp2, the
+// sum.  One thread issues the matrix instructions.  All operands are K-major with the 128-byte swizzle.
+//
 // A block of threads has two tiles of query rows (one for 256-wide heads, whose results fill tensor memory) that share the
 // unpacked tokens: while one's scores become probabilities the matrix unit works for the other.  Unpacked tiles are
 // double-buffered (not for 256-wide heads, where shared memory holds one).
@@ -33,6 +35,8 @@ namespace {
 constexpr int kRows = 128;          // query rows of a tile
 constexpr int kTokens = 128;        // tokens of a tile
 constexpr int kSite = kSiteAttentionWait;
+constexpr int kNoExponent = 1000;
+constexpr float kProbabilityUp = 7.0f;  // probabilities are kept times 2^7: up to 2^15 with a lagging maximum, FP16's normal range down to 2^-21
 
 template <int D>
 struct Tiles {
@@ -46,13 +50,10 @@ struct Tiles {
     static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V of one tile
     static constexpr int kKeys = kQueryTiles * kOperandBytes;      // stages of K, then of V
     static constexpr int kParams = kKeys + 2 * kStages * kOperandBytes;
-    static constexpr int kParamBytes = 6 * kTokens * 4;            // of one tile; two tiles' worth
+    static constexpr int kParamBytes = 2 * kTokens * 4;            // of one tile's keys; two tiles' worth
     static constexpr size_t kBytes = kParams + 2 * kParamBytes + 1024;  // 1024: alignment
     static constexpr uint32_t kTmemColumns = 512;
 };
-// Arrays of a tile's parameters.
-enum { kScaleK = 0, kMinK = 1, kScaleV = 2, kMinV = 3, kInverseV = 4, kRatioV = 5 };
-
 __device__ __forceinline__ void MmaShared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
@@ -79,6 +80,17 @@ __device__ __forceinline__ void TmemStore16(uint32_t addr, const uint32_t* r) {
                  : "memory");
 }
 __device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Two tokens' values of one element: codes in bits 0 .. 3 of both halves of x (HIGH: bits 4 .. 7), times scale, plus minimum.
+// 1024 + c and 1024 + 16 c are half-precision numbers made by an OR, c = (1024 + c) - 1024 = (1024 + 16 c) / 16 - 64 exactly.
+template <int HIGH>
+__device__ __forceinline__ uint32_t ValuePair(uint32_t x, uint32_t scale, uint32_t minimum) {
+    const uint32_t bits = (x & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+    const __half2 n = *reinterpret_cast<const __half2*>(&bits);
+    const __half2 c = HIGH ? __hfma2(n, __half2half2(__ushort_as_half(0x2c00)), __half2half2(__ushort_as_half(0xd400)))
+                           : __hsub2(n, __half2half2(__ushort_as_half(0x6400)));
+    const __half2 v = __hfma2(c, *reinterpret_cast<const __half2*>(&scale), *reinterpret_cast<const __half2*>(&minimum));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ void WarpsSync(int barrier, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory"); }
 __device__ __forceinline__ float Max3(float a, float b, float c) {
     float d;
@@ -86,6 +98,20 @@ __device__ __forceinline__ float Max3(float a, float b, float c) {
     return d;
 }
 
+// The rows' results so far times `factor`, by the warp that owns them.
+template <int D>
+__device__ __forceinline__ void ScaleResults(uint32_t o_tmem, float factor) {
+#pragma unroll 1
+    for (int b = 0; b < D / 16; ++b) {
+        uint32_t w[16];
+        umma::TmemLoad16(o_tmem + b * 16, w);
+        umma::TmemLoadWait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * factor);
+        TmemStore16(o_tmem + b * 16, w);
+    }
+    TmemStoreWait();
+}
 __device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
     return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
 }
@@ -155,7 +181,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
     __shared__ int64_t work_total;
     __shared__ Place start;
     __shared__ uint32_t present[2][4];     // a bit per token of a tile that some row may see
-    __shared__ float scale_range[2][4][2]; // smallest and largest value scale of those tokens, by unpacking warp
+    __shared__ float value_up[2];          // power of two on the values of a tile
+    __shared__ float value_big[4];         // largest value of a tile, by unpacking warp
+    __shared__ __align__(16) __half value_scale[kTokens], value_min[kTokens];
     __shared__ float q_big[4 * G], unit_back;
     __shared__ int join_last[G];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -304,9 +332,14 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         const int tid = threadIdx.x - T::kSoftmax;
         Place u = start;
         uint32_t tile_count = 0, unit_count = 0;
-        // this thread's 16-byte pieces: K piece j is 32 elements of a token, V piece j four words of a pair of tokens
+        // K: this thread's 16-byte pieces, 32 elements of a token each.  V: eight tokens (four pairs) by kTaskWords words of four
+        // elements; neighbouring lanes take neighbouring eights of tokens, so that the eight lanes of a store phase hit eight
+        // different 16-byte columns.
+        constexpr int kTaskWords = D == 64 ? 2 : 4, kTasks = D / (32 * kTaskWords);
+        const int octet = tid & 15;
         constexpr int kPieces = D / 32;
-        uint4 kw[kPieces], vw[kPieces];
+        uint4 kw[kPieces];
+        uint32_t vw[kTasks][4][kTaskWords];
         uint32_t kp, vp;
         bool there;
         do {
@@ -318,9 +351,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             // lanes of a store phase hit eight different 16-byte columns
             const auto k_token = [&](int j) { return ((tid + 128 * j) >> 1 & 3) | ((tid + 128 * j) / (4 * kPieces) << 2); };
             const auto k_piece = [&](int j) { return ((tid + 128 * j) & 1) | (((tid + 128 * j) >> 3) % (kPieces / 2) << 1); };
-            // block numbers of the tokens of this thread's pieces (both kinds lie in the same sixteen tokens) and of its own
-            // token, fetched a tile before they are needed; -1: no row sees the tokens
-            int ids[kPieces], own_id;
+            // block numbers of the tokens of this thread's K pieces, of its V tokens and of its own token, fetched a tile before
+            // they are needed; -1: no row sees the tokens
+            int ids[kPieces], id_v, own_id;
             const auto lookup = [&](int step) {
                 const auto at = [&](int in_tile) {
                     const int token = (u.t0 + step) * kTokens + (in_tile & ~15);
@@ -328,6 +361,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 };
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) ids[j] = at(k_token(j));
+                id_v = at(octet * 8);
                 own_id = at(tid);
             };
             // a number that is no block hides its tokens
@@ -351,17 +385,28 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     vp = p.cache.v_params[at];
                 }
             };
-            // V: neighbouring lanes take 64 bytes of one pair of tokens, then of the next
-            const auto v_pair = [&](int j) { return ((tid + 128 * j) >> 2 & 1) | ((tid + 128 * j) / (8 * T::kBlocks64) << 1); };
-            const auto v_piece = [&](int j) { return ((tid + 128 * j) & 3) | (((tid + 128 * j) >> 3) % T::kBlocks64 << 2); };
             const auto load_v = [&](int step) {
+                const bool there_v = exists(id_v);
+                const uint8_t* from = p.cache.v_codes + (there_v ? index(id_v, step, octet * 8) * (D / 2) : 0);
 #pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
-                    vw[j] = make_uint4(0, 0, 0, 0);
-                    if (exists(ids[j])) vw[j] = LoadStream16(p.cache.v_codes + index(ids[j], step, 2 * v_pair(j)) * (D / 2) + v_piece(j) * 16);
-                }
+                for (int t = 0; t < kTasks; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint8_t* row = from + j * D + ((tid >> 4) + 8 * t) * (kTaskWords * 4);
+                        if constexpr (kTaskWords == 4) {
+                            const uint4 x = there_v ? LoadStream16(row) : make_uint4(0, 0, 0, 0);
+                            vw[t][j][0] = x.x;
+                            vw[t][j][1] = x.y;
+                            vw[t][j][2] = x.z;
+                            vw[t][j][3] = x.w;
+                        } else {
+                            const uint2 x = there_v ? *reinterpret_cast<const uint2*>(row) : make_uint2(0, 0);
+                            vw[t][j][0] = x.x;
+                            vw[t][j][1] = x.y;
+                        }
+                    }
             };
-            static_assert(kTokens == 128, "piece j of K and of V lie in the same sixteen tokens");
+            int up_exponent = kNoExponent;   // of the values, largest so far in the unit
             lookup(0);
             load_k(0);
             load_v(0);
@@ -389,42 +434,57 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 if (tile_count >= S) wait(&v_empty[stage], turn ^ 1u, 1);
                 if (step == 0) wait(&back_full, unit_count & 1u, 9);
                 {
-                    float* a = params + par * (T::kParamBytes / 4) + tid;
                     const float vs = ParamScale(vp), vm = ParamMin(vp);
-                    a[kScaleK * kTokens] = ParamScale(kp) * unit_back;
-                    a[kMinK * kTokens] = ParamMin(kp);
-                    a[kScaleV * kTokens] = vs;
-                    a[kMinV * kTokens] = vm;
-                    if constexpr (DTYPE == FTH_B200_FP16) {
-                        const float inverse = Reciprocal(vs);
-                        a[kInverseV * kTokens] = inverse;
-                        a[kRatioV * kTokens] = vm * inverse;
-                    }
+                    // a token with a scale that is no number spoils the rows that see it through its score; as a value it must not
+                    // reach the others (0 * NaN is no zero)
+                    const bool spoiled = there && (!(ParamScale(kp) < INFINITY) || !(vs < INFINITY) || !(fabsf(vm) < INFINITY));
+                    float* a = params + par * (T::kParamBytes / 4) + tid;
+                    a[0] = spoiled ? __uint_as_float(0x7fc00000u) : ParamScale(kp) * unit_back;
+                    a[kTokens] = ParamMin(kp);
                     const uint32_t bits = __ballot_sync(0xffffffffu, there);
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, there ? vp << 16 : 0u), low = __reduce_min_sync(0xffffffffu, there ? vp << 16 : 0x7f800000u);
+                    const float own_big = there && !spoiled ? fmaxf(fabsf(vm), fabsf(fmaf(15.0f, vs, vm))) : 0.0f;
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(own_big));
                     if (lane == 0) {
                         present[par][warp - kUnpackWarp] = bits;
-                        scale_range[par][warp - kUnpackWarp][0] = __uint_as_float(low);
-                        scale_range[par][warp - kUnpackWarp][1] = __uint_as_float(top);
+                        value_big[warp - kUnpackWarp] = __uint_as_float(top);
                     }
+                    WarpsSync(4, 128);
+                    const float big = fmaxf(fmaxf(value_big[0], value_big[1]), fmaxf(value_big[2], value_big[3]));
+                    if (big > 0.0f) {
+                        const int e = QueryExponent(big);
+                        if (up_exponent == kNoExponent || e < up_exponent) up_exponent = e;
+                    }
+                    const float up = PowerOfTwo(up_exponent == kNoExponent ? 0 : up_exponent);
+                    value_scale[tid] = __float2half_rn(there && !spoiled ? vs * up : 0.0f);
+                    value_min[tid] = __float2half_rn(there && !spoiled ? vm * up : 0.0f);
+                    if (tid == 0) value_up[par] = up;
+                    WarpsSync(4, 128);
                 }
                 MbarArrive(&params_full[par]);
                 if (step + 1 < u.steps) load_k(step + 1);
+                {
+                    const uint4 s4 = *reinterpret_cast<const uint4*>(&value_scale[octet * 8]), m4 = *reinterpret_cast<const uint4*>(&value_min[octet * 8]);
+                    const uint32_t sp[4] = {s4.x, s4.y, s4.z, s4.w}, mp[4] = {m4.x, m4.y, m4.z, m4.w};
+                    uint8_t* const block = v_smem + (octet >> 3) * (D * 128);
 #pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
-                    const int pair = v_pair(j), piece = v_piece(j);
-                    const uint32_t w[4] = {vw[j].x, vw[j].y, vw[j].z, vw[j].w};
+                    for (int t = 0; t < kTasks; ++t) {
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        // half v of the sixteen elements, of token 2 * pair + odd; the order of the halves alternates with the
-                        // pair, so that a store phase hits eight different 16-byte columns
-                        const int odd = s & 1, v = (s >> 1) ^ (pair & 1);
-                        const uint32_t x0 = v ? w[2] : w[0], x1 = v ? w[3] : w[1];
-                        const uint32_t low = odd ? 0x4242u : 0x4040u, high = odd ? 0x4343u : 0x4141u;
-                        const int token = 2 * pair + odd, column = 2 * (piece & 3) + v;
-                        *reinterpret_cast<uint4*>(v_smem + (piece >> 2) * T::kPieceBytes + token * 128 + ((column ^ (token & 7)) << 4)) =
-                            make_uint4(__byte_perm(x0, 0, low) & 0x00f0000fu, __byte_perm(x0, 0, high) & 0x00f0000fu,
-                                       __byte_perm(x1, 0, low) & 0x00f0000fu, __byte_perm(x1, 0, high) & 0x00f0000fu);
+                        for (int w = 0; w < kTaskWords; ++w) {
+                            uint32_t v[4][4];   // element, pair
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t x = vw[t][j][w], y = x >> 8;
+                                v[0][j] = ValuePair<0>(x, sp[j], mp[j]);
+                                v[1][j] = ValuePair<1>(x, sp[j], mp[j]);
+                                v[2][j] = ValuePair<0>(y, sp[j], mp[j]);
+                                v[3][j] = ValuePair<1>(y, sp[j], mp[j]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int element = (((tid >> 4) + 8 * t) * kTaskWords + w) * 4 + i;
+                                *reinterpret_cast<uint4*>(block + element * 128 + (((octet & 7) ^ (element & 7)) << 4)) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                            }
+                        }
                     }
                 }
                 FenceProxyAsync();
@@ -440,7 +500,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         // ================================================ products ===================================================
         if (lane == 0) {
             Place u = start;
-            const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, true, kRows, D);
+            const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
             const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
             uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
             const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
@@ -463,7 +523,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 const uint32_t v = v_addr + (tile % S) * T::kOperandBytes;
 #pragma unroll
                 for (int i = 0; i < kTokens / 16; ++i)
-                    MmaTensor(tmem + g * 256 + 128, tmem + g * 256 + i * 8, umma::SmemDesc(v + i * 2048, T::kPieceBytes, 1024), o_desc, !first || i > 0);
+                    MmaTensor(tmem + g * 256 + 128, tmem + g * 256 + i * 8, umma::SmemDesc(v + (i >> 2) * (D * 128) + (i & 3) * 32, 0, 1024), o_desc, !first || i > 0);
                 umma::Commit(&o_done[g]);
                 ++used[g];
             };
@@ -565,11 +625,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             int low = 0, high = 0;
             if (valid) Visible(p, u.req, query, &low, &high);
 
-            // ---- tiles.  Scores are kept relative to ref = maximum - k, where 2^k brings the value scales below 2^7: all sums
-            // and the weights carry the same factor 2^k, which the division at the end takes out.
-            float ref = 0.0f, limit = kNotStarted, scale_limit = 0.0f;
-            int k = 0;
-            float2 sum = make_float2(0.0f, 0.0f), mass = sum, offset = sum;
+            // ---- tiles.  Scores are kept relative to ref = maximum - 7.
+            float ref = 0.0f, limit = kNotStarted, up_now = 1.0f;
+            float2 mass = make_float2(0.0f, 0.0f);
             if (!active) tile_count += u.steps;   // no rows
             for (int step = 0; active && step < u.steps; ++step, ++tile_count, ++used) {
                 const uint32_t par = tile_count & 1u;
@@ -581,27 +639,19 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 const uint32_t pr[4] = {present[par][0], present[par][1], present[par][2], present[par][3]};
                 const bool all_there = (pr[0] & pr[1] & pr[2] & pr[3]) == 0xffffffffu;
                 const bool inside = all_there && __all_sync(0xffffffffu, !valid || (token0 >= low && token0 + kTokens <= high));
-                float biggest = 0.0f, smallest = INFINITY;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    smallest = fminf(smallest, scale_range[par][w][0]);
-                    biggest = fmaxf(biggest, scale_range[par][w][1]);   // NaN drops out; the weights show it
+                const float tile_up = value_up[par];
+                if (tile_up != up_now) {   // the same for every row
+                    if (step > 0) ScaleResults<D>(o_tmem, tile_up / up_now);
+                    up_now = tile_up;
                 }
-                int new_k = k;
-                if (biggest > scale_limit) {
-                    const int se = ScaleExponent(biggest);
-                    new_k = 7 - se;
-                    scale_limit = PowerOfTwo(se);
-                }
-                const bool exact_weights = DTYPE == FTH_B200_FP16 && inside && smallest * PowerOfTwo(new_k) >= 1.0f;
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t s[32];
                     TmemLoad32(s_tmem + c * 32, s);
                     float2 z[16];
                     float best = -INFINITY;
-                    const float4* ks = reinterpret_cast<const float4*>(a + kScaleK * kTokens + c * 32);
-                    const float4* km = reinterpret_cast<const float4*>(a + kMinK * kTokens + c * 32);
+                    const float4* ks = reinterpret_cast<const float4*>(a + c * 32);
+                    const float4* km = reinterpret_cast<const float4*>(a + kTokens + c * 32);
                     const float2 qq = make_float2(qsum, qsum), rr = make_float2(-ref, -ref);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -610,33 +660,32 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                         z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), Fma2(make_float2(m4.z, m4.w), qq, rr));
                     }
                     if (!inside) {
+                        // bits of the tokens of this chunk that the row sees
+                        const int from = low - token0 - c * 32, to = high - token0 - c * 32;
+                        uint32_t seen = pr[c];
+                        if (from > 0) seen = from < 32 ? seen & (0xffffffffu << from) : 0u;
+                        if (to < 32) seen = to > 0 ? seen & (0xffffffffu >> (32 - to)) : 0u;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int token = token0 + c * 32 + i;
-                            if (token < low || token >= high || ((pr[c] >> i) & 1u) == 0) {
-                                if (i & 1) z[i >> 1].y = -INFINITY;
-                                else z[i >> 1].x = -INFINITY;
-                            }
+                        for (int i = 0; i < 16; ++i) {
+                            if (((seen >> (2 * i)) & 1u) == 0) z[i].x = -INFINITY;
+                            if (((seen >> (2 * i + 1)) & 1u) == 0) z[i].y = -INFINITY;
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) best = Max3(best, z[i].x, z[i].y);
-                    if (__any_sync(0xffffffffu, best > limit || new_k != k)) {
-                        // move the maximum: scores of this chunk, the weights of the tile's earlier ones, sums and results
+                    if (__any_sync(0xffffffffu, best > limit)) {
+                        // move the maximum: scores of this chunk, the probabilities of the tile's earlier ones, sums and results
                         const bool first = limit == kNotStarted;
-                        const float over = best - static_cast<float>(k);   // above the old maximum
-                        float moved = 0.0f;
+                        const float over = first ? best : best - kProbabilityUp;   // above the old maximum
+                        float shift = 0.0f;
                         if (first ? over > kNotStarted : over > 0.0f) {
-                            moved = over;
-                            if (!first) moved = ceilf(moved);   // a whole number of doublings keeps earlier weights exact
+                            // a whole number of doublings keeps earlier probabilities' bits
+                            shift = first ? over - kProbabilityUp : ceilf(over);
+                            limit = kLazy + kProbabilityUp;
                         }
-                        const float shift = moved + static_cast<float>(k - new_k);
-                        if (!first || moved != 0.0f || over > kNotStarted) limit = first && !(over > kNotStarted) ? kNotStarted : kLazy + static_cast<float>(new_k);
                         const float alpha = first ? 0.0f : Exp2(-shift);
                         ref += shift;
-                        sum = Mul2(sum, make_float2(alpha, alpha));
                         mass = Mul2(mass, make_float2(alpha, alpha));
-                        offset = Mul2(offset, make_float2(alpha, alpha));
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[i] = make_float2(z[i].x - shift, z[i].y - shift);
                         TmemStoreWait();
@@ -651,75 +700,15 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                             }
                             TmemStore16(s_tmem + b * 16, w);
                         }
-                        if (step > 0) {
-                            for (int b = 0; b < D / 16; ++b) {
-                                uint32_t w[16];
-                                umma::TmemLoad16(o_tmem + b * 16, w);
-                                umma::TmemLoadWait();
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
-                                TmemStore16(o_tmem + b * 16, w);
-                            }
-                        }
+                        if (step > 0) ScaleResults<D>(o_tmem, alpha);
                         TmemStoreWait();
-                        k = new_k;
                     }
                     uint32_t packed[16];
-                    const float4* vs = reinterpret_cast<const float4*>(a + kScaleV * kTokens + c * 32);
-                    const float4* vm = reinterpret_cast<const float4*>(a + kMinV * kTokens + c * 32);
-                    if (exact_weights) {
-                        const float4* vi = reinterpret_cast<const float4*>(a + kInverseV * kTokens + c * 32);
-                        const float4* vr = reinterpret_cast<const float4*>(a + kRatioV * kTokens + c * 32);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float4 s4 = vs[i], i4 = vi[i], r4 = vr[i];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float2 prob = make_float2(Exp2(z[2 * i + h].x), Exp2(z[2 * i + h].y));
-                                mass = Add2(mass, prob);
-                                const float2 w = Mul2(prob, h ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y));
-                                packed[2 * i + h] = PackHalf(w.x, w.y);
-                                const float2 kept = HalfPair<FTH_B200_FP16>(packed[2 * i + h]);
-                                sum = Fma2(kept, h ? make_float2(i4.z, i4.w) : make_float2(i4.x, i4.y), sum);
-                                offset = Fma2(kept, h ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y), offset);
-                            }
-                        }
-                    } else if (DTYPE == FTH_B200_BF16 && inside) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float4 s4 = vs[i], m4 = vm[i];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float2 prob = make_float2(Exp2(z[2 * i + h].x), Exp2(z[2 * i + h].y));
-                                mass = Add2(mass, prob);
-                                offset = Fma2(prob, h ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y), offset);
-                                const float2 w = Mul2(prob, h ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y));
-                                packed[2 * i + h] = PackHalf(w.x, w.y);
-                            }
-                        }
-                    } else {
-                        // hidden tokens (whatever stands there: 0 * NaN is no zero), or value scales too small beside the largest
-                        // for a weight to give the probability back
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float w[2];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float score = h ? z[i].y : z[i].x;
-                                const bool hidden = score == -INFINITY;
-                                const float prob = Exp2(score);
-                                const float scale = a[kScaleV * kTokens + c * 32 + 2 * i + h], minimum = a[kMinV * kTokens + c * 32 + 2 * i + h];
-                                w[h] = hidden ? 0.0f : __half2float(__float2half_rn(prob * scale));
-                                float kept = prob;
-                                if (DTYPE == FTH_B200_FP16 && scale * PowerOfTwo(k) >= 1.0f) kept = w[h] * a[kInverseV * kTokens + c * 32 + 2 * i + h];
-                                if (!hidden) {
-                                    mass.x += prob;
-                                    if (DTYPE == FTH_B200_FP16) sum.x += kept;
-                                    offset.x = fmaf(kept, minimum, offset.x);
-                                }
-                            }
-                            packed[i] = PackHalf(w[0], w[1]);
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 prob = make_float2(Exp2(z[i].x), Exp2(z[i].y));
+                        mass = Add2(mass, prob);
+                        packed[i] = PackHalf(prob.x, prob.y);
                     }
                     TmemStore16(s_tmem + c * 16, packed);
                 }
@@ -731,7 +720,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             // ---- the unit's results
             if (active) wait(&o_done[g], (used - 1) & 1u, 7);
             umma::FenceAfterThreadSync();
-            const float all = mass.x + mass.y, total = DTYPE == FTH_B200_FP16 ? sum.x + sum.y : all, shift = offset.x + offset.y;
+            const float total = mass.x + mass.y;
             const int64_t unit_begin = u.at - u.into, unit_end = unit_begin + (u.tile_last - u.tile_first);
             const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : Divide(unit_begin, per);
             const int64_t part_last = unit_end <= share_end ? blockIdx.x : Divide(unit_end - 1, per);
@@ -744,7 +733,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const int64_t q_row = u.req.first_row + static_cast<int64_t>(query);
             uint16_t* const out = static_cast<uint16_t*>(p.out) + q_row * p.ldo + static_cast<int64_t>(q_head) * D;
             const float scale = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-            const float even = 16777216.0f, odd = 1048576.0f;   // 2^24, 2^20: what the codes' places make of them
+            const float down = 1.0f / up_now;   // a power of two
 #pragma unroll 1
             for (int c = 0; active && c < D / 16; ++c) {
                 uint32_t w[16];
@@ -754,7 +743,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 if (!valid || failed) continue;   // a wait that gave up is in the status word; nothing is stored then
                 float v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = fmaf(__uint_as_float(w[i]), (i & 1) ? odd : even, shift);
+                for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]) * down;
                 if (whole) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 8) {
@@ -769,9 +758,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 }
             }
             if (active && whole && valid && !failed && p.lse != nullptr)
-                p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(all)) * 0.6931471805599453f;
+                p.lse[q_row * p.kv_heads * p.group + q_head] = total == 0.0f ? -INFINITY : (best + log2f(total)) * 0.6931471805599453f;
             if (active && !whole) {
-                if (valid) *reinterpret_cast<float4*>(partial + D) = make_float4(best, 0.0f, total, all);
+                if (valid) *reinterpret_cast<float4*>(partial + D) = make_float4(best, 0.0f, total, total);
                 const int parts = static_cast<int>(part_last - part_first) + 1;
                 const auto sync = [&] { WarpsSync(1 + g, 128); };
                 __threadfence();
