@@ -67,7 +67,10 @@ struct Layout {
 };
 
 // Barrier of the warps that compute.
-__device__ __forceinline__ void ComputeSync() { asm volatile("bar.sync 1, %0;" ::"n"(kCompute) : "memory"); }
+__device__ __forceinline__ void ComputeSync() {
+    __syncwarp();
+    asm volatile("barrier.cta.sync 1, %0;" ::"n"(kCompute) : "memory");   // not the aligned form: lanes may come one after another
+}
 
 // Sum of v over the block, and the sum over the threads before this one.
 __device__ __forceinline__ int64_t ScanWork(int64_t v, int64_t* shared, int64_t* total) {
@@ -381,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     uint32_t f[4];
-                    QueryOperands<DTYPE>(raw[n][w], up, f);
+                    QueryOperands<DTYPE>(raw[n][w], up, 0.0625f, f);
                     if constexpr (QS) {
                         if (warp == 0) q_shared[(n * W + w) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
                     } else {

@@ -155,15 +155,15 @@ __device__ __forceinline__ int ScaleExponent(float biggest) {
     const int e = static_cast<int>((__float_as_uint(biggest) >> 23) & 0xffu) - 126;
     return e > 120 ? 120 : e < -100 ? -100 : e;
 }
-// Eight query elements in the order a word of eight codes gives its operands: (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
+// Eight query elements in the order a word of eight codes gives its operands: (0, 4), (1, 5) * odd, (2, 6), (3, 7) * odd.
 template <int DTYPE>
-__device__ __forceinline__ void QueryOperands(const uint32_t (&raw)[4], float up, uint32_t (&f)[4]) {
+__device__ __forceinline__ void QueryOperands(const uint32_t (&raw)[4], float up, float odd, uint32_t (&f)[4]) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 v = HalfPair<DTYPE>(raw[i]);
         x[2 * i] = v.x * up;
-        x[2 * i + 1] = v.y * (up * 0.0625f);
+        x[2 * i + 1] = v.y * (up * odd);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = PackHalf(x[i], x[i + 4]);

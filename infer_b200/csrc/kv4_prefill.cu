@@ -1,18 +1,23 @@
 // Attention over the 4-bit cache, many query rows per kv head (prompts, chunks of them, long drafts).
 //
 // A tile of 128 query rows (queries x heads of the group, so a group shares every key) against tiles of 128 tokens,
-//     S = Q C_k^T   tcgen05.mma kind::f16, both operands in shared memory, accumulator in tensor memory
-//     P = exp2(s_k S + m_k sum(q) - maximum), rounded to FP16, written over S in tensor memory
+//     S = Q K^T     tcgen05.mma kind::f16, both operands in shared memory, accumulator in tensor memory
+//     P = exp2(S - maximum), rounded to FP16, written over S in tensor memory
 //     O = O + P V   the probabilities read from tensor memory
-// Keys enter as their codes: c * 2^-24 in the low four bits of a half-precision number and 16 c * 2^-24 four bits higher,
-// both exact (kv4_attention.cu), eight codes in five operations and one 16-byte store; q has its elements in the order
-// this gives.  Values enter as numbers, minimum + scale * code rounded once to FP16 (11 bits) after a power of two that
-// brings the largest of the tokens so far to 2^14: a scale and a minimum per token would have to be handed to every row of
+// Values enter as numbers, minimum + scale * code rounded once to FP16 (11 bits) after a power of two that brings the
+// largest of the tokens so far to 2^14: a scale and a minimum per token would have to be handed to every row of
 // probabilities, and what a warp reads from shared memory for all its lanes costs as much as 32 different words.  The
 // rounding moves a result by at most 2^-12 of the values it averages, as the rounding of the probabilities does.
-// Four warps unpack, holding the next tile's words in registers while the matrix unit still reads the present one.  Four
-// more per tile of rows own a row per thread: scores out of tensor memory 32 at a time, two FMAs on pairs, one exp2, the
-// sum.  One thread issues the matrix instructions.  All operands are K-major with the 128-byte swizzle.
+// Keys enter the same way with BF16 queries, whose own elements are eight times coarser than the rounding.  With FP16 queries
+// they enter as their codes, c * 2^-24 in the low four bits of a half-precision number and 16 c * 2^-24 four bits higher, both
+// exact (kv4_attention.cu); q has its elements in the order this gives, and scale and minimum are applied to the scores, two
+// reads of shared memory for four of them.
+// Four warps unpack, holding the next tile's words in registers while the matrix unit still reads the present one; one warp
+// prepares the tokens' parameters.  Four more per tile of rows own a row per thread: scores out of tensor memory 32 at a
+// time, an FMA or two on pairs, one exp2, the sum.  One thread issues the matrix instructions.  All operands are K-major
+// with the 128-byte swizzle.  The loops are rolled where that costs a few moves: with five kinds of warps at work their code
+// together has to stay in the SM's instruction cache (fully unrolled, with keys and values in separate warps, a quarter of
+// the fetches missed it and 3 prompts of 4000 rows took 1.97 ms).
 //
 // A block of threads has two tiles of query rows (one for 256-wide heads, whose results fill tensor memory) that share the
 // unpacked tokens: while one's scores become probabilities the matrix unit works for the other.  Unpacked tiles are
@@ -43,8 +48,8 @@ struct Tiles {
     static constexpr int kQueryTiles = D == 256 ? 1 : 2;
     static constexpr int kUnitRows = kQueryTiles * kRows;
     static constexpr int kStages = D == 256 ? 1 : 2;               // unpacked tiles of tokens
-    static constexpr int kSoftmax = kQueryTiles * 128;             // threads: softmax, unpacking, the warp that issues
-    static constexpr int kThreads = kSoftmax + 128 + 32;
+    static constexpr int kSoftmax = kQueryTiles * 128;             // threads: softmax, then unpacking, then a warp that issues
+    static constexpr int kThreads = kSoftmax + 128 + 64;           // products and one for parameters
     static constexpr int kBlocks64 = D / 64;                       // 128-byte wide pieces of a row
     static constexpr int kPieceBytes = 128 * 128;
     static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V of one tile
@@ -91,7 +96,12 @@ __device__ __forceinline__ uint32_t ValuePair(uint32_t x, uint32_t scale, uint32
     const __half2 v = __hfma2(c, *reinterpret_cast<const __half2*>(&scale), *reinterpret_cast<const __half2*>(&minimum));
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ void WarpsSync(int barrier, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory"); }
+// A barrier of some warps.  Not the aligned form: one thread of a warp may come to it later than the others (it has been
+// at work for its group), and the compiler may place the instruction on both paths.
+__device__ __forceinline__ void WarpsSync(int barrier, int threads) {
+    __syncwarp();
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
 __device__ __forceinline__ float Max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -101,6 +111,7 @@ __device__ __forceinline__ float Max3(float a, float b, float c) {
 // The rows' results so far times `factor`, by the warp that owns them.
 template <int D>
 __device__ __forceinline__ void ScaleResults(uint32_t o_tmem, float factor) {
+    __syncwarp();
 #pragma unroll 1
     for (int b = 0; b < D / 16; ++b) {
         uint32_t w[16];
@@ -134,24 +145,37 @@ __device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, const 
     return WarpSum(sum);
 }
 
-// What a block of threads works on: a place in the list of units.
+// What a block of threads works on: a place in the list of units.  Every group of warps keeps its own in shared memory (the
+// groups run ahead of each other), so that it costs no registers in the loops over tokens.
 struct Place {
     int b, head, row;
     int tile_first, tile_last;  // of the unit
+    int t0, steps;              // this block's tiles of it
+    int low, high;              // tokens that some row of the unit sees
+    int more;                   // a unit, not the end of the share
     int64_t into;               // tiles of the unit that other blocks take
     int64_t at;                 // in the flat list
-    int t0, steps;              // this block's tiles of it
     Request req;
 };
-__device__ __forceinline__ void Settle(int64_t share_end, Place& u) {
+template <int UNIT>
+__device__ __forceinline__ void Settle(const AttentionParams& p, int64_t share_end, Place& u) {
     const int64_t left = share_end - u.at, tiles = u.tile_last - u.tile_first - u.into;
     u.t0 = u.tile_first + static_cast<int>(u.into);
     u.steps = static_cast<int>(tiles < left ? tiles : left);
+    int unused;
+    Visible(p, u.req, u.row / p.group, &u.low, &unused);
+    Visible(p, u.req, ((u.row + UNIT < u.req.rows ? u.row + UNIT : u.req.rows) - 1) / p.group, &unused, &u.high);
+    u.more = 1;
 }
+// By one thread of the group.
 template <int UNIT>
-__device__ __forceinline__ bool Advance(const AttentionParams& p, int64_t share_end, Place& u) {
+__device__ __forceinline__ void Advance(const AttentionParams& p, int64_t share_end, Place* place) {
+    Place u = *place;
     u.at += u.steps;
-    if (u.at >= share_end) return false;
+    if (u.at >= share_end) {
+        place->more = 0;
+        return;
+    }
     u.into = 0;
     u.row += UNIT;
     if (u.row >= u.req.rows) {
@@ -165,29 +189,60 @@ __device__ __forceinline__ bool Advance(const AttentionParams& p, int64_t share_
         }
     }
     UnitTiles<kTokens>(p, u.req, u.row, UNIT, &u.tile_first, &u.tile_last);
-    Settle(share_end, u);
+    Settle<UNIT>(p, share_end, u);
+    *place = u;
+}
+
+// Bounded like MbarWait, in little code.  The lanes of a warp may leave it one after another: a __syncwarp comes before the
+// next tensor-memory instruction, which the whole warp executes together.
+__device__ __forceinline__ bool WaitFor(uint64_t* bar, uint32_t parity, int* status, int detail) {
+    uint64_t since = 0;
+#pragma unroll 1
+    for (int i = 1; !MbarTryWait(bar, parity); ++i) {
+        if ((i & 255) != 0) continue;
+        const uint64_t now = GlobalTimerNs();
+        if (since == 0) since = now;
+        else if (now - since > kWaitBudgetNs) {
+            ReportTimeout(status, kSite, detail);
+            return false;
+        }
+    }
     return true;
+}
+// Whether some row sees one of the sixteen tokens around `token`.
+__device__ __forceinline__ bool SomeSeen(const Place& u, int token) { return (token & ~15) < u.high && (token & ~15) + 16 > u.low; }
+// What the table names as the block of `token` if any of its sixteen neighbours is seen by a row, else -1.
+__device__ __forceinline__ int BlockOf(const AttentionParams& p, const Place& u, int token) {
+    return SomeSeen(u, token) ? p.table[static_cast<int64_t>(u.b) * p.max_blocks + (token >> p.cache.block_shift)] : -1;
+}
+__device__ __forceinline__ bool IsBlock(const AttentionParams& p, int id) { return id >= 0 && id < p.cache.blocks; }
+__device__ __forceinline__ int64_t TokenIndex(const AttentionParams& p, int block, int head, int token) {
+    return HeadBase(p.cache, block, head) + (token & ((1 << p.cache.block_shift) - 1));
 }
 
 template <int D, int DTYPE>
 __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __grid_constant__ AttentionParams p) {
     using T = Tiles<D>;
     constexpr int kThreads = T::kThreads, G = T::kQueryTiles, S = T::kStages, kUnit = T::kUnitRows;
+    constexpr bool kKeyCodes = DTYPE == FTH_B200_FP16;   // keys as codes, else as numbers
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(8) uint64_t q_full[G], s_full[G], p_full[G], o_done[G], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[2], back_full;
+    __shared__ __align__(8) uint64_t q_full[G], s_full[G], p_full[G], o_done[G], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[2], tile_done[2], back_full;
     __shared__ int64_t unit_work[kThreads];
     __shared__ int64_t work_total;
-    __shared__ Place start;
-    __shared__ uint32_t present[2][4];     // a bit per token of a tile that some row may see
-    __shared__ float value_up[2];          // power of two on the values of a tile
-    __shared__ float value_big[4];         // largest value of a tile, by unpacking warp
-    __shared__ __align__(16) __half value_scale[kTokens], value_min[kTokens];
+    constexpr int kUnpackPlace = G, kIssuePlace = G + 1, kParamPlace = G + 2, kPlaces = G + 3;
+    __shared__ Place places[kPlaces];      // one per tile of rows (softmax), unpacking, products, parameters
+    // of a tile, by its parity
+    __shared__ uint32_t present[2][4];     // a bit per token that some row may see
+    __shared__ uint32_t spoiled[2][4];     // a bit per token whose parameters are no numbers
+    __shared__ float value_up[2];          // power of two on the values
+    __shared__ float key_back[2];          // what takes scores to exponents of two (keys as numbers)
+    __shared__ __align__(16) __half value_scale[2][kTokens], value_min[2][kTokens], key_scale[2][kTokens], key_min[2][kTokens];
     __shared__ float q_big[4 * G], unit_back;
     __shared__ int join_last[G];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kUnpackWarp = T::kSoftmax / 32, kIssueWarp = kUnpackWarp + 4;
+    constexpr int kUnpackWarp = T::kSoftmax / 32, kIssueWarp = kUnpackWarp + 4, kParamWarp = kIssueWarp + 1;
     if (threadIdx.x == 0) {
         for (int g = 0; g < G; ++g) {
             MbarInit(&q_full[g], 128);
@@ -201,8 +256,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             MbarInit(&v_full[s], 128);
             MbarInit(&v_empty[s], 1);
         }
-        MbarInit(&params_full[0], 128);
-        MbarInit(&params_full[1], 128);
+        for (int i = 0; i < 2; ++i) {
+            MbarInit(&params_full[i], 32);
+            MbarInit(&tile_done[i], 1);
+        }
         MbarInit(&back_full, 1);
         FenceBarrierInit();
     }
@@ -305,8 +362,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                                     u.tile_last = c;
                                     u.into = off - (upto - (c - a));
                                     u.at = share_begin;
-                                    Settle(share_end, u);
-                                    start = u;
+                                    Settle<kUnit>(p, share_end, u);
+                                    for (int i = 0; i < kPlaces; ++i) places[i] = u;
                                 }
                                 break;
                             }
@@ -324,241 +381,17 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
     float* const params = reinterpret_cast<float*>(smem + T::kParams);
     bool failed = false;
     const auto wait = [&](uint64_t* bar, uint32_t parity, int detail) {
-        if (!failed && !MbarWait(bar, parity, p.status, kSite, 16 + detail)) failed = true;
+        if (!failed && !WaitFor(bar, parity, p.status, 16 + detail)) failed = true;
     };
 
-    if (busy && warp >= kUnpackWarp && warp < kIssueWarp) {
-        // ================================================ unpacking ==================================================
-        const int tid = threadIdx.x - T::kSoftmax;
-        Place u = start;
-        uint32_t tile_count = 0, unit_count = 0;
-        // K: this thread's 16-byte pieces, 32 elements of a token each.  V: eight tokens (four pairs) by kTaskWords words of four
-        // elements; neighbouring lanes take neighbouring eights of tokens, so that the eight lanes of a store phase hit eight
-        // different 16-byte columns.
-        constexpr int kTaskWords = D == 64 ? 2 : 4, kTasks = D / (32 * kTaskWords);
-        const int octet = tid & 15;
-        constexpr int kPieces = D / 32;
-        uint4 kw[kPieces];
-        uint32_t vw[kTasks][4][kTaskWords];
-        uint32_t kp, vp;
-        bool there;
-        do {
-            int first_low, last_high, unused;
-            Visible(p, u.req, u.row / p.group, &first_low, &unused);
-            Visible(p, u.req, ((u.row + kUnit < u.req.rows ? u.row + kUnit : u.req.rows) - 1) / p.group, &unused, &last_high);
-            const int32_t* table = p.table + static_cast<int64_t>(u.b) * p.max_blocks;
-            // K: neighbouring lanes take the halves of 64 bytes of four tokens, then further 64-byte pieces, so that the eight
-            // lanes of a store phase hit eight different 16-byte columns
-            const auto k_token = [&](int j) { return ((tid + 128 * j) >> 1 & 3) | ((tid + 128 * j) / (4 * kPieces) << 2); };
-            const auto k_piece = [&](int j) { return ((tid + 128 * j) & 1) | (((tid + 128 * j) >> 3) % (kPieces / 2) << 1); };
-            // block numbers of the tokens of this thread's K pieces, of its V tokens and of its own token, fetched a tile before
-            // they are needed; -1: no row sees the tokens
-            int ids[kPieces], id_v, own_id;
-            const auto lookup = [&](int step) {
-                const auto at = [&](int in_tile) {
-                    const int token = (u.t0 + step) * kTokens + (in_tile & ~15);
-                    return step < u.steps && token < last_high && token + 16 > first_low ? table[token >> p.cache.block_shift] : -1;
-                };
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) ids[j] = at(k_token(j));
-                id_v = at(octet * 8);
-                own_id = at(tid);
-            };
-            // a number that is no block hides its tokens
-            const auto exists = [&](int id) { return id >= 0 && id < p.cache.blocks; };
-            const auto index = [&](int id, int step, int in_tile) {
-                return HeadBase(p.cache, id, u.head) + (((u.t0 + step) * kTokens + in_tile) & ((1 << p.cache.block_shift) - 1));
-            };
-            const auto load_k = [&](int step) {
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
-                    kw[j] = make_uint4(0, 0, 0, 0);
-                    if (exists(ids[j])) kw[j] = LoadStream16(p.cache.k_codes + index(ids[j], step, k_token(j)) * (D / 2) + k_piece(j) * 16);
-                }
-                const int token = (u.t0 + step) * kTokens + tid;
-                there = exists(own_id) && token >= first_low && token < last_high;
-                if (!exists(own_id) && token >= first_low && token < last_high) ReportTimeout(p.status, kSiteAttention, u.b);
-                kp = vp = 0;
-                if (there) {
-                    const int64_t at = index(own_id, step, tid);
-                    kp = p.cache.k_params[at];
-                    vp = p.cache.v_params[at];
-                }
-            };
-            const auto load_v = [&](int step) {
-                const bool there_v = exists(id_v);
-                const uint8_t* from = p.cache.v_codes + (there_v ? index(id_v, step, octet * 8) * (D / 2) : 0);
-#pragma unroll
-                for (int t = 0; t < kTasks; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint8_t* row = from + j * D + ((tid >> 4) + 8 * t) * (kTaskWords * 4);
-                        if constexpr (kTaskWords == 4) {
-                            const uint4 x = there_v ? LoadStream16(row) : make_uint4(0, 0, 0, 0);
-                            vw[t][j][0] = x.x;
-                            vw[t][j][1] = x.y;
-                            vw[t][j][2] = x.z;
-                            vw[t][j][3] = x.w;
-                        } else {
-                            const uint2 x = there_v ? *reinterpret_cast<const uint2*>(row) : make_uint2(0, 0);
-                            vw[t][j][0] = x.x;
-                            vw[t][j][1] = x.y;
-                        }
-                    }
-            };
-            int up_exponent = kNoExponent;   // of the values, largest so far in the unit
-            lookup(0);
-            load_k(0);
-            load_v(0);
-            lookup(1);
-            for (int step = 0; step < u.steps; ++step, ++tile_count) {
-                const uint32_t stage = tile_count % S, turn = (tile_count / S) & 1u, par = tile_count & 1u;
-                uint8_t* const k_smem = smem + T::kKeys + stage * T::kOperandBytes;
-                uint8_t* const v_smem = smem + T::kKeys + (S + stage) * T::kOperandBytes;
-                if (tile_count >= S) wait(&k_empty[stage], turn ^ 1u, 0);
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
-                    const int token = k_token(j), piece = k_piece(j);
-                    uint8_t* row = k_smem + (piece >> 1) * T::kPieceBytes + token * 128;
-                    const uint32_t w[4] = {kw[j].x, kw[j].y, kw[j].z, kw[j].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t x = w[i], y = x >> 8;
-                        *reinterpret_cast<uint4*>(row + ((((piece & 1) * 4 + i) ^ (token & 7)) << 4)) =
-                            make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
-                    }
-                }
-                FenceProxyAsync();
-                MbarArrive(&k_full[stage]);
-                // parameters, and the token's bit; the tile two before is done with their place when its V is
-                if (tile_count >= S) wait(&v_empty[stage], turn ^ 1u, 1);
-                if (step == 0) wait(&back_full, unit_count & 1u, 9);
-                {
-                    const float vs = ParamScale(vp), vm = ParamMin(vp);
-                    // a token with a scale that is no number spoils the rows that see it through its score; as a value it must not
-                    // reach the others (0 * NaN is no zero)
-                    const bool spoiled = there && (!(ParamScale(kp) < INFINITY) || !(vs < INFINITY) || !(fabsf(vm) < INFINITY));
-                    float* a = params + par * (T::kParamBytes / 4) + tid;
-                    a[0] = spoiled ? __uint_as_float(0x7fc00000u) : ParamScale(kp) * unit_back;
-                    a[kTokens] = ParamMin(kp);
-                    const uint32_t bits = __ballot_sync(0xffffffffu, there);
-                    const float own_big = there && !spoiled ? fmaxf(fabsf(vm), fabsf(fmaf(15.0f, vs, vm))) : 0.0f;
-                    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(own_big));
-                    if (lane == 0) {
-                        present[par][warp - kUnpackWarp] = bits;
-                        value_big[warp - kUnpackWarp] = __uint_as_float(top);
-                    }
-                    WarpsSync(4, 128);
-                    const float big = fmaxf(fmaxf(value_big[0], value_big[1]), fmaxf(value_big[2], value_big[3]));
-                    if (big > 0.0f) {
-                        const int e = QueryExponent(big);
-                        if (up_exponent == kNoExponent || e < up_exponent) up_exponent = e;
-                    }
-                    const float up = PowerOfTwo(up_exponent == kNoExponent ? 0 : up_exponent);
-                    value_scale[tid] = __float2half_rn(there && !spoiled ? vs * up : 0.0f);
-                    value_min[tid] = __float2half_rn(there && !spoiled ? vm * up : 0.0f);
-                    if (tid == 0) value_up[par] = up;
-                    WarpsSync(4, 128);
-                }
-                MbarArrive(&params_full[par]);
-                if (step + 1 < u.steps) load_k(step + 1);
-                {
-                    const uint4 s4 = *reinterpret_cast<const uint4*>(&value_scale[octet * 8]), m4 = *reinterpret_cast<const uint4*>(&value_min[octet * 8]);
-                    const uint32_t sp[4] = {s4.x, s4.y, s4.z, s4.w}, mp[4] = {m4.x, m4.y, m4.z, m4.w};
-                    uint8_t* const block = v_smem + (octet >> 3) * (D * 128);
-#pragma unroll
-                    for (int t = 0; t < kTasks; ++t) {
-#pragma unroll
-                        for (int w = 0; w < kTaskWords; ++w) {
-                            uint32_t v[4][4];   // element, pair
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t x = vw[t][j][w], y = x >> 8;
-                                v[0][j] = ValuePair<0>(x, sp[j], mp[j]);
-                                v[1][j] = ValuePair<1>(x, sp[j], mp[j]);
-                                v[2][j] = ValuePair<0>(y, sp[j], mp[j]);
-                                v[3][j] = ValuePair<1>(y, sp[j], mp[j]);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int element = (((tid >> 4) + 8 * t) * kTaskWords + w) * 4 + i;
-                                *reinterpret_cast<uint4*>(block + element * 128 + (((octet & 7) ^ (element & 7)) << 4)) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
-                            }
-                        }
-                    }
-                }
-                FenceProxyAsync();
-                MbarArrive(&v_full[stage]);
-                if (step + 1 < u.steps) {
-                    load_v(step + 1);
-                    lookup(step + 2);
-                }
-            }
-            ++unit_count;
-        } while (Advance<kUnit>(p, share_end, u));
-    } else if (busy && warp == kIssueWarp) {
-        // ================================================ products ===================================================
-        if (lane == 0) {
-            Place u = start;
-            const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
-            const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
-            uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
-            const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
-                // S is written where the last tile's P was read
-                if (used[g] > 0) wait(&o_done[g], (used[g] - 1) & 1u, 8);
-                umma::FenceAfterThreadSync();
-                if (failed) return;
-                const uint32_t q = q_addr + g * T::kOperandBytes, k = k_addr + (tile % S) * T::kOperandBytes;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t at = (i >> 2) * T::kPieceBytes + (i & 3) * 32;
-                    MmaShared(tmem + g * 256, umma::SmemDesc(q + at, 0, 1024), umma::SmemDesc(k + at, 0, 1024), s_desc, i > 0);
-                }
-                umma::Commit(&s_full[g]);
-            };
-            const auto values = [&](int g, uint32_t tile, bool first) {
-                wait(&p_full[g], used[g] & 1u, 4);
-                umma::FenceAfterThreadSync();
-                if (failed) return;
-                const uint32_t v = v_addr + (tile % S) * T::kOperandBytes;
-#pragma unroll
-                for (int i = 0; i < kTokens / 16; ++i)
-                    MmaTensor(tmem + g * 256 + 128, tmem + g * 256 + i * 8, umma::SmemDesc(v + (i >> 2) * (D * 128) + (i & 3) * 32, 0, 1024), o_desc, !first || i > 0);
-                umma::Commit(&o_done[g]);
-                ++used[g];
-            };
-            do {
-                const int active = u.req.rows - u.row > kRows ? G : 1;   // tiles of rows that have any
-                wait(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
-                for (int g = 0; g < active; ++g) {
-                    wait(&q_full[g], unit_count & 1u, 2);
-                    scores(g, tile_count);
-                }
-                umma::Commit(&k_empty[tile_count % S]);
-                for (int step = 0; step < u.steps && !failed; ++step, ++tile_count) {
-                    const bool more = step + 1 < u.steps;
-                    const uint32_t next = tile_count + 1;
-                    wait(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
-                    for (int g = 0; g < active; ++g) {
-                        values(g, tile_count, step == 0);
-                        if (g + 1 == active) umma::Commit(&v_empty[tile_count % S]);
-                        if (more) {
-                            if (g == 0) wait(&k_full[next % S], (next / S) & 1u, 3);
-                            scores(g, next);
-                            if (g + 1 == active) umma::Commit(&k_empty[next % S]);
-                        }
-                    }
-                }
-                ++unit_count;
-            } while (!failed && Advance<kUnit>(p, share_end, u));
-        }
-    } else if (busy && warp < kUnpackWarp) {
+    if (warp < kUnpackWarp) {
+        if (busy) {
         // ================================================ softmax ====================================================
         const int g = warp >> 2;                   // tile of rows
         const int r = threadIdx.x & 127;           // row of the tile, lane of tensor memory
         const uint32_t s_tmem = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * 256, o_tmem = s_tmem + 128;
         uint8_t* const q_smem = smem + g * T::kOperandBytes;
-        Place u = start;
+        const Place& u = places[g];
         uint32_t tile_count = 0, unit_count = 0, used = 0;
         for (;;) {
             // ---- the unit's queries, as operands
@@ -603,14 +436,14 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const int e = QueryExponent(big);
             const float up = PowerOfTwo(e);
             if (threadIdx.x == 0) {
-                unit_back = p.scale_log2 * PowerOfTwo(24 - e);
+                unit_back = p.scale_log2 * PowerOfTwo((kKeyCodes ? 24 : 0) - e);
                 MbarArrive(&back_full);
             }
             qsum *= p.scale_log2;
             const auto place = [&](int w, uint4 x) {
                 const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
                 uint32_t f[4];
-                QueryOperands<DTYPE>(raw, up, f);
+                QueryOperands<DTYPE>(raw, up, kKeyCodes ? 0.0625f : 1.0f, f);
                 *reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + r * 128 + (((w & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
             };
             if constexpr (D <= 128) {
@@ -628,16 +461,17 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             // ---- tiles.  Scores are kept relative to ref = maximum - 7.
             float ref = 0.0f, limit = kNotStarted, up_now = 1.0f;
             float2 mass = make_float2(0.0f, 0.0f);
-            if (!active) tile_count += u.steps;   // no rows
-            for (int step = 0; active && step < u.steps; ++step, ++tile_count, ++used) {
+            const int steps = u.steps, first_token = u.t0 * kTokens;
+            if (!active) tile_count += steps;   // no rows
+            for (int step = 0; active && step < steps; ++step, ++tile_count, ++used) {
                 const uint32_t par = tile_count & 1u;
                 wait(&params_full[par], (tile_count >> 1) & 1u, 10);
                 wait(&s_full[g], used & 1u, 6);
+                __syncwarp();
                 umma::FenceAfterThreadSync();
-                const float* a = params + par * (T::kParamBytes / 4);
-                const int token0 = (u.t0 + step) * kTokens;
-                const uint32_t pr[4] = {present[par][0], present[par][1], present[par][2], present[par][3]};
-                const bool all_there = (pr[0] & pr[1] & pr[2] & pr[3]) == 0xffffffffu;
+                const int token0 = first_token + step * kTokens;
+                const float back = key_back[par];
+                const bool all_there = (present[par][0] & present[par][1] & present[par][2] & present[par][3]) == 0xffffffffu && (spoiled[par][0] | spoiled[par][1] | spoiled[par][2] | spoiled[par][3]) == 0;
                 const bool inside = all_there && __all_sync(0xffffffffu, !valid || (token0 >= low && token0 + kTokens <= high));
                 const float tile_up = value_up[par];
                 if (tile_up != up_now) {   // the same for every row
@@ -647,22 +481,30 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t s[32];
+                    __syncwarp();
                     TmemLoad32(s_tmem + c * 32, s);
                     float2 z[16];
                     float best = -INFINITY;
-                    const float4* ks = reinterpret_cast<const float4*>(a + c * 32);
-                    const float4* km = reinterpret_cast<const float4*>(a + kTokens + c * 32);
-                    const float2 qq = make_float2(qsum, qsum), rr = make_float2(-ref, -ref);
+                    const float2 rr = make_float2(-ref, -ref);
+                    if constexpr (kKeyCodes) {
+                        const float4* ks = reinterpret_cast<const float4*>(params + par * (T::kParamBytes / 4) + c * 32);
+                        const float4* km = ks + kTokens / 4;
+                        const float2 qq = make_float2(qsum, qsum);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float4 s4 = ks[i], m4 = km[i];
-                        z[2 * i] = Fma2(make_float2(s4.x, s4.y), make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), Fma2(make_float2(m4.x, m4.y), qq, rr));
-                        z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), Fma2(make_float2(m4.z, m4.w), qq, rr));
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 s4 = ks[i], m4 = km[i];
+                            z[2 * i] = Fma2(make_float2(s4.x, s4.y), make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), Fma2(make_float2(m4.x, m4.y), qq, rr));
+                            z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), Fma2(make_float2(m4.z, m4.w), qq, rr));
+                        }
+                    } else {
+                        const float2 bb = make_float2(back, back);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[i] = Fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), bb, rr);
                     }
-                    if (!inside) {
+                    if (__builtin_expect(!inside, 0)) {
                         // bits of the tokens of this chunk that the row sees
                         const int from = low - token0 - c * 32, to = high - token0 - c * 32;
-                        uint32_t seen = pr[c];
+                        uint32_t seen = present[par][c];
                         if (from > 0) seen = from < 32 ? seen & (0xffffffffu << from) : 0u;
                         if (to < 32) seen = to > 0 ? seen & (0xffffffffu >> (32 - to)) : 0u;
 #pragma unroll
@@ -670,10 +512,12 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                             if (((seen >> (2 * i)) & 1u) == 0) z[i].x = -INFINITY;
                             if (((seen >> (2 * i + 1)) & 1u) == 0) z[i].y = -INFINITY;
                         }
+                        const uint32_t bad = spoiled[par][c] & seen;
+                        if (bad != 0) z[0].x = NAN;   // the row is NaN, whichever token makes it
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) best = Max3(best, z[i].x, z[i].y);
-                    if (__any_sync(0xffffffffu, best > limit)) {
+                    if (__builtin_expect(__any_sync(0xffffffffu, best > limit), 0)) {
                         // move the maximum: scores of this chunk, the probabilities of the tile's earlier ones, sums and results
                         const bool first = limit == kNotStarted;
                         const float over = first ? best : best - kProbabilityUp;   // above the old maximum
@@ -710,6 +554,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                         mass = Add2(mass, prob);
                         packed[i] = PackHalf(prob.x, prob.y);
                     }
+                    __syncwarp();
                     TmemStore16(s_tmem + c * 16, packed);
                 }
                 TmemStoreWait();
@@ -719,6 +564,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
 
             // ---- the unit's results
             if (active) wait(&o_done[g], (used - 1) & 1u, 7);
+            __syncwarp();
             umma::FenceAfterThreadSync();
             const float total = mass.x + mass.y;
             const int64_t unit_begin = u.at - u.into, unit_end = unit_begin + (u.tile_last - u.tile_first);
@@ -781,7 +627,285 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             }
             ++unit_count;
             umma::FenceBeforeThreadSync();
-            if (!Advance<kUnit>(p, share_end, u)) break;
+            WarpsSync(1 + g, 128);
+            if (r == 0) Advance<kUnit>(p, share_end, &places[g]);
+            WarpsSync(1 + g, 128);
+            if (!u.more) break;
+        }
+        }
+    } else if (warp < kIssueWarp) {
+        if (busy) {
+        // ================================================ unpacking ==================================================
+        // K: this thread's 16-byte pieces, 32 elements of a token each: neighbouring lanes take the halves of 64 bytes of four
+        // tokens, then further 64-byte pieces.  V: eight tokens (four pairs) by kWords words of four elements: neighbouring
+        // lanes take neighbouring eights of tokens.  Either way the eight lanes of a store phase hit eight different 16-byte
+        // columns.
+        const int tid = threadIdx.x & 127, octet = tid & 15;
+        constexpr int kPieces = D / 32, kWords = D == 64 ? 2 : 4, kTasks = D / (32 * kWords);
+        const auto token_of = [&](int j) { return ((tid + 128 * j) >> 1 & 3) | ((tid + 128 * j) / (4 * kPieces) << 2); };
+        const auto piece_of = [&](int j) { return ((tid + 128 * j) & 1) | (((tid + 128 * j) >> 3) % (kPieces / 2) << 1); };
+        const Place& u = places[kUnpackPlace];
+        uint32_t tile_count = 0;
+        uint4 keys[kPieces];
+        uint32_t values[kTasks][4][kWords];
+        do {
+            const int steps = u.steps, first_token = u.t0 * kTokens;
+            int ids[kPieces], id;   // block numbers, fetched a tile before they are needed
+            const auto lookup = [&](int step) {
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) ids[j] = step < steps ? BlockOf(p, u, first_token + step * kTokens + token_of(j)) : -1;
+                id = step < steps ? BlockOf(p, u, first_token + step * kTokens + octet * 8) : -1;
+            };
+            const auto load_keys = [&](int step) {
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    keys[j] = make_uint4(0, 0, 0, 0);
+                    if (IsBlock(p, ids[j])) keys[j] = LoadStream16(p.cache.k_codes + TokenIndex(p, ids[j], u.head, first_token + step * kTokens + token_of(j)) * (D / 2) + piece_of(j) * 16);
+                }
+            };
+            const auto load_values = [&](int step) {
+                const bool there = IsBlock(p, id);
+                const uint8_t* from = p.cache.v_codes + (there ? TokenIndex(p, id, u.head, first_token + step * kTokens + octet * 8) * (D / 2) : 0);
+#pragma unroll
+                for (int t = 0; t < kTasks; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint8_t* row = from + j * D + ((tid >> 4) + 8 * t) * (kWords * 4);
+                        if constexpr (kWords == 4) {
+                            const uint4 x = there ? LoadStream16(row) : make_uint4(0, 0, 0, 0);
+                            values[t][j][0] = x.x;
+                            values[t][j][1] = x.y;
+                            values[t][j][2] = x.z;
+                            values[t][j][3] = x.w;
+                        } else {
+                            const uint2 x = there ? *reinterpret_cast<const uint2*>(row) : make_uint2(0, 0);
+                            values[t][j][0] = x.x;
+                            values[t][j][1] = x.y;
+                        }
+                    }
+            };
+            lookup(0);
+            load_keys(0);
+            load_values(0);
+            lookup(1);
+            for (int step = 0; step < steps; ++step, ++tile_count) {
+                const uint32_t stage = tile_count % S, turn = (tile_count / S) & 1u, par = tile_count & 1u;
+                uint8_t* const k_smem = smem + T::kKeys + stage * T::kOperandBytes;
+                uint8_t* const v_smem = smem + T::kKeys + (S + stage) * T::kOperandBytes + (octet >> 3) * (D * 128);
+                if (tile_count >= S) wait(&k_empty[stage], turn ^ 1u, 0);
+                wait(&params_full[par], (tile_count >> 1) & 1u, 10);
+#pragma unroll 1
+                for (int j = 0; j < kPieces; ++j) {
+                    const int token = token_of(j), piece = piece_of(j);
+                    uint8_t* row = k_smem + (piece >> 1) * T::kPieceBytes + token * 128;
+                    const uint32_t w[4] = {keys[0].x, keys[0].y, keys[0].z, keys[0].w};
+                    uint32_t scale = 0, minimum = 0;
+                    if constexpr (!kKeyCodes) {
+                        scale = *reinterpret_cast<const uint16_t*>(&key_scale[par][token]) * 0x10001u;
+                        minimum = *reinterpret_cast<const uint16_t*>(&key_min[par][token]) * 0x10001u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t x = w[i], y = x >> 8;
+                        uint4 o;
+                        if constexpr (kKeyCodes) o = make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
+                        else o = make_uint4(ValuePair<0>(x, scale, minimum), ValuePair<1>(x, scale, minimum), ValuePair<0>(y, scale, minimum), ValuePair<1>(y, scale, minimum));
+                        *reinterpret_cast<uint4*>(row + ((((piece & 1) * 4 + i) ^ (token & 7)) << 4)) = o;
+                    }
+#pragma unroll
+                    for (int i = 0; i + 1 < kPieces; ++i) keys[i] = keys[i + 1];   // the next one to the front
+                }
+                FenceProxyAsync();
+                MbarArrive(&k_full[stage]);
+                if (step + 1 < steps) load_keys(step + 1);
+                if (tile_count >= S) wait(&v_empty[stage], turn ^ 1u, 1);
+                const uint4 s4 = *reinterpret_cast<const uint4*>(&value_scale[par][octet * 8]), m4 = *reinterpret_cast<const uint4*>(&value_min[par][octet * 8]);
+                const uint32_t sp[4] = {s4.x, s4.y, s4.z, s4.w}, mp[4] = {m4.x, m4.y, m4.z, m4.w};
+#pragma unroll 1
+                for (int w = 0; w < kTasks * kWords; ++w) {
+                    uint32_t v[4][4];   // element, pair
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x = values[0][j][0], y = x >> 8;
+                        v[0][j] = ValuePair<0>(x, sp[j], mp[j]);
+                        v[1][j] = ValuePair<1>(x, sp[j], mp[j]);
+                        v[2][j] = ValuePair<0>(y, sp[j], mp[j]);
+                        v[3][j] = ValuePair<1>(y, sp[j], mp[j]);
+#pragma unroll
+                        for (int i = 0; i + 1 < kTasks * kWords; ++i) values[i / kWords][j][i % kWords] = values[(i + 1) / kWords][j][(i + 1) % kWords];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int element = (((tid >> 4) + 8 * (w / kWords)) * kWords + w % kWords) * 4 + i;
+                        *reinterpret_cast<uint4*>(v_smem + element * 128 + (((octet & 7) ^ (element & 7)) << 4)) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                    }
+                }
+                FenceProxyAsync();
+                MbarArrive(&v_full[stage]);
+                if (step + 1 < steps) {
+                    load_values(step + 1);
+                    lookup(step + 2);
+                }
+            }
+            WarpsSync(4, 128);
+            if (tid == 0) Advance<kUnit>(p, share_end, &places[kUnpackPlace]);
+            WarpsSync(4, 128);
+        } while (u.more);
+        }
+    } else {
+        if (busy && warp == kParamWarp) {
+        // ================================================ parameters =================================================
+        // A lane has four neighbouring tokens of a tile.
+        const Place& u = places[kParamPlace];
+        uint32_t tile_count = 0, unit_count = 0;
+        do {
+            const int steps = u.steps, first_token = u.t0 * kTokens;
+            int id;
+            bool has;   // this lane's tokens are in a block
+            uint4 kp, vp;
+            const auto lookup = [&](int step) { id = step < steps ? BlockOf(p, u, first_token + step * kTokens + lane * 4) : -1; };
+            const auto load = [&](int step) {
+                has = IsBlock(p, id);
+                kp = vp = make_uint4(0, 0, 0, 0);
+                if (has) {
+                    const int64_t at = TokenIndex(p, id, u.head, first_token + step * kTokens + lane * 4);
+                    kp = *reinterpret_cast<const uint4*>(p.cache.k_params + at);
+                    vp = *reinterpret_cast<const uint4*>(p.cache.v_params + at);
+                } else if (step < steps && SomeSeen(u, first_token + step * kTokens + lane * 4)) {
+                    ReportTimeout(p.status, kSiteAttention, u.b);
+                }
+            };
+            int up_exponent = kNoExponent;   // of the values, largest so far in the unit
+            lookup(0);
+            load(0);
+            wait(&back_full, unit_count & 1u, 9);
+            const float back = unit_back;
+            for (int step = 0; step < steps; ++step, ++tile_count) {
+                const uint32_t par = tile_count & 1u;
+                const int token = first_token + step * kTokens + lane * 4;
+                lookup(step + 1);
+                const uint32_t k4[4] = {kp.x, kp.y, kp.z, kp.w}, v4[4] = {vp.x, vp.y, vp.z, vp.w};
+                uint32_t there = 0, bad = 0;
+                float big_k = 0.0f, big_v = 0.0f, ks[4], km[4], vs[4], vm[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // a token with parameters that are no numbers spoils the rows that see it through its score; as an operand it
+                    // must not reach the others (0 * NaN is no zero)
+                    const bool here = has && token + i >= u.low && token + i < u.high;
+                    ks[i] = ParamScale(k4[i]);
+                    km[i] = ParamMin(k4[i]);
+                    vs[i] = ParamScale(v4[i]);
+                    vm[i] = ParamMin(v4[i]);
+                    const bool finite = ks[i] < INFINITY && fabsf(km[i]) < INFINITY && vs[i] < INFINITY && fabsf(vm[i]) < INFINITY;
+                    there |= (here ? 1u : 0u) << i;
+                    bad |= (here && !finite ? 1u : 0u) << i;
+                    if (!here || !finite) ks[i] = km[i] = vs[i] = vm[i] = 0.0f;
+                    big_k = fmaxf(big_k, fmaxf(fabsf(km[i]), fabsf(fmaf(15.0f, ks[i], km[i]))));
+                    big_v = fmaxf(big_v, fmaxf(fabsf(vm[i]), fabsf(fmaf(15.0f, vs[i], vm[i]))));
+                }
+                const uint32_t eight = 0xffu << (lane & 24);   // lanes of the same word
+                there = __reduce_or_sync(eight, there << (4 * (lane & 7)));
+                bad = __reduce_or_sync(eight, bad << (4 * (lane & 7)));
+                __syncwarp();
+                big_v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big_v)));
+                if (big_v > 0.0f) {
+                    const int e = QueryExponent(big_v);
+                    if (up_exponent == kNoExponent || e < up_exponent) up_exponent = e;
+                }
+                const float up = PowerOfTwo(up_exponent == kNoExponent ? 0 : up_exponent);
+                if (tile_count >= 2) wait(&tile_done[par], ((tile_count >> 1) & 1u) ^ 1u, 11);
+                if ((lane & 7) == 0) {
+                    present[par][lane >> 3] = there;
+                    spoiled[par][lane >> 3] = bad;
+                }
+                *reinterpret_cast<uint2*>(&value_scale[par][lane * 4]) = make_uint2(PackHalf(vs[0] * up, vs[1] * up), PackHalf(vs[2] * up, vs[3] * up));
+                *reinterpret_cast<uint2*>(&value_min[par][lane * 4]) = make_uint2(PackHalf(vm[0] * up, vm[1] * up), PackHalf(vm[2] * up, vm[3] * up));
+                if (lane == 0) value_up[par] = up;
+                if constexpr (kKeyCodes) {
+                    float4* a = reinterpret_cast<float4*>(params + par * (T::kParamBytes / 4)) + lane;
+                    a[0] = make_float4(ks[0] * back, ks[1] * back, ks[2] * back, ks[3] * back);
+                    a[kTokens / 4] = make_float4(km[0], km[1], km[2], km[3]);
+                } else {
+                    big_k = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big_k)));
+                    const int e = QueryExponent(big_k);
+                    const float ku = PowerOfTwo(e);
+                    *reinterpret_cast<uint2*>(&key_scale[par][lane * 4]) = make_uint2(PackHalf(ks[0] * ku, ks[1] * ku), PackHalf(ks[2] * ku, ks[3] * ku));
+                    *reinterpret_cast<uint2*>(&key_min[par][lane * 4]) = make_uint2(PackHalf(km[0] * ku, km[1] * ku), PackHalf(km[2] * ku, km[3] * ku));
+                    if (lane == 0) key_back[par] = back * PowerOfTwo(-e);
+                }
+                MbarArrive(&params_full[par]);
+                load(step + 1);
+            }
+            ++unit_count;
+            __syncwarp();
+            if (lane == 0) Advance<kUnit>(p, share_end, &places[kParamPlace]);
+            __syncwarp();
+        } while (u.more);
+        } else if (busy && warp == kIssueWarp) {
+        // ================================================ products ===================================================
+        if (lane == 0) {
+            const Place& u = places[kIssuePlace];
+            const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
+            const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
+            uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
+            const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
+                // S is written where the last tile's P was read
+                if (used[g] > 0) wait(&o_done[g], (used[g] - 1) & 1u, 8);
+                umma::FenceAfterThreadSync();
+                if (failed) return;
+                const uint32_t q = q_addr + g * T::kOperandBytes, k = k_addr + (tile % S) * T::kOperandBytes;
+#pragma unroll 1
+                for (int i = 0; i < T::kBlocks64; ++i) {
+                    const uint64_t qd = umma::SmemDesc(q + i * T::kPieceBytes, 0, 1024), kd = umma::SmemDesc(k + i * T::kPieceBytes, 0, 1024);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) MmaShared(tmem + g * 256, qd + 2 * j, kd + 2 * j, s_desc, i + j > 0);   // 32 bytes on
+                }
+                umma::Commit(&s_full[g]);
+            };
+            const auto values = [&](int g, uint32_t tile, bool first) {
+                wait(&p_full[g], used[g] & 1u, 4);
+                umma::FenceAfterThreadSync();
+                if (failed) return;
+                const uint32_t v = v_addr + (tile % S) * T::kOperandBytes;
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i) {
+                    const uint64_t vd = umma::SmemDesc(v + i * (D * 128), 0, 1024);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) MmaTensor(tmem + g * 256 + 128, tmem + g * 256 + i * 32 + j * 8, vd + 2 * j, o_desc, !first || i + j > 0);
+                }
+                umma::Commit(&o_done[g]);
+                ++used[g];
+            };
+            do {
+                const int steps = u.steps;
+                const int active = u.req.rows - u.row > kRows ? G : 1;   // tiles of rows that have any
+                wait(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+                for (int g = 0; g < G; ++g) {
+                    wait(&q_full[g], unit_count & 1u, 2);   // of a tile without rows too: its phases go on
+                    if (g < active) scores(g, tile_count);
+                }
+                umma::Commit(&k_empty[tile_count % S]);
+                for (int step = 0; step < steps && !failed; ++step, ++tile_count) {
+                    const bool more = step + 1 < steps;
+                    const uint32_t next = tile_count + 1;
+                    wait(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
+                    for (int g = 0; g < active; ++g) {
+                        values(g, tile_count, step == 0);
+                        if (g + 1 == active) {
+                            umma::Commit(&v_empty[tile_count % S]);
+                            umma::Commit(&tile_done[tile_count & 1u]);
+                        }
+                        if (more) {
+                            if (g == 0) wait(&k_full[next % S], (next / S) & 1u, 3);
+                            scores(g, next);
+                            if (g + 1 == active) umma::Commit(&k_empty[next % S]);
+                        }
+                    }
+                }
+                ++unit_count;
+                Advance<kUnit>(p, share_end, &places[kIssuePlace]);
+            } while (!failed && u.more);
+        }
         }
     }
     __syncwarp();

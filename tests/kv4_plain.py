@@ -127,7 +127,7 @@ def read(torch, cache, bs, slots):
     return out
 
 
-def attention(torch, cache, bs, table, q, lens, new, heads, scale, causal, window, hidden=()):
+def attention(torch, cache, bs, table, q, lens, new, heads, scale, causal, window, hidden=(), key_rounding=0.0):
     """(out, lse, limit, lse limit) in 64 bits; the limits are those of the kernels' arithmetic, see test_gpu_kv4.py."""
     rows, hq, dim = q.shape
     group = hq // heads
@@ -166,7 +166,7 @@ def attention(torch, cache, bs, table, q, lens, new, heads, scale, causal, windo
             clean_p = torch.where(spoiled[:, None] | ~some[:, None], 0.0, (p / mass).nan_to_num(0.0))
             clean_v = torch.where(seen.any(0)[:, None], vh, 0.0).nan_to_num(0.0)
             y = clean_p @ clean_v
-            score_error = torch.where(seen, size, 0.0).amax(-1) * 2.0 ** -23 * (dim / 16 + 8)
+            score_error = torch.where(seen, size, 0.0).amax(-1) * (2.0 ** -23 * (dim / 16 + 8) + key_rounding)
             weight_error = score_error + 2.0 ** -12 + 2.0 ** -20
             far = torch.where(seen.any(0)[:, None], clean_v, 0.0)
             spread = far.abs().amax() + y.abs().amax(-1, keepdim=True)

@@ -7,7 +7,9 @@ Tolerances count roundings.  eps(t) / 2 is the largest relative error of one rou
 * attention: q and codes enter exactly, scores are FP32 sums of at most 256 products of both signs of the minimum and the
   code part.  With A = scale * sum |q| * (|min| + 15 s) the score is off by at most 2^-23 * (256 / 16 + 8) * A (the matrix
   instruction adds 16 products at a time and truncates, a unit of 2^-23 each time), which multiplies a probability by at most
-  1 + that; a probability times its scale is rounded to 11 bits, 2^-12.  Weights off by a relative w each move a weighted mean
+  1 + that; a probability (times its scale, with few rows) is rounded to 11 bits, 2^-12.  With more than 16 rows a kv head values enter
+  rounded to 11 bits, 2^-12 * |v| each, which the bound below holds room for (the probabilities' part is 2^-12 * |v| then, and
+  |v| <= spread), and with BF16 queries the keys too: 2^-12 * A more on a score.  Weights off by a relative w each move a weighted mean
   of values by at most 2 w * mean(|v - out|) <= 2 w * spread, spread the largest |v - out|.  The sums over tokens add
   2^-23 * (tokens / 16 + 8) * (|v| + 15 s) in the worst case; one rounding to the output type ends it."""
 import ctypes as C
@@ -314,6 +316,10 @@ def test_rope_in_the_append_launch(cuda, dtype, tokens, hq, hk, dim, rotary, lay
     assert B.device_status() == 0
 
 
+def key_rounding(dtype, rows):
+    return 2.0 ** -12 if dtype == "bf16" and rows > 16 else 0.0
+
+
 # ---- attention ----------------------------------------------------------------------------------------------------------
 def attend(torch, *, dtype, lens, new, hq, hk, dim, bs, window=0, causal=True, seed=0, q_gain=1.0, v_gain=None, lse=True, starts=True, guard=2, scale=None,
            mutate=None, pad=0, max_query=None):
@@ -361,7 +367,7 @@ def attend(torch, *, dtype, lens, new, hq, hk, dim, bs, window=0, causal=True, s
     assert not ws[:4096].any(), "arrival counters are not back at zero"
     got = out[:rows, :hq * dim].reshape(rows, hq, dim).double()
     want, want_lse, limit, limit_lse = P.attention(torch, cache, bs, table, q[:rows, :hq * dim].reshape(rows, hq, dim), lens, new, hk,
-                                                   d.scale, causal, window)
+                                                   d.scale, causal, window, key_rounding=key_rounding(dtype, d.max_query * hq // hk))
     step = half_step(torch, dt)
     limit = limit + step * want.abs() + torch.finfo(dt).smallest_normal * step
     nan = want.isnan()
@@ -469,7 +475,7 @@ def test_block_numbers_outside_the_cache_hide_their_tokens(cuda, new):
         B.kv4_attention(r["desc"])
         assert B.device_status() >> 16 == 42
         got = r["out"][:new].reshape(new, 4, 128).double()
-        want, _, limit, _ = P.attention(torch, r["cache"], 16, table, r["q"][:new].reshape(new, 4, 128), [200], [new], 2, 128 ** -0.5, True, 0, hidden=range(32, 48))
+        want, _, limit, _ = P.attention(torch, r["cache"], 16, table, r["q"][:new].reshape(new, 4, 128), [200], [new], 2, 128 ** -0.5, True, 0, hidden=range(32, 48), key_rounding=key_rounding("bf16", 2 * new))
         assert ((got - want).abs() <= limit + 2.0 ** -8 * want.abs() + 1e-30).all()
         r["table"].copy_(table)
 
@@ -539,7 +545,7 @@ def test_lengths_change_under_a_captured_step(cuda):
         P.append(torch, mirror, bs, kr[:rows], v[:rows], slots[:rows])
         for name in cache:
             same(cache[name], mirror[name])
-        want, _, limit, _ = P.attention(torch, mirror, bs, table, qp[:rows], have, grow, hk, dim ** -0.5, True, 0)
+        want, _, limit, _ = P.attention(torch, mirror, bs, table, qp[:rows], have, grow, hk, dim ** -0.5, True, 0, key_rounding=key_rounding("bf16", 4 * capacity))
         got = (out if i % 2 == 0 else descs[1]._keep[2])[:rows].double()
         assert ((got - want).abs() <= limit + 2.0 ** -8 * want.abs() + 1e-30).all()
     del graphs, ws
@@ -570,7 +576,7 @@ def test_a_cache_beyond_four_gigabytes(cuda):
                                  query_start=torch.tensor([0, new], dtype=torch.int32, device="cuda"))
         B.kv4_attention_workspace(torch, d)
         B.kv4_attention(d)
-        want, _, limit, _ = P.attention(torch, cache, bs, table, q, lens, [new], hk, dim ** -0.5, True, 0)
+        want, _, limit, _ = P.attention(torch, cache, bs, table, q, lens, [new], hk, dim ** -0.5, True, 0, key_rounding=key_rounding("bf16", 2 * new))
         assert ((out.double() - want).abs() <= limit + 2.0 ** -8 * want.abs()).all()
     assert B.device_status() == 0
 
