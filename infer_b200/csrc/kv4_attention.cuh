@@ -219,8 +219,8 @@ __device__ __forceinline__ void FmaFour(float4& a, float w, float4 x) {
     a.w = fmaf(w, x.w, a.w);
 }
 // Joins the parts of a unit, in order: part i is slot 1 of block `first` for i = 0 and slot 0 of block first + i behind it.
-// Every part's weight is computed once into shared memory; the values are then read sixteen bytes at a time with no load
-// waiting for another.  `sync` is a barrier of the THREADS threads (thread = 0 .. THREADS - 1) that call this.
+// Every part's weight is computed once into shared memory, by as many lanes per row as there are parts; the values are then
+// read sixteen bytes at a time, four rows' pieces by four parts in flight together.  `sync` is a barrier of the THREADS threads (thread = 0 .. THREADS - 1) that call this.
 template <int D, int DTYPE, int THREADS, typename Sync>
 __device__ __forceinline__ void JoinParts(const AttentionParams& p, const Request& req, int head, int row, int rows, const float* partials, int first, int parts,
                                           int64_t slot_floats, float* shared, int shared_floats, int thread, Sync sync) {
@@ -231,44 +231,65 @@ __device__ __forceinline__ void JoinParts(const AttentionParams& p, const Reques
     if (at_once < 1) return;                     // cannot be: shared memory is sized for it
     float* best_of = shared;                     // [at_once] maximum, sum, sum for the lse
     float* weights = shared + 3 * at_once;       // [at_once][parts]
-    const int lane = thread & 31, warp = thread >> 5;
+    int lanes = 1;                               // that share a row
+    while (lanes < parts && lanes < 32) lanes <<= 1;
+    const int i0 = thread & (lanes - 1);
     for (int r0 = 0; r0 < rows; r0 += at_once) {
         const int count = rows - r0 < at_once ? rows - r0 : at_once;
         sync();
-        for (int r = warp; r < count; r += THREADS / 32) {
+        for (int first_row = 0; first_row < count; first_row += THREADS / lanes) {
+            const int r = first_row + thread / lanes;
             float best = kNoMax, total = 0.0f, mass = 0.0f;
+            if (r < count) {
 #pragma unroll 4
-            for (int i = lane; i < parts; i += 32) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (r0 + r) * kRow<D> + D));
-                weights[r * parts + i] = v.x;
-                const float next = fmaxf(best, v.x), old = Exp2(best - next), now = Exp2(v.x - next);
-                total = fmaf(now, v.z, total * old);
-                mass = fmaf(now, v.w, mass * old);
-                best = next;
+                for (int i = i0; i < parts; i += lanes) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i) + (r0 + r) * kRow<D> + D));
+                    weights[r * parts + i] = v.x;
+                    const float next = fmaxf(best, v.x), old = Exp2(best - next), now = Exp2(v.x - next);
+                    total = fmaf(now, v.z, total * old);
+                    mass = fmaf(now, v.w, mass * old);
+                    best = next;
+                }
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
+            __syncwarp();
+            for (int o = lanes >> 1; o > 0; o >>= 1) {
                 const float b = __shfl_xor_sync(0xffffffffu, best, o), t = __shfl_xor_sync(0xffffffffu, total, o), m = __shfl_xor_sync(0xffffffffu, mass, o);
                 const float next = fmaxf(best, b), old = Exp2(best - next), now = Exp2(b - next);
                 total = fmaf(now, t, total * old);
                 mass = fmaf(now, m, mass * old);
                 best = next;
             }
-            for (int i = lane; i < parts; i += 32) weights[r * parts + i] = Exp2(weights[r * parts + i] - best);
-            if (lane == 0) {
-                best_of[r] = best;
-                best_of[at_once + r] = total;
-                best_of[2 * at_once + r] = mass;
+            if (r < count) {
+                for (int i = i0; i < parts; i += lanes) weights[r * parts + i] = Exp2(weights[r * parts + i] - best);
+                if (i0 == 0) {
+                    best_of[r] = best;
+                    best_of[at_once + r] = total;
+                    best_of[2 * at_once + r] = mass;
+                }
             }
         }
         sync();
-        for (int i = thread; i < count * (D / 4); i += THREADS) {
-            const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-            float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 16
-            for (int c = 0; c < parts; ++c)
-                FmaFour(value, weights[r * parts + c], __ldcg(reinterpret_cast<const float4*>(slot(c) + (r0 + r) * kRow<D> + d)));
-            StoreFour<D, DTYPE>(p, req, head, row + r0 + r, d, value, best_of[at_once + r], best_of[r], best_of[2 * at_once + r]);
+        constexpr int kFours = 4;                // of a thread at a time
+        for (int i = thread; i < count * (D / 4); i += kFours * THREADS) {
+            float4 value[kFours];
+            int r[kFours], d[kFours];
+#pragma unroll
+            for (int j = 0; j < kFours; ++j) {
+                r[j] = (i + j * THREADS) / (D / 4);
+                d[j] = (i + j * THREADS - r[j] * (D / 4)) * 4;
+                if (r[j] >= count) r[j] = -1;
+                value[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll 4
+            for (int c = 0; c < parts; ++c) {
+                const float* from = slot(c);
+#pragma unroll
+                for (int j = 0; j < kFours; ++j)
+                    if (r[j] >= 0) FmaFour(value[j], weights[r[j] * parts + c], __ldcg(reinterpret_cast<const float4*>(from + (r0 + r[j]) * kRow<D> + d[j])));
+            }
+#pragma unroll
+            for (int j = 0; j < kFours; ++j)
+                if (r[j] >= 0) StoreFour<D, DTYPE>(p, req, head, row + r0 + r[j], d[j], value[j], best_of[at_once + r[j]], best_of[r[j]], best_of[2 * at_once + r[j]]);
         }
     }
 }

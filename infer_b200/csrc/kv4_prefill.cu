@@ -55,8 +55,9 @@ struct Tiles {
     static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V of one tile
     static constexpr int kKeys = kQueryTiles * kOperandBytes;      // stages of K, then of V
     static constexpr int kParams = kKeys + 2 * kStages * kOperandBytes;
-    static constexpr int kParamBytes = 2 * kTokens * 4;            // of one tile's keys; two tiles' worth
-    static constexpr size_t kBytes = kParams + 2 * kParamBytes + 1024;  // 1024: alignment
+    static constexpr int kParamStages = 4;                         // tiles whose parameters are prepared: two ahead of the operands
+    static constexpr int kParamBytes = 2 * kTokens * 4;            // of one tile's keys
+    static constexpr size_t kBytes = kParams + kParamStages * kParamBytes + 1024;  // 1024: alignment
     static constexpr uint32_t kTmemColumns = 512;
 };
 __device__ __forceinline__ void MmaShared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -66,6 +67,12 @@ __device__ __forceinline__ void MmaShared(uint32_t d, uint64_t a, uint64_t b, ui
 __device__ __forceinline__ void MmaTensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// One lane of the warp, the same at every call.
+__device__ __forceinline__ bool ElectOne() {
+    uint32_t chosen;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(chosen));
+    return chosen != 0;
 }
 __device__ __forceinline__ void TmemLoad32(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile(
@@ -223,22 +230,22 @@ __device__ __forceinline__ int64_t TokenIndex(const AttentionParams& p, int bloc
 template <int D, int DTYPE>
 __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __grid_constant__ AttentionParams p) {
     using T = Tiles<D>;
-    constexpr int kThreads = T::kThreads, G = T::kQueryTiles, S = T::kStages, kUnit = T::kUnitRows;
+    constexpr int kThreads = T::kThreads, G = T::kQueryTiles, S = T::kStages, P = T::kParamStages, kUnit = T::kUnitRows;
     constexpr bool kKeyCodes = DTYPE == FTH_B200_FP16;   // keys as codes, else as numbers
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(8) uint64_t q_full[G], s_full[G], p_full[G], o_done[G], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[2], tile_done[2], back_full;
+    __shared__ __align__(8) uint64_t q_full[G], s_full[G], p_full[G], o_done[G], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[P], tile_done[P], back_full;
     __shared__ int64_t unit_work[kThreads];
     __shared__ int64_t work_total;
     constexpr int kUnpackPlace = G, kIssuePlace = G + 1, kParamPlace = G + 2, kPlaces = G + 3;
     __shared__ Place places[kPlaces];      // one per tile of rows (softmax), unpacking, products, parameters
-    // of a tile, by its parity
-    __shared__ uint32_t present[2][4];     // a bit per token that some row may see
-    __shared__ uint32_t spoiled[2][4];     // a bit per token whose parameters are no numbers
-    __shared__ float value_up[2];          // power of two on the values
-    __shared__ float key_back[2];          // what takes scores to exponents of two (keys as numbers)
-    __shared__ __align__(16) __half value_scale[2][kTokens], value_min[2][kTokens], key_scale[2][kTokens], key_min[2][kTokens];
+    // of a tile
+    __shared__ uint32_t present[P][4];     // a bit per token that some row may see
+    __shared__ uint32_t spoiled[P][4];     // a bit per token whose parameters are no numbers
+    __shared__ float4 about[P];            // power of two on the values; 1 / that on the keys; 1: all present, none spoiled
+    __shared__ int64_t place_of[P][kTokens / 16];   // offset of the codes of sixteen tokens, -1: no block
+    __shared__ __align__(16) __half value_scale[P][kTokens], value_min[P][kTokens], key_scale[P][kTokens], key_min[P][kTokens];
     __shared__ float q_big[4 * G], unit_back;
     __shared__ int join_last[G];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             MbarInit(&v_full[s], 128);
             MbarInit(&v_empty[s], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < P; ++i) {
             MbarInit(&params_full[i], 32);
             MbarInit(&tile_done[i], 1);
         }
@@ -430,13 +437,14 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             if (lane == 0) q_big[warp] = big;
-            WarpsSync(3, T::kSoftmax);
+            // one power of two for the unit where it goes into the keys' parameters, else one for the tile of rows
+            WarpsSync(kKeyCodes ? 3 : 1 + g, kKeyCodes ? T::kSoftmax : 128);
 #pragma unroll
-            for (int w = 0; w < 4 * G; ++w) big = fmaxf(big, q_big[w]);
+            for (int w = 0; w < (kKeyCodes ? 4 * G : 4); ++w) big = fmaxf(big, q_big[kKeyCodes ? w : 4 * g + w]);
             const int e = QueryExponent(big);
-            const float up = PowerOfTwo(e);
-            if (threadIdx.x == 0) {
-                unit_back = p.scale_log2 * PowerOfTwo((kKeyCodes ? 24 : 0) - e);
+            const float up = PowerOfTwo(e), back = p.scale_log2 * PowerOfTwo((kKeyCodes ? 24 : 0) - e);
+            if (kKeyCodes && threadIdx.x == 0) {
+                unit_back = back;
                 MbarArrive(&back_full);
             }
             qsum *= p.scale_log2;
@@ -464,16 +472,15 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const int steps = u.steps, first_token = u.t0 * kTokens;
             if (!active) tile_count += steps;   // no rows
             for (int step = 0; active && step < steps; ++step, ++tile_count, ++used) {
-                const uint32_t par = tile_count & 1u;
-                wait(&params_full[par], (tile_count >> 1) & 1u, 10);
+                const uint32_t par = tile_count % P;
+                wait(&params_full[par], (tile_count / P) & 1u, 10);
+                const float4 tile = about[par];
+                const int token0 = first_token + step * kTokens;
+                const bool inside = __all_sync(0xffffffffu, tile.z != 0.0f && (!valid || (token0 >= low && token0 + kTokens <= high)));
                 wait(&s_full[g], used & 1u, 6);
                 __syncwarp();
                 umma::FenceAfterThreadSync();
-                const int token0 = first_token + step * kTokens;
-                const float back = key_back[par];
-                const bool all_there = (present[par][0] & present[par][1] & present[par][2] & present[par][3]) == 0xffffffffu && (spoiled[par][0] | spoiled[par][1] | spoiled[par][2] | spoiled[par][3]) == 0;
-                const bool inside = all_there && __all_sync(0xffffffffu, !valid || (token0 >= low && token0 + kTokens <= high));
-                const float tile_up = value_up[par];
+                const float tile_up = tile.x;
                 if (tile_up != up_now) {   // the same for every row
                     if (step > 0) ScaleResults<D>(o_tmem, tile_up / up_now);
                     up_now = tile_up;
@@ -497,7 +504,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                             z[2 * i + 1] = Fma2(make_float2(s4.z, s4.w), make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), Fma2(make_float2(m4.z, m4.w), qq, rr));
                         }
                     } else {
-                        const float2 bb = make_float2(back, back);
+                        const float2 bb = make_float2(back * tile.y, back * tile.y);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[i] = Fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), bb, rr);
                     }
@@ -649,51 +656,44 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         uint4 keys[kPieces];
         uint32_t values[kTasks][4][kWords];
         do {
-            const int steps = u.steps, first_token = u.t0 * kTokens;
-            int ids[kPieces], id;   // block numbers, fetched a tile before they are needed
-            const auto lookup = [&](int step) {
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) ids[j] = step < steps ? BlockOf(p, u, first_token + step * kTokens + token_of(j)) : -1;
-                id = step < steps ? BlockOf(p, u, first_token + step * kTokens + octet * 8) : -1;
-            };
-            const auto load_keys = [&](int step) {
+            const int steps = u.steps;
+            const auto load_keys = [&](uint32_t tile) {
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
+                    const int64_t from = place_of[tile % P][token_of(j) >> 4];
                     keys[j] = make_uint4(0, 0, 0, 0);
-                    if (IsBlock(p, ids[j])) keys[j] = LoadStream16(p.cache.k_codes + TokenIndex(p, ids[j], u.head, first_token + step * kTokens + token_of(j)) * (D / 2) + piece_of(j) * 16);
+                    if (from >= 0) keys[j] = LoadStream16(p.cache.k_codes + from + (token_of(j) & 15) * (D / 2) + piece_of(j) * 16);
                 }
             };
-            const auto load_values = [&](int step) {
-                const bool there = IsBlock(p, id);
-                const uint8_t* from = p.cache.v_codes + (there ? TokenIndex(p, id, u.head, first_token + step * kTokens + octet * 8) * (D / 2) : 0);
+            const auto load_values = [&](uint32_t tile) {
+                const int64_t from = place_of[tile % P][octet >> 1];
+                const uint8_t* codes = p.cache.v_codes + from + (octet & 1) * (8 * D / 2) + (tid >> 4) * (kWords * 4);
 #pragma unroll
                 for (int t = 0; t < kTasks; ++t)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint8_t* row = from + j * D + ((tid >> 4) + 8 * t) * (kWords * 4);
+                        const uint8_t* row = codes + j * D + 8 * t * (kWords * 4);
                         if constexpr (kWords == 4) {
-                            const uint4 x = there ? LoadStream16(row) : make_uint4(0, 0, 0, 0);
+                            const uint4 x = from >= 0 ? LoadStream16(row) : make_uint4(0, 0, 0, 0);
                             values[t][j][0] = x.x;
                             values[t][j][1] = x.y;
                             values[t][j][2] = x.z;
                             values[t][j][3] = x.w;
                         } else {
-                            const uint2 x = there ? *reinterpret_cast<const uint2*>(row) : make_uint2(0, 0);
+                            const uint2 x = from >= 0 ? *reinterpret_cast<const uint2*>(row) : make_uint2(0, 0);
                             values[t][j][0] = x.x;
                             values[t][j][1] = x.y;
                         }
                     }
             };
-            lookup(0);
-            load_keys(0);
-            load_values(0);
-            lookup(1);
+            wait(&params_full[tile_count % P], (tile_count / P) & 1u, 10);
+            load_keys(tile_count);
+            load_values(tile_count);
             for (int step = 0; step < steps; ++step, ++tile_count) {
-                const uint32_t stage = tile_count % S, turn = (tile_count / S) & 1u, par = tile_count & 1u;
+                const uint32_t stage = tile_count % S, turn = (tile_count / S) & 1u, par = tile_count % P, next = tile_count + 1;
                 uint8_t* const k_smem = smem + T::kKeys + stage * T::kOperandBytes;
                 uint8_t* const v_smem = smem + T::kKeys + (S + stage) * T::kOperandBytes + (octet >> 3) * (D * 128);
                 if (tile_count >= S) wait(&k_empty[stage], turn ^ 1u, 0);
-                wait(&params_full[par], (tile_count >> 1) & 1u, 10);
 #pragma unroll 1
                 for (int j = 0; j < kPieces; ++j) {
                     const int token = token_of(j), piece = piece_of(j);
@@ -717,7 +717,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 }
                 FenceProxyAsync();
                 MbarArrive(&k_full[stage]);
-                if (step + 1 < steps) load_keys(step + 1);
+                if (step + 1 < steps) {
+                    wait(&params_full[next % P], (next / P) & 1u, 10);
+                    load_keys(next);
+                }
                 if (tile_count >= S) wait(&v_empty[stage], turn ^ 1u, 1);
                 const uint4 s4 = *reinterpret_cast<const uint4*>(&value_scale[par][octet * 8]), m4 = *reinterpret_cast<const uint4*>(&value_min[par][octet * 8]);
                 const uint32_t sp[4] = {s4.x, s4.y, s4.z, s4.w}, mp[4] = {m4.x, m4.y, m4.z, m4.w};
@@ -742,10 +745,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 }
                 FenceProxyAsync();
                 MbarArrive(&v_full[stage]);
-                if (step + 1 < steps) {
-                    load_values(step + 1);
-                    lookup(step + 2);
-                }
+                if (step + 1 < steps) load_values(next);
             }
             WarpsSync(4, 128);
             if (tid == 0) Advance<kUnit>(p, share_end, &places[kUnpackPlace]);
@@ -761,14 +761,15 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         do {
             const int steps = u.steps, first_token = u.t0 * kTokens;
             int id;
-            bool has;   // this lane's tokens are in a block
+            bool has;     // this lane's tokens are in a block
+            int64_t at;
             uint4 kp, vp;
             const auto lookup = [&](int step) { id = step < steps ? BlockOf(p, u, first_token + step * kTokens + lane * 4) : -1; };
             const auto load = [&](int step) {
                 has = IsBlock(p, id);
                 kp = vp = make_uint4(0, 0, 0, 0);
                 if (has) {
-                    const int64_t at = TokenIndex(p, id, u.head, first_token + step * kTokens + lane * 4);
+                    at = TokenIndex(p, id, u.head, first_token + step * kTokens + lane * 4);
                     kp = *reinterpret_cast<const uint4*>(p.cache.k_params + at);
                     vp = *reinterpret_cast<const uint4*>(p.cache.v_params + at);
                 } else if (step < steps && SomeSeen(u, first_token + step * kTokens + lane * 4)) {
@@ -778,10 +779,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             int up_exponent = kNoExponent;   // of the values, largest so far in the unit
             lookup(0);
             load(0);
-            wait(&back_full, unit_count & 1u, 9);
-            const float back = unit_back;
+            if (kKeyCodes) wait(&back_full, unit_count & 1u, 9);
+            const float back = kKeyCodes ? unit_back : 1.0f;
             for (int step = 0; step < steps; ++step, ++tile_count) {
-                const uint32_t par = tile_count & 1u;
+                const uint32_t par = tile_count % P;
                 const int token = first_token + step * kTokens + lane * 4;
                 lookup(step + 1);
                 const uint32_t k4[4] = {kp.x, kp.y, kp.z, kp.w}, v4[4] = {vp.x, vp.y, vp.z, vp.w};
@@ -813,14 +814,16 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     if (up_exponent == kNoExponent || e < up_exponent) up_exponent = e;
                 }
                 const float up = PowerOfTwo(up_exponent == kNoExponent ? 0 : up_exponent);
-                if (tile_count >= 2) wait(&tile_done[par], ((tile_count >> 1) & 1u) ^ 1u, 11);
+                if (tile_count >= P) wait(&tile_done[par], ((tile_count / P) & 1u) ^ 1u, 11);
                 if ((lane & 7) == 0) {
                     present[par][lane >> 3] = there;
                     spoiled[par][lane >> 3] = bad;
                 }
                 *reinterpret_cast<uint2*>(&value_scale[par][lane * 4]) = make_uint2(PackHalf(vs[0] * up, vs[1] * up), PackHalf(vs[2] * up, vs[3] * up));
                 *reinterpret_cast<uint2*>(&value_min[par][lane * 4]) = make_uint2(PackHalf(vm[0] * up, vm[1] * up), PackHalf(vm[2] * up, vm[3] * up));
-                if (lane == 0) value_up[par] = up;
+                if ((lane & 3) == 0) place_of[par][lane >> 2] = has ? at * (D / 2) : -1;   // this lane's first token is the sixteen's first
+                const bool plain = __all_sync(0xffffffffu, there == 0xffffffffu && bad == 0);
+                float down = 1.0f;   // of the keys
                 if constexpr (kKeyCodes) {
                     float4* a = reinterpret_cast<float4*>(params + par * (T::kParamBytes / 4)) + lane;
                     a[0] = make_float4(ks[0] * back, ks[1] * back, ks[2] * back, ks[3] * back);
@@ -831,8 +834,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     const float ku = PowerOfTwo(e);
                     *reinterpret_cast<uint2*>(&key_scale[par][lane * 4]) = make_uint2(PackHalf(ks[0] * ku, ks[1] * ku), PackHalf(ks[2] * ku, ks[3] * ku));
                     *reinterpret_cast<uint2*>(&key_min[par][lane * 4]) = make_uint2(PackHalf(km[0] * ku, km[1] * ku), PackHalf(km[2] * ku, km[3] * ku));
-                    if (lane == 0) key_back[par] = back * PowerOfTwo(-e);
+                    down = PowerOfTwo(-e);
                 }
+                if (lane == 0) about[par] = make_float4(up, down, plain ? 1.0f : 0.0f, 0.0f);
                 MbarArrive(&params_full[par]);
                 load(step + 1);
             }
@@ -843,69 +847,86 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         } while (u.more);
         } else if (busy && warp == kIssueWarp) {
         // ================================================ products ===================================================
-        if (lane == 0) {
-            const Place& u = places[kIssuePlace];
-            const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
-            const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
-            uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
-            const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
-                // S is written where the last tile's P was read
-                if (used[g] > 0) wait(&o_done[g], (used[g] - 1) & 1u, 8);
-                umma::FenceAfterThreadSync();
-                if (failed) return;
-                const uint32_t q = q_addr + g * T::kOperandBytes, k = k_addr + (tile % S) * T::kOperandBytes;
-#pragma unroll 1
-                for (int i = 0; i < T::kBlocks64; ++i) {
-                    const uint64_t qd = umma::SmemDesc(q + i * T::kPieceBytes, 0, 1024), kd = umma::SmemDesc(k + i * T::kPieceBytes, 0, 1024);
+        // The whole warp runs the loops, so that descriptors are computed once for the warp and not gathered from a lane
+        // (82 .. 93 cycles per product when one lane did); one lane issues.
+        const Place& u = places[kIssuePlace];
+        const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
+        const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
+        const uint32_t d_tmem = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
+        const auto wait_all = [&](uint64_t* bar, uint32_t parity, int detail) {
+            if (!failed && !WaitFor(bar, parity, p.status, 16 + detail)) failed = true;
+            failed = __any_sync(0xffffffffu, failed);
+        };
+        const auto commit = [&](uint64_t* bar) {
+            if (ElectOne()) umma::Commit(bar);
+        };
+        const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
+            // S is written where the last tile's P was read
+            if (used[g] > 0) wait_all(&o_done[g], (used[g] - 1) & 1u, 8);
+            umma::FenceAfterThreadSync();
+            if (failed) return;
+            const uint64_t qd = umma::SmemDesc(q_addr + g * T::kOperandBytes, 0, 1024), kd = umma::SmemDesc(k_addr + (tile % S) * T::kOperandBytes, 0, 1024);
+            if (ElectOne()) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) MmaShared(tmem + g * 256, qd + 2 * j, kd + 2 * j, s_desc, i + j > 0);   // 32 bytes on
+                for (int i = 0; i < T::kBlocks64 * 4; ++i) {   // 32 bytes on, then the next piece
+                    const uint64_t at = (i >> 2) * (T::kPieceBytes >> 4) + (i & 3) * 2;
+                    MmaShared(d_tmem + g * 256, qd + at, kd + at, s_desc, i > 0);
                 }
                 umma::Commit(&s_full[g]);
-            };
-            const auto values = [&](int g, uint32_t tile, bool first) {
-                wait(&p_full[g], used[g] & 1u, 4);
-                umma::FenceAfterThreadSync();
-                if (failed) return;
-                const uint32_t v = v_addr + (tile % S) * T::kOperandBytes;
-#pragma unroll 1
-                for (int i = 0; i < 2; ++i) {
-                    const uint64_t vd = umma::SmemDesc(v + i * (D * 128), 0, 1024);
+            }
+            __syncwarp();
+        };
+        const auto values = [&](int g, uint32_t tile, bool first) {
+            wait_all(&p_full[g], used[g] & 1u, 4);
+            umma::FenceAfterThreadSync();
+            if (failed) return;
+            const uint64_t vd = umma::SmemDesc(v_addr + (tile % S) * T::kOperandBytes, 0, 1024);
+            if (ElectOne()) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) MmaTensor(tmem + g * 256 + 128, tmem + g * 256 + i * 32 + j * 8, vd + 2 * j, o_desc, !first || i + j > 0);
-                }
+                for (int i = 0; i < kTokens / 16; ++i)
+                    MmaTensor(d_tmem + g * 256 + 128, d_tmem + g * 256 + i * 8, vd + (i >> 2) * (D * 128 >> 4) + (i & 3) * 2, o_desc, !first || i > 0);
                 umma::Commit(&o_done[g]);
-                ++used[g];
-            };
-            do {
-                const int steps = u.steps;
-                const int active = u.req.rows - u.row > kRows ? G : 1;   // tiles of rows that have any
-                wait(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+            }
+            __syncwarp();
+            ++used[g];
+        };
+        bool more_units = true;
+        do {
+            const int steps = __shfl_sync(0xffffffffu, u.steps, 0);
+            const int active = __shfl_sync(0xffffffffu, u.req.rows - u.row > kRows ? G : 1, 0);   // tiles of rows that have any
+            wait_all(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                wait_all(&q_full[g], unit_count & 1u, 2);   // of a tile without rows too: its phases go on
+                if (g < active) scores(g, tile_count);
+            }
+            commit(&k_empty[tile_count % S]);
+            for (int step = 0; step < steps && !failed; ++step, ++tile_count) {
+                const bool more = step + 1 < steps;
+                const uint32_t next = tile_count + 1;
+                wait_all(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
+#pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    wait(&q_full[g], unit_count & 1u, 2);   // of a tile without rows too: its phases go on
-                    if (g < active) scores(g, tile_count);
-                }
-                umma::Commit(&k_empty[tile_count % S]);
-                for (int step = 0; step < steps && !failed; ++step, ++tile_count) {
-                    const bool more = step + 1 < steps;
-                    const uint32_t next = tile_count + 1;
-                    wait(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
-                    for (int g = 0; g < active; ++g) {
-                        values(g, tile_count, step == 0);
-                        if (g + 1 == active) {
-                            umma::Commit(&v_empty[tile_count % S]);
-                            umma::Commit(&tile_done[tile_count & 1u]);
-                        }
-                        if (more) {
-                            if (g == 0) wait(&k_full[next % S], (next / S) & 1u, 3);
-                            scores(g, next);
-                            if (g + 1 == active) umma::Commit(&k_empty[next % S]);
-                        }
+                    if (g >= active) break;
+                    values(g, tile_count, step == 0);
+                    if (g + 1 == active) {
+                        commit(&v_empty[tile_count % S]);
+                        commit(&tile_done[tile_count % P]);
+                    }
+                    if (more) {
+                        if (g == 0) wait_all(&k_full[next % S], (next / S) & 1u, 3);
+                        scores(g, next);
+                        if (g + 1 == active) commit(&k_empty[next % S]);
                     }
                 }
-                ++unit_count;
-                Advance<kUnit>(p, share_end, &places[kIssuePlace]);
-            } while (!failed && u.more);
-        }
+            }
+            ++unit_count;
+            __syncwarp();
+            if (lane == 0) Advance<kUnit>(p, share_end, &places[kIssuePlace]);
+            __syncwarp();
+            more_units = __shfl_sync(0xffffffffu, u.more, 0) != 0;
+        } while (!failed && more_units);
         }
     }
     __syncwarp();
