@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         t0 = tile_first + static_cast<int>(into);
         steps = static_cast<int>(tiles < left ? tiles : left);
         int unused;
-        Visible(p, req, row / p.group, &first_low, &unused);
-        Visible(p, req, ((row + R < req.rows ? row + R : req.rows) - 1) / p.group, &unused, &last_high);
+        Visible(p, req, QueryOf(p, row), &first_low, &unused);
+        Visible(p, req, QueryOf(p, (row + R < req.rows ? row + R : req.rows) - 1), &unused, &last_high);
     };
     const auto next_unit = [&] {   // false: the share is done
         at += steps;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
             for (int n = 0; n < NT; ++n) {
                 const int r = row + n * 8 + g;
                 const bool valid = r < req.rows;
-                const int query = valid ? r / p.group : 0;
+                const int query = valid ? QueryOf(p, r) : 0;
                 const uint16_t* from = static_cast<const uint16_t*>(p.q) + (req.first_row + static_cast<int64_t>(query)) * p.ldq +
                                        (static_cast<int64_t>(head) * p.group + r - query * p.group) * D;
 #pragma unroll
@@ -808,6 +808,7 @@ extern "C" int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* d, fth_
     p.max_query = d->max_query;
     p.kv_heads = d->cache.kv_heads;
     p.group = d->q_heads / d->cache.kv_heads;
+    p.group_inverse = 0xffffffffu / static_cast<uint32_t>(p.group);
     p.causal = d->causal != 0;
     p.window = d->window;
     p.q_vec = kv4::AlignedTo(d->q, 16) && p.ldq % 8 == 0;

@@ -22,6 +22,7 @@ struct AttentionParams {
     const int32_t* total_lens;
     const int32_t* query_start;
     int requests, max_blocks, max_query, kv_heads, group, causal, window, q_vec, out_vec;
+    uint32_t group_inverse;  // floor((2^32 - 1) / group)
     int few_units;     // no request has more than a few units of rows
     float scale_log2;  // scale * log2(e): scores are kept as exponents of two
     int* status;
@@ -29,6 +30,11 @@ struct AttentionParams {
     float* partials;   // [block of threads][2][rows of a unit][head_dim values, maximum, unused, sum, sum for the lse]
 };
 
+// row / group.  The product is at most one short: row / group - row * inverse / 2^32 < (row / 2^32) * 2 <= 1.
+__device__ __forceinline__ int QueryOf(const AttentionParams& p, int row) {
+    const uint32_t q = __umulhi(static_cast<uint32_t>(row), p.group_inverse);
+    return static_cast<int>(q + (static_cast<uint32_t>(row) - q * static_cast<uint32_t>(p.group) >= static_cast<uint32_t>(p.group) ? 1u : 0u));
+}
 // The rows of one request and what they see.  Row i of n stands at position total - n + i.
 struct Request {
     int first_row;  // row of its first query in q
@@ -77,8 +83,8 @@ __device__ __forceinline__ void UnitTiles(const AttentionParams& p, const Reques
     int end = row + count;
     if (end > r.rows) end = r.rows;
     int l0, h0, l1, h1;
-    Visible(p, r, row / p.group, &l0, &h0);
-    Visible(p, r, (end - 1) / p.group, &l1, &h1);
+    Visible(p, r, QueryOf(p, row), &l0, &h0);
+    Visible(p, r, QueryOf(p, end - 1), &l1, &h1);
     *first = l0 / TILE;
     *last = h1 > 0 ? (h1 + TILE - 1) / TILE : 0;
     if (*last <= *first) *last = *first + 1;
@@ -138,6 +144,13 @@ __device__ __forceinline__ uint32_t PackHalf(float low, float high) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <int DTYPE>
+__device__ __forceinline__ uint32_t PackTo(float low, float high) {
+    if constexpr (DTYPE == FTH_B200_FP16) return PackHalf(low, high);
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(high), "f"(low));
+    return d;
+}
+template <int DTYPE>
 __device__ __forceinline__ float2 HalfPair(uint32_t x) {
     if constexpr (DTYPE == FTH_B200_BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
     else return __half22float2(*reinterpret_cast<const __half2*>(&x));
@@ -189,22 +202,14 @@ constexpr int kRow = D + 4;
 // with its first elements.
 template <int D, int DTYPE>
 __device__ __forceinline__ void StoreFour(const AttentionParams& p, const Request& req, int head, int row, int d, float4 v, float total, float best, float mass) {
-    const int query = row / p.group;
+    const int query = QueryOf(p, row);
     const int64_t q_row = req.first_row + static_cast<int64_t>(query);
     const int q_head = head * p.group + row - query * p.group;
     const float scale = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
     const float x[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
     const int64_t at = q_row * p.ldo + static_cast<int64_t>(q_head) * D + d;
     if (p.out_vec) {
-        uint2 packed;
-        if constexpr (DTYPE == FTH_B200_BF16) {
-            packed.x = EncodeBf16Cast(x[0]) | (static_cast<uint32_t>(EncodeBf16Cast(x[1])) << 16);
-            packed.y = EncodeBf16Cast(x[2]) | (static_cast<uint32_t>(EncodeBf16Cast(x[3])) << 16);
-        } else {
-            packed.x = PackHalf(x[0], x[1]);
-            packed.y = PackHalf(x[2], x[3]);
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = packed;
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(PackTo<DTYPE>(x[0], x[1]), PackTo<DTYPE>(x[2], x[3]));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) rowops::WriteFloat<DTYPE>(p.out, at + i, x[i]);
@@ -220,7 +225,7 @@ __device__ __forceinline__ void FmaFour(float4& a, float w, float4 x) {
 }
 // Joins the parts of a unit, in order: part i is slot 1 of block `first` for i = 0 and slot 0 of block first + i behind it.
 // Every part's weight is computed once into shared memory, by as many lanes per row as there are parts; the values are then
-// read sixteen bytes at a time, four rows' pieces by four parts in flight together.  `sync` is a barrier of the THREADS threads (thread = 0 .. THREADS - 1) that call this.
+// read sixteen bytes at a time, four pieces by four parts in flight together.  `sync` is a barrier of the THREADS threads (thread = 0 .. THREADS - 1) that call this.
 template <int D, int DTYPE, int THREADS, typename Sync>
 __device__ __forceinline__ void JoinParts(const AttentionParams& p, const Request& req, int head, int row, int rows, const float* partials, int first, int parts,
                                           int64_t slot_floats, float* shared, int shared_floats, int thread, Sync sync) {

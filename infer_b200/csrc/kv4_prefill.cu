@@ -19,6 +19,9 @@
 // together has to stay in the SM's instruction cache (fully unrolled, with keys and values in separate warps, a quarter of
 // the fetches missed it and 3 prompts of 4000 rows took 1.97 ms).
 //
+// Scores of half a tile and probabilities of the other half lie side by side: the matrix unit multiplies one while the other
+// becomes probabilities.
+//
 // A block of threads has two tiles of query rows (one for 256-wide heads, whose results fill tensor memory) that share the
 // unpacked tokens: while one's scores become probabilities the matrix unit works for the other.  Unpacked tiles are
 // double-buffered (not for 256-wide heads, where shared memory holds one).
@@ -48,8 +51,8 @@ struct Tiles {
     static constexpr int kQueryTiles = D == 256 ? 1 : 2;
     static constexpr int kUnitRows = kQueryTiles * kRows;
     static constexpr int kStages = D == 256 ? 1 : 2;               // unpacked tiles of tokens
-    static constexpr int kSoftmax = kQueryTiles * 128;             // threads: softmax, then unpacking, then a warp that issues
-    static constexpr int kThreads = kSoftmax + 128 + 64;           // products and one for parameters
+    static constexpr int kSoftmax = kQueryTiles * 128;             // threads: softmax, then unpacking, then a warp for parameters
+    static constexpr int kThreads = kSoftmax + 128 + 32 + kQueryTiles * 32;   // and one per tile of rows that issues products
     static constexpr int kBlocks64 = D / 64;                       // 128-byte wide pieces of a row
     static constexpr int kPieceBytes = 128 * 128;
     static constexpr int kOperandBytes = kBlocks64 * kPieceBytes;  // Q, K or V of one tile
@@ -170,8 +173,8 @@ __device__ __forceinline__ void Settle(const AttentionParams& p, int64_t share_e
     u.t0 = u.tile_first + static_cast<int>(u.into);
     u.steps = static_cast<int>(tiles < left ? tiles : left);
     int unused;
-    Visible(p, u.req, u.row / p.group, &u.low, &unused);
-    Visible(p, u.req, ((u.row + UNIT < u.req.rows ? u.row + UNIT : u.req.rows) - 1) / p.group, &unused, &u.high);
+    Visible(p, u.req, QueryOf(p, u.row), &u.low, &unused);
+    Visible(p, u.req, QueryOf(p, (u.row + UNIT < u.req.rows ? u.row + UNIT : u.req.rows) - 1), &unused, &u.high);
     u.more = 1;
 }
 // By one thread of the group.
@@ -235,11 +238,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(8) uint64_t q_full[G], s_full[G], p_full[G], o_done[G], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[P], tile_done[P], back_full;
+    __shared__ __align__(8) uint64_t q_full[G], s_full[G][2], p_full[G][2], o_done[G][2], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[P], tile_done[P], back_full;
     __shared__ int64_t unit_work[kThreads];
     __shared__ int64_t work_total;
-    constexpr int kUnpackPlace = G, kIssuePlace = G + 1, kParamPlace = G + 2, kPlaces = G + 3;
-    __shared__ Place places[kPlaces];      // one per tile of rows (softmax), unpacking, products, parameters
+    constexpr int kUnpackPlace = G, kParamPlace = G + 1, kIssuePlace = G + 2, kPlaces = 2 * G + 2;
+    __shared__ Place places[kPlaces];      // one per tile of rows (softmax), unpacking, parameters, one per tile of rows (products)
     // of a tile
     __shared__ uint32_t present[P][4];     // a bit per token that some row may see
     __shared__ uint32_t spoiled[P][4];     // a bit per token whose parameters are no numbers
@@ -249,23 +252,25 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
     __shared__ float q_big[4 * G], unit_back;
     __shared__ int join_last[G];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kUnpackWarp = T::kSoftmax / 32, kIssueWarp = kUnpackWarp + 4, kParamWarp = kIssueWarp + 1;
+    constexpr int kUnpackWarp = T::kSoftmax / 32, kParamWarp = kUnpackWarp + 4, kIssueWarp = kParamWarp + 1;
     if (threadIdx.x == 0) {
         for (int g = 0; g < G; ++g) {
             MbarInit(&q_full[g], 128);
-            MbarInit(&s_full[g], 1);
-            MbarInit(&p_full[g], 128);
-            MbarInit(&o_done[g], 1);
+            for (int h = 0; h < 2; ++h) {
+                MbarInit(&s_full[g][h], 1);
+                MbarInit(&p_full[g][h], 128);
+                MbarInit(&o_done[g][h], 1);
+            }
         }
         for (int s = 0; s < S; ++s) {
             MbarInit(&k_full[s], 128);
-            MbarInit(&k_empty[s], 1);
+            MbarInit(&k_empty[s], G);
             MbarInit(&v_full[s], 128);
-            MbarInit(&v_empty[s], 1);
+            MbarInit(&v_empty[s], G);
         }
         for (int i = 0; i < P; ++i) {
             MbarInit(&params_full[i], 32);
-            MbarInit(&tile_done[i], 1);
+            MbarInit(&tile_done[i], G);
         }
         MbarInit(&back_full, 1);
         FenceBarrierInit();
@@ -401,38 +406,41 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         const Place& u = places[g];
         uint32_t tile_count = 0, unit_count = 0, used = 0;
         for (;;) {
-            // ---- the unit's queries, as operands
-            const int row = u.row + g * kRows + r;
+            // ---- the unit's queries, as operands: copied as they are, measured by the thread that owns the row, rewritten in place
+            const int tile_row = u.row + g * kRows, row = tile_row + r;
             const bool active = g == 0 || u.req.rows - u.row > kRows;
             const bool valid = row < u.req.rows;
-            const int query = valid ? row / p.group : 0;
-            const uint16_t* from = static_cast<const uint16_t*>(p.q) + (u.req.first_row + static_cast<int64_t>(query)) * p.ldq +
-                                   (static_cast<int64_t>(u.head) * p.group + (row - query * p.group)) * D;
-            // the row stays in registers between the two passes when it fits (all its loads in flight together)
-            constexpr int kHeld = D <= 128 ? D / 8 : 1;
-            uint4 held[kHeld];
-            const auto fetch = [&](int w) {
-                if (!valid) return make_uint4(0, 0, 0, 0);
-                return p.q_vec ? *reinterpret_cast<const uint4*>(from + w * 8) : LoadUnaligned8(from + w * 8);
-            };
+            const int query = valid ? QueryOf(p, row) : 0;
+            const auto piece = [&](int of, int w) { return reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + of * 128 + (((w & 7) ^ (of & 7)) << 4)); };
+            const int64_t own = (u.req.first_row + static_cast<int64_t>(query)) * p.ldq + (static_cast<int64_t>(u.head) * p.group + (row - query * p.group)) * D;
+            {   // the 32 rows of a warp, neighbouring lanes neighbouring pieces of a row
+                constexpr int kLanes = D / 8 < 32 ? D / 8 : 32, kRowsAtOnce = 32 / kLanes;
+                const int w = lane % kLanes;
+                const auto copy = [&](int i, auto fetch) {
+                    const int lane_of = i * kRowsAtOnce + lane / kLanes, of = (warp & 3) * 32 + lane_of;
+                    const int64_t from = __shfl_sync(0xffffffffu, own, lane_of);
+                    *piece(of, w) = tile_row + of < u.req.rows ? fetch(static_cast<const uint16_t*>(p.q) + from + w * 8) : make_uint4(0, 0, 0, 0);
+                };
+                if (p.q_vec) {
+#pragma unroll 8
+                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) copy(i, [](const uint16_t* from) { return *reinterpret_cast<const uint4*>(from); });
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) copy(i, [](const uint16_t* from) { return LoadUnaligned8(from); });
+                }
+                __syncwarp();
+            }
             float big = 0.0f, qsum = 0.0f;
-            const auto measure = [&](uint4 x) {
+#pragma unroll 2
+            for (int w = 0; w < D / 8; ++w) {
+                const uint4 x = *piece(r, w);
                 const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 v = HalfPair<DTYPE>(raw[i]);
-                    big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
-                    qsum += v.x + v.y;
+                    big = Max3(big, fabsf(v.x), fabsf(v.y));
+                    if constexpr (kKeyCodes) qsum += v.x + v.y;
                 }
-            };
-            if constexpr (D <= 128) {
-#pragma unroll
-                for (int w = 0; w < D / 8; ++w) held[w] = fetch(w);
-#pragma unroll
-                for (int w = 0; w < D / 8; ++w) measure(held[w]);
-            } else {
-#pragma unroll 8
-                for (int w = 0; w < D / 8; ++w) measure(fetch(w));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
@@ -448,18 +456,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 MbarArrive(&back_full);
             }
             qsum *= p.scale_log2;
-            const auto place = [&](int w, uint4 x) {
+#pragma unroll 2
+            for (int w = 0; w < D / 8; ++w) {
+                const uint4 x = *piece(r, w);
                 const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
                 uint32_t f[4];
                 QueryOperands<DTYPE>(raw, up, kKeyCodes ? 0.0625f : 1.0f, f);
-                *reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + r * 128 + (((w & 7) ^ (r & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
-            };
-            if constexpr (D <= 128) {
-#pragma unroll
-                for (int w = 0; w < D / 8; ++w) place(w, held[w]);
-            } else {
-#pragma unroll 8
-                for (int w = 0; w < D / 8; ++w) place(w, fetch(w));
+                *piece(r, w) = make_uint4(f[0], f[1], f[2], f[3]);
             }
             FenceProxyAsync();
             MbarArrive(&q_full[g]);
@@ -477,21 +480,29 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 const float4 tile = about[par];
                 const int token0 = first_token + step * kTokens;
                 const bool inside = __all_sync(0xffffffffu, tile.z != 0.0f && (!valid || (token0 >= low && token0 + kTokens <= high)));
-                wait(&s_full[g], used & 1u, 6);
-                __syncwarp();
-                umma::FenceAfterThreadSync();
                 const float tile_up = tile.x;
                 if (tile_up != up_now) {   // the same for every row
-                    if (step > 0) ScaleResults<D>(o_tmem, tile_up / up_now);
+                    if (step > 0) {
+                        wait(&o_done[g][1], (used - 1) & 1u, 7);
+                        __syncwarp();
+                        umma::FenceAfterThreadSync();
+                        ScaleResults<D>(o_tmem, tile_up / up_now);
+                    }
                     up_now = tile_up;
                 }
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
+                    const int h = c >> 1;
+                    const uint32_t p_tmem = s_tmem + h * 64;   // the half's probabilities, over its scores
                     uint32_t s[32];
+                    if ((c & 1) == 0) {
+                        wait(&s_full[g][h], used & 1u, 6);
+                        __syncwarp();
+                        umma::FenceAfterThreadSync();
+                    }
                     __syncwarp();
                     TmemLoad32(s_tmem + c * 32, s);
                     float2 z[16];
-                    float best = -INFINITY;
                     const float2 rr = make_float2(-ref, -ref);
                     if constexpr (kKeyCodes) {
                         const float4* ks = reinterpret_cast<const float4*>(params + par * (T::kParamBytes / 4) + c * 32);
@@ -522,10 +533,12 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                         const uint32_t bad = spoiled[par][c] & seen;
                         if (bad != 0) z[0].x = NAN;   // the row is NaN, whichever token makes it
                     }
+                    float bests[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) best = Max3(best, z[i].x, z[i].y);
+                    for (int i = 0; i < 16; ++i) bests[i & 3] = Max3(bests[i & 3], z[i].x, z[i].y);
+                    const float best = Max3(fmaxf(bests[0], bests[1]), bests[2], bests[3]);
                     if (__builtin_expect(__any_sync(0xffffffffu, best > limit), 0)) {
-                        // move the maximum: scores of this chunk, the probabilities of the tile's earlier ones, sums and results
+                        // move the maximum: scores of this chunk, the probabilities of the half's first one, sums and results
                         const bool first = limit == kNotStarted;
                         const float over = first ? best : best - kProbabilityUp;   // above the old maximum
                         float shift = 0.0f;
@@ -540,18 +553,23 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[i] = make_float2(z[i].x - shift, z[i].y - shift);
                         TmemStoreWait();
-                        for (int b = 0; b < c; ++b) {
+                        if ((c & 1) != 0) {
                             uint32_t w[16];
-                            umma::TmemLoad16(s_tmem + b * 16, w);
+                            umma::TmemLoad16(p_tmem, w);
                             umma::TmemLoadWait();
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
                                 const float2 v = HalfPair<FTH_B200_FP16>(w[i]);
                                 w[i] = PackHalf(v.x * alpha, v.y * alpha);
                             }
-                            TmemStore16(s_tmem + b * 16, w);
+                            TmemStore16(p_tmem, w);
                         }
-                        if (step > 0) ScaleResults<D>(o_tmem, alpha);
+                        if (step > 0 || h > 0) {   // after the products of the half before
+                            wait(&o_done[g][h ^ 1], (h == 0 ? used - 1 : used) & 1u, 7);
+                            __syncwarp();
+                            umma::FenceAfterThreadSync();
+                            ScaleResults<D>(o_tmem, alpha);
+                        }
                         TmemStoreWait();
                     }
                     uint32_t packed[16];
@@ -562,15 +580,17 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                         packed[i] = PackHalf(prob.x, prob.y);
                     }
                     __syncwarp();
-                    TmemStore16(s_tmem + c * 16, packed);
+                    TmemStore16(p_tmem + (c & 1) * 16, packed);
+                    if ((c & 1) != 0) {
+                        TmemStoreWait();
+                        umma::FenceBeforeThreadSync();
+                        MbarArrive(&p_full[g][h]);
+                    }
                 }
-                TmemStoreWait();
-                umma::FenceBeforeThreadSync();
-                MbarArrive(&p_full[g]);
             }
 
             // ---- the unit's results
-            if (active) wait(&o_done[g], (used - 1) & 1u, 7);
+            if (active) wait(&o_done[g][1], (used - 1) & 1u, 7);
             __syncwarp();
             umma::FenceAfterThreadSync();
             const float total = mass.x + mass.y;
@@ -599,11 +619,19 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]) * down;
                 if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        float eight[8];
+                    for (int i = 0; i < 16; ++i) v[i] = total == 0.0f ? 0.0f : v[i] * scale;
+                    if (p.out_vec) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) eight[j] = total == 0.0f ? 0.0f : v[i + j] * scale;
-                        rowops::WriteEight<DTYPE>(out, c * 16 + i, p.out_vec != 0, eight);
+                        for (int i = 0; i < 16; i += 8)
+                            *reinterpret_cast<uint4*>(out + c * 16 + i) = make_uint4(PackTo<DTYPE>(v[i], v[i + 1]), PackTo<DTYPE>(v[i + 2], v[i + 3]),
+                                                                                     PackTo<DTYPE>(v[i + 4], v[i + 5]), PackTo<DTYPE>(v[i + 6], v[i + 7]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const uint32_t two = PackTo<DTYPE>(v[i], v[i + 1]);
+                            out[c * 16 + i] = static_cast<uint16_t>(two);
+                            out[c * 16 + i + 1] = static_cast<uint16_t>(two >> 16);
+                        }
                     }
                 } else {
 #pragma unroll
@@ -640,7 +668,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             if (!u.more) break;
         }
         }
-    } else if (warp < kIssueWarp) {
+    } else if (warp < kParamWarp) {
         if (busy) {
         // ================================================ unpacking ==================================================
         // K: this thread's 16-byte pieces, 32 elements of a token each: neighbouring lanes take the halves of 64 bytes of four
@@ -845,87 +873,92 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             if (lane == 0) Advance<kUnit>(p, share_end, &places[kParamPlace]);
             __syncwarp();
         } while (u.more);
-        } else if (busy && warp == kIssueWarp) {
+        } else if (busy) {
         // ================================================ products ===================================================
         // The whole warp runs the loops, so that descriptors are computed once for the warp and not gathered from a lane
         // (82 .. 93 cycles per product when one lane did); one lane issues.
-        const Place& u = places[kIssuePlace];
-        const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
-        const uint32_t q_addr = SmemAddr(smem), k_addr = q_addr + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
-        const uint32_t d_tmem = __shfl_sync(0xffffffffu, tmem, 0);
-        uint32_t tile_count = 0, unit_count = 0, used[G] = {};   // tiles of tokens; tiles of each tile of rows
+        const int g = __shfl_sync(0xffffffffu, warp - kIssueWarp, 0);   // tile of rows
+        Place* const place = &places[kIssuePlace + g];
+        const uint32_t s_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, kTokens / 2), o_desc = umma::InstrDesc(1, 0, 0, false, false, kRows, D);
+        const uint32_t q_addr = SmemAddr(smem) + g * T::kOperandBytes, k_addr = SmemAddr(smem) + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
+        const uint32_t s_tmem = __shfl_sync(0xffffffffu, tmem, 0) + g * 256, o_tmem = s_tmem + 128;
+        const uint64_t qd = umma::SmemDesc(q_addr, 0, 1024);
+        uint32_t tile_count = 0, unit_count = 0, used = 0;   // tiles of tokens; those that this tile of rows took part in
         const auto wait_all = [&](uint64_t* bar, uint32_t parity, int detail) {
             if (!failed && !WaitFor(bar, parity, p.status, 16 + detail)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
         };
-        const auto commit = [&](uint64_t* bar) {
-            if (ElectOne()) umma::Commit(bar);
-        };
-        const auto scores = [&](int g, uint32_t tile) {   // S of rows g against the tile
-            // S is written where the last tile's P was read
-            if (used[g] > 0) wait_all(&o_done[g], (used[g] - 1) & 1u, 8);
+        // S against half a tile.  It is written where an earlier tile's P was read, whose products are done.
+        const auto scores = [&](int h, uint32_t tile) {
             umma::FenceAfterThreadSync();
             if (failed) return;
-            const uint64_t qd = umma::SmemDesc(q_addr + g * T::kOperandBytes, 0, 1024), kd = umma::SmemDesc(k_addr + (tile % S) * T::kOperandBytes, 0, 1024);
+            const uint64_t kd = umma::SmemDesc(k_addr + (tile % S) * T::kOperandBytes + h * (64 * 128), 0, 1024);
             if (ElectOne()) {
 #pragma unroll
                 for (int i = 0; i < T::kBlocks64 * 4; ++i) {   // 32 bytes on, then the next piece
                     const uint64_t at = (i >> 2) * (T::kPieceBytes >> 4) + (i & 3) * 2;
-                    MmaShared(d_tmem + g * 256, qd + at, kd + at, s_desc, i > 0);
+                    MmaShared(s_tmem + h * 64, qd + at, kd + at, s_desc, i > 0);
                 }
-                umma::Commit(&s_full[g]);
+                umma::Commit(&s_full[g][h]);
+                if (h == 1) umma::Commit(&k_empty[tile % S]);
             }
             __syncwarp();
         };
-        const auto values = [&](int g, uint32_t tile, bool first) {
-            wait_all(&p_full[g], used[g] & 1u, 4);
+        const auto values = [&](int h, uint32_t tile, bool first) {
+            wait_all(&p_full[g][h], used & 1u, 4);
             umma::FenceAfterThreadSync();
             if (failed) return;
-            const uint64_t vd = umma::SmemDesc(v_addr + (tile % S) * T::kOperandBytes, 0, 1024);
+            const uint64_t vd = umma::SmemDesc(v_addr + (tile % S) * T::kOperandBytes + h * (D * 128), 0, 1024);
             if (ElectOne()) {
 #pragma unroll
-                for (int i = 0; i < kTokens / 16; ++i)
-                    MmaTensor(d_tmem + g * 256 + 128, d_tmem + g * 256 + i * 8, vd + (i >> 2) * (D * 128 >> 4) + (i & 3) * 2, o_desc, !first || i > 0);
-                umma::Commit(&o_done[g]);
+                for (int i = 0; i < 4; ++i) MmaTensor(o_tmem, s_tmem + h * 64 + i * 8, vd + i * 2, o_desc, !first || i > 0);
+                umma::Commit(&o_done[g][h]);
+                if (h == 1) {
+                    umma::Commit(&v_empty[tile % S]);
+                    umma::Commit(&tile_done[tile % P]);
+                }
             }
             __syncwarp();
-            ++used[g];
         };
         bool more_units = true;
         do {
-            const int steps = __shfl_sync(0xffffffffu, u.steps, 0);
-            const int active = __shfl_sync(0xffffffffu, u.req.rows - u.row > kRows ? G : 1, 0);   // tiles of rows that have any
-            wait_all(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+            const int steps = __shfl_sync(0xffffffffu, place->steps, 0);
+            const bool active = g == 0 || __shfl_sync(0xffffffffu, place->req.rows - place->row, 0) > kRows;   // has rows
+            wait_all(&q_full[g], unit_count & 1u, 2);
+            if (active) {
+                wait_all(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+                if (used > 0) wait_all(&o_done[g][1], (used - 1) & 1u, 8);   // and with it the other half's
+                scores(0, tile_count);
+                scores(1, tile_count);
+                for (int step = 0; step < steps && !failed; ++step, ++tile_count, ++used) {
+                    const uint32_t next = tile_count + 1;
+                    wait_all(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                wait_all(&q_full[g], unit_count & 1u, 2);   // of a tile without rows too: its phases go on
-                if (g < active) scores(g, tile_count);
-            }
-            commit(&k_empty[tile_count % S]);
-            for (int step = 0; step < steps && !failed; ++step, ++tile_count) {
-                const bool more = step + 1 < steps;
-                const uint32_t next = tile_count + 1;
-                wait_all(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    if (g >= active) break;
-                    values(g, tile_count, step == 0);
-                    if (g + 1 == active) {
-                        commit(&v_empty[tile_count % S]);
-                        commit(&tile_done[tile_count % P]);
+                    for (int h = 0; h < 2; ++h) {
+                        values(h, tile_count, step == 0 && h == 0);
+                        if (step + 1 < steps) {
+                            if (h == 0) wait_all(&k_full[next % S], (next / S) & 1u, 3);
+                            wait_all(&o_done[g][h], used & 1u, 8);
+                            scores(h, next);
+                        }
                     }
-                    if (more) {
-                        if (g == 0) wait_all(&k_full[next % S], (next / S) & 1u, 3);
-                        scores(g, next);
-                        if (g + 1 == active) commit(&k_empty[next % S]);
+                }
+            } else {
+                for (int step = 0; step < steps && !failed; ++step, ++tile_count) {
+                    wait_all(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
+                    if (lane == 0) MbarArrive(&k_empty[tile_count % S]);
+                    wait_all(&v_full[tile_count % S], (tile_count / S) & 1u, 5);
+                    if (lane == 0) {
+                        MbarArrive(&v_empty[tile_count % S]);
+                        MbarArrive(&tile_done[tile_count % P]);
                     }
                 }
             }
             ++unit_count;
             __syncwarp();
-            if (lane == 0) Advance<kUnit>(p, share_end, &places[kIssuePlace]);
+            if (lane == 0) Advance<kUnit>(p, share_end, place);
             __syncwarp();
-            more_units = __shfl_sync(0xffffffffu, u.more, 0) != 0;
+            more_units = __shfl_sync(0xffffffffu, place->more, 0) != 0;
         } while (!failed && more_units);
         }
     }
