@@ -44,6 +44,7 @@ constexpr int kRows = 128;          // query rows of a tile
 constexpr int kTokens = 128;        // tokens of a tile
 constexpr int kSite = kSiteAttentionWait;
 constexpr int kNoExponent = 1000;
+constexpr int kUnitCost = 4, kLongShare = 64;
 constexpr float kProbabilityUp = 7.0f;  // probabilities are kept times 2^7: up to 2^15 with a lagging maximum, FP16's normal range down to 2^-21
 
 template <int D>
@@ -164,7 +165,7 @@ struct Place {
     int low, high;              // tokens that some row of the unit sees
     int more;                   // a unit, not the end of the share
     int64_t into;               // tiles of the unit that other blocks take
-    int64_t at;                 // in the flat list
+    int64_t at;                 // in the flat list: of the first of this block's tiles
     Request req;
 };
 template <int UNIT>
@@ -177,16 +178,15 @@ __device__ __forceinline__ void Settle(const AttentionParams& p, int64_t share_e
     Visible(p, u.req, QueryOf(p, (u.row + UNIT < u.req.rows ? u.row + UNIT : u.req.rows) - 1), &unused, &u.high);
     u.more = 1;
 }
-// By one thread of the group.
+// To the next unit.
 template <int UNIT>
-__device__ __forceinline__ void Advance(const AttentionParams& p, int64_t share_end, Place* place) {
-    Place u = *place;
-    u.at += u.steps;
+__device__ __forceinline__ void Advance(const AttentionParams& p, int64_t share_end, int cost, Place& u) {
+    u.at += u.tile_last - u.tile_first - u.into + cost;
+    u.into = 0;
     if (u.at >= share_end) {
-        place->more = 0;
+        u.more = 0;
         return;
     }
-    u.into = 0;
     u.row += UNIT;
     if (u.row >= u.req.rows) {
         u.row = 0;
@@ -200,6 +200,12 @@ __device__ __forceinline__ void Advance(const AttentionParams& p, int64_t share_
     }
     UnitTiles<kTokens>(p, u.req, u.row, UNIT, &u.tile_first, &u.tile_last);
     Settle<UNIT>(p, share_end, u);
+}
+// By one thread of the group.
+template <int UNIT>
+__device__ __forceinline__ void Advance(const AttentionParams& p, int64_t share_end, int cost, Place* place) {
+    Place u = *place;
+    Advance<UNIT>(p, share_end, cost, u);
     *place = u;
 }
 
@@ -239,8 +245,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(8) uint64_t q_full[G], s_full[G][2], p_full[G][2], o_done[G][2], k_full[S], k_empty[S], v_full[S], v_empty[S], params_full[P], tile_done[P], back_full;
-    __shared__ int64_t unit_work[kThreads];
-    __shared__ int64_t work_total;
+    __shared__ int64_t unit_work[kThreads];   // of a request, per kv head: tiles of its units
+    __shared__ int unit_count_of[kThreads];   // and units
+    __shared__ int64_t work_total, units_total;
     constexpr int kUnpackPlace = G, kParamPlace = G + 1, kIssuePlace = G + 2, kPlaces = 2 * G + 2;
     __shared__ Place places[kPlaces];      // one per tile of rows (softmax), unpacking, parameters, one per tile of rows (products)
     // of a tile
@@ -285,8 +292,18 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
 
     // ---- this block's share ----------------------------------------------------------------------------------------------
     // A warp takes a request at a time; thread 0 adds.  Few requests have many rows.
-    if (threadIdx.x == 0) work_total = 0;
+    if (threadIdx.x == 0) work_total = units_total = 0;
     __syncthreads();
+    const auto count_tiles = [&](int base, int count) {
+        for (int i = warp; i < count; i += kThreads / 32) {
+            const Request r = LoadRequest(p, base + i);
+            const int64_t sum = RequestTiles<kUnit>(p, r);
+            if (lane == 0) {
+                unit_work[i] = sum;
+                unit_count_of[i] = (r.rows + kUnit - 1) / kUnit;
+            }
+        }
+    };
     for (int base = 0; base < p.requests; base += kThreads) {
         const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
         if (p.few_units) {
@@ -299,27 +316,36 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     sum += b - a;
                 }
                 unit_work[threadIdx.x] = sum;
+                unit_count_of[threadIdx.x] = (r.rows + kUnit - 1) / kUnit;
             }
         } else {
-            for (int i = warp; i < count; i += kThreads / 32) {
-                const int64_t sum = RequestTiles<kUnit>(p, LoadRequest(p, base + i));
-                if (lane == 0) unit_work[i] = sum;
-            }
+            count_tiles(base, count);
         }
         __syncthreads();
         if (warp == 0) {
-            int64_t sum = 0;
-            for (int i = lane; i < count; i += 32) sum += unit_work[i];
+            int64_t sum = 0, units = 0;
+            for (int i = lane; i < count; i += 32) {
+                sum += unit_work[i];
+                units += unit_count_of[i];
+            }
             sum = WarpSum(sum);
-            if (lane == 0) work_total += sum * p.kv_heads;
+            units = WarpSum(units);
+            if (lane == 0) {
+                work_total += sum * p.kv_heads;
+                units_total += units * p.kv_heads;
+            }
         }
         __syncthreads();
     }
-    const int64_t work = work_total;
+    // Starting and ending a unit takes about as long as kUnitCost tiles (25 thousand cycles): with long shares it is counted as
+    // such, behind the unit's tiles, so that shares of many short units are not the last to end (three prompts of 4000 rows over
+    // 8100 tokens: 1059 us without, 1008, 998 and 1006 us with 2, 4 and 8).  Short shares are rather cut evenly.
+    const int cost = work_total >= kLongShare * gridDim.x ? kUnitCost : 0;
+    const int64_t work = work_total + cost * units_total;
     const int64_t per = work > 0 ? Divide(work + gridDim.x - 1, gridDim.x) : 1;
     const int64_t share_begin = blockIdx.x * per;
     const int64_t share_end = share_begin + per < work ? share_begin + per : work;
-    const bool busy = share_begin < share_end;
+    bool busy = share_begin < share_end;
     if (busy) {
         // the request, then the head, then the rows that share_begin falls into
         int64_t passed = 0;
@@ -327,16 +353,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
             if (p.requests > kThreads) {
                 __syncthreads();
-                for (int i = warp; i < count; i += kThreads / 32) {
-                    const int64_t sum = RequestTiles<kUnit>(p, LoadRequest(p, base + i));
-                    if (lane == 0) unit_work[i] = sum;
-                }
+                count_tiles(base, count);
                 __syncthreads();
             }
             bool found = false;
             if (warp == 0) {
                 for (int i = 0; i < count && !found; i += 32) {
-                    int64_t mine = i + lane < count ? unit_work[i + lane] * p.kv_heads : 0, sum = mine;
+                    int64_t mine = i + lane < count ? (unit_work[i + lane] + cost * unit_count_of[i + lane]) * p.kv_heads : 0, sum = mine;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const int64_t n = __shfl_up_sync(0xffffffffu, sum, o);
@@ -349,7 +372,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                         found = true;
                         const int src = __ffs(who) - 1;
                         int64_t off = share_begin - __shfl_sync(0xffffffffu, before, src);
-                        const int64_t per_head = unit_work[i + src];
+                        const int64_t per_head = unit_work[i + src] + cost * unit_count_of[i + src];
                         Place u;
                         u.b = base + i + src;
                         u.req = LoadRequest(p, u.b);
@@ -360,7 +383,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                             const int my_row = row + lane * kUnit;
                             int a = 0, c = 0;
                             if (my_row < u.req.rows) UnitTiles<kTokens>(p, u.req, my_row, kUnit, &a, &c);
-                            int64_t upto = c - a;
+                            const int64_t own = c - a + (c > a ? cost : 0);
+                            int64_t upto = own;
 #pragma unroll
                             for (int o = 1; o < 32; o <<= 1) {
                                 const int64_t n = __shfl_up_sync(0xffffffffu, upto, o);
@@ -372,9 +396,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                                     u.row = my_row;
                                     u.tile_first = a;
                                     u.tile_last = c;
-                                    u.into = off - (upto - (c - a));
+                                    u.into = off - (upto - own);
                                     u.at = share_begin;
-                                    Settle<kUnit>(p, share_end, u);
+                                    u.more = 1;
+                                    if (u.into < c - a) Settle<kUnit>(p, share_end, u);
+                                    else Advance<kUnit>(p, share_end, cost, u);   // the share begins behind its last tile
                                     for (int i = 0; i < kPlaces; ++i) places[i] = u;
                                 }
                                 break;
@@ -388,6 +414,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             if (__syncthreads_or(found ? 1 : 0)) break;
         }
         __syncthreads();
+        busy = places[0].more != 0;
+        __syncthreads();   // before a group moves on
     }
 
     float* const params = reinterpret_cast<float*>(smem + T::kParams);
@@ -663,7 +691,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             ++unit_count;
             umma::FenceBeforeThreadSync();
             WarpsSync(1 + g, 128);
-            if (r == 0) Advance<kUnit>(p, share_end, &places[g]);
+            if (r == 0) Advance<kUnit>(p, share_end, cost, &places[g]);
             WarpsSync(1 + g, 128);
             if (!u.more) break;
         }
@@ -776,7 +804,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 if (step + 1 < steps) load_values(next);
             }
             WarpsSync(4, 128);
-            if (tid == 0) Advance<kUnit>(p, share_end, &places[kUnpackPlace]);
+            if (tid == 0) Advance<kUnit>(p, share_end, cost, &places[kUnpackPlace]);
             WarpsSync(4, 128);
         } while (u.more);
         }
@@ -870,7 +898,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             }
             ++unit_count;
             __syncwarp();
-            if (lane == 0) Advance<kUnit>(p, share_end, &places[kParamPlace]);
+            if (lane == 0) Advance<kUnit>(p, share_end, cost, &places[kParamPlace]);
             __syncwarp();
         } while (u.more);
         } else if (busy) {
@@ -956,7 +984,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             }
             ++unit_count;
             __syncwarp();
-            if (lane == 0) Advance<kUnit>(p, share_end, place);
+            if (lane == 0) Advance<kUnit>(p, share_end, cost, place);
             __syncwarp();
             more_units = __shfl_sync(0xffffffffu, place->more, 0) != 0;
         } while (!failed && more_units);
