@@ -82,6 +82,51 @@ __device__ __forceinline__ int64_t HeadBase(const Cache& c, int block, int head)
 __device__ __forceinline__ float ParamScale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float ParamMin(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// ---- arithmetic ----------------------------------------------------------------------------------------------------------
+// Two FP32 operations per instruction.
+__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 Add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ uint32_t PackHalf(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int DTYPE>
+__device__ __forceinline__ uint32_t PackTo(float low, float high) {
+    if constexpr (DTYPE == FTH_B200_FP16) return PackHalf(low, high);
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(high), "f"(low));
+    return d;
+}
+template <int DTYPE>
+__device__ __forceinline__ float2 HalfPair(uint32_t x) {
+    if constexpr (DTYPE == FTH_B200_BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+__device__ __forceinline__ float Max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // ---- rotary positions --------------------------------------------------------------------------------------------------
 struct Rope {
     int half_layout, head_dim, rotary_dim, q_heads, k_heads;
@@ -152,13 +197,6 @@ __device__ __forceinline__ void RopeEight(const Rope& r, const void* x, int64_t 
             v[i + 1] = y.y;
         }
     }
-}
-// The value a row holds after it has been stored as DTYPE.
-template <int DTYPE>
-__device__ __forceinline__ float Rounded(float v) {
-    if constexpr (DTYPE == FTH_B200_FP32) return v;
-    else if constexpr (DTYPE == FTH_B200_BF16) return DecodeBf16(EncodeBf16Cast(v));
-    else return __half2float(__float2half_rn(v));
 }
 
 }  // namespace kv4

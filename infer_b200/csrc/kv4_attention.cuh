@@ -117,44 +117,6 @@ __device__ __forceinline__ float Reciprocal(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two FP32 operations per instruction.
-__device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 Add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ uint32_t PackHalf(float low, float high) {
-    const __half2 h = __floats2half2_rn(low, high);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <int DTYPE>
-__device__ __forceinline__ uint32_t PackTo(float low, float high) {
-    if constexpr (DTYPE == FTH_B200_FP16) return PackHalf(low, high);
-    uint32_t d;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(high), "f"(low));
-    return d;
-}
-template <int DTYPE>
-__device__ __forceinline__ float2 HalfPair(uint32_t x) {
-    if constexpr (DTYPE == FTH_B200_BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-    else return __half22float2(*reinterpret_cast<const __half2*>(&x));
-}
 __device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // Power of two that brings the largest query element to [2^14, 2^15); 24 - e stays an FP32 exponent.

@@ -113,11 +113,6 @@ __device__ __forceinline__ void WarpsSync(int barrier, int threads) {
     __syncwarp();
     asm volatile("barrier.cta.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 }
-__device__ __forceinline__ float Max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 
 // The rows' results so far times `factor`, by the warp that owns them.
 template <int D>
