@@ -20,7 +20,7 @@
 // a rounding of that token's share of (v - out), not by one of its code, which is far larger than the value when minimum
 // and code cancel.  The lse is taken from the probabilities before the rounding.
 //
-// Work is the flat list of (request, kv head, block of 8 or 16 query rows, tile of tokens); every block of threads
+// Work is the flat list of (request, kv head, tile of tokens; all of a head's query rows, 8 or 16, together); every block of threads
 // takes an equal, contiguous share, found from the lengths on the device.  A unit cut by shares leaves partial results
 // (maximum, sum, weighted values, FP32) in the workspace; the part that arrives last joins them in order.
 //
@@ -72,38 +72,14 @@ __device__ __forceinline__ void ComputeSync() {
     asm volatile("barrier.cta.sync 1, %0;" ::"n"(kCompute) : "memory");   // not the aligned form: lanes may come one after another
 }
 
-// Sum of v over the block, and the sum over the threads before this one.
-__device__ __forceinline__ int64_t ScanWork(int64_t v, int64_t* shared, int64_t* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t n = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += n;
-    }
-    __syncthreads();
-    if (lane == 31) shared[warp] = s;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) before += shared[w];
-        all += shared[w];
-    }
-    *total = all;
-    return before + s - v;
-}
-
-// Tiles of all units of one kv head of a request.
+// Token tiles of request b's unit (one per kv head: all its rows), 0 without rows.
 template <int TILE>
-__device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, const Request& r, int unit_rows) {
-    int64_t sum = 0;
-    for (int row = 0; row < r.rows; row += unit_rows) {
-        int a, b;
-        UnitTiles<TILE>(p, r, row, unit_rows, &a, &b);
-        sum += b - a;
-    }
-    return sum;
+__device__ __forceinline__ int RequestTiles(const AttentionParams& p, int b, int unit_rows) {
+    const Request r = LoadRequest(p, b);
+    if (r.rows == 0) return 0;
+    int first, last;
+    UnitTiles<TILE>(p, r, 0, unit_rows, &first, &last);
+    return last - first;
 }
 
 // A lane's packed words of one token row (or row of a pair of tokens): four words every 64 (K) or 128 (V) bytes.
@@ -132,10 +108,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     constexpr bool QS = kQueriesInShared<D, NT>;
     constexpr int I = 2;   // sixteens of tokens worked on together
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scan[kThreads / 32];
-    __shared__ Request start_req;
-    __shared__ int start_request;
-    __shared__ int64_t start_offset, start_per_head;
     __shared__ int join_last;
     __shared__ __align__(8) uint64_t full[S], empty[S];
     __shared__ uint32_t stage_present[S];   // a bit for every 16 tokens of the stage that are there
@@ -148,65 +120,61 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         }
         FenceBarrierInit();
     }
+    __syncthreads();
     WaitForPrevious();
 
-    // ---- this block's share of the tiles --------------------------------------------------------------------------------
-    int64_t work = 0, mine = 0, before = 0, per_head = 0;
-    Request req;
-    for (int base = 0; base < p.requests; base += kThreads) {
-        const int b = base + threadIdx.x;
-        mine = 0;
-        if (b < p.requests) {
-            req = LoadRequest(p, b);
-            per_head = RequestTiles<T::kTile>(p, req, R);
-            mine = per_head * p.kv_heads;
-        }
-        int64_t total;
-        before = ScanWork(mine, scan, &total);
-        work += total;
-    }
-    int64_t per = (work + gridDim.x - 1) / gridDim.x;
+    // ---- this block's share of the tiles: every warp finds it by itself, a lane per request --------------------------------
+    int64_t work = 0;
+#pragma unroll 4
+    for (int i = lane; i < p.requests; i += 32) work += RequestTiles<T::kTile>(p, i, R);
+    work = WarpSum(work) * p.kv_heads;
+    int64_t per = Divide(work + gridDim.x - 1, gridDim.x);
     if (per < kMinShare) per = kMinShare;
+    // With fewer units than blocks of threads a share ends with its unit, if there are blocks enough: units up to `per` tiles
+    // are not cut then (one request of 333 tokens, 2 kv heads: 13.9 us when the second unit was).  In the list such a unit
+    // is as long as its shares.
+    bool apart = static_cast<int64_t>(p.requests) * p.kv_heads <= gridDim.x;
+    if (apart) {
+        int64_t shares = 0;
+        for (int i = lane; i < p.requests; i += 32) shares += Divide(RequestTiles<T::kTile>(p, i, R) + per - 1, per);
+        shares = WarpSum(shares) * p.kv_heads;
+        apart = shares <= gridDim.x;
+        if (apart) work = shares * per;
+    }
     const int64_t share_begin = blockIdx.x * per;
     const int64_t share_end = share_begin + per < work ? share_begin + per : work;
     if (share_begin >= share_end) return;
-    int64_t passed = 0;
-    for (int base = 0; base < p.requests; base += kThreads) {
-        int64_t total = work;
-        if (p.requests > kThreads) {
-            const int b = base + threadIdx.x;
-            mine = 0;
-            if (b < p.requests) {
-                req = LoadRequest(p, b);
-                per_head = RequestTiles<T::kTile>(p, req, R);
-                mine = per_head * p.kv_heads;
-            }
-            before = ScanWork(mine, scan, &total);
-        }
-        if (share_begin >= passed + before && share_begin < passed + before + mine) {
-            start_request = base + threadIdx.x;
-            start_offset = share_begin - passed - before;
-            start_req = req;
-            start_per_head = per_head;
-        }
-        passed += total;
-        if (passed > share_begin) break;
-    }
-    __syncthreads();
 
-    // ---- the first unit: request, head, rows, tiles ---------------------------------------------------------------------
-    int b = start_request;
-    req = start_req;
-    int head = static_cast<int>(start_offset / start_per_head);
-    int row = 0;
-    int64_t into = start_offset - head * start_per_head;  // tiles of the unit that other blocks take
-    int tile_first, tile_last;
-    for (;;) {
-        UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
-        if (into < tile_last - tile_first) break;
-        into -= tile_last - tile_first;
-        row += R;
+    // ---- the first unit: request, head, tiles -----------------------------------------------------------------------------
+    int b = 0;
+    int64_t offset_in = 0, per_head = 1;   // of share_begin in the request; the request's length in the list per head
+    int64_t passed = 0;
+    for (int base = 0; base < p.requests; base += 32) {
+        int64_t length = base + lane < p.requests ? RequestTiles<T::kTile>(p, base + lane, R) : 0;
+        if (apart) length = Divide(length + per - 1, per) * per;
+        const int64_t mine = length * p.kv_heads;
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t n = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += n;
+        }
+        const uint32_t who = __ballot_sync(0xffffffffu, share_begin < passed + upto);
+        if (who != 0) {
+            const int src = __ffs(who) - 1;
+            b = base + src;
+            offset_in = share_begin - passed - __shfl_sync(0xffffffffu, upto - mine, src);
+            per_head = __shfl_sync(0xffffffffu, length, src);
+            break;
+        }
+        passed += __shfl_sync(0xffffffffu, upto, 31);
     }
+    Request req = LoadRequest(p, b);
+    int head = static_cast<int>(Divide(offset_in, per_head));
+    constexpr int row = 0;   // a unit holds all rows
+    int64_t into = offset_in - head * per_head;  // tiles of the unit that other blocks take
+    int tile_first, tile_last;
+    UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
     int64_t at = share_begin;
     int t0, steps, first_low, last_high;   // of this block's part of the unit
     const auto place = [&] {
@@ -219,18 +187,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     };
     const auto next_unit = [&] {   // false: the share is done
         at += steps;
-        if (at >= share_end) return false;
+        if (apart || at >= share_end) return false;
         into = 0;
-        row += R;
-        if (row >= req.rows) {
-            row = 0;
-            if (++head == p.kv_heads) {
-                head = 0;
-                do {
-                    ++b;
-                    req = LoadRequest(p, b);
-                } while (req.rows == 0);
-            }
+        if (++head == p.kv_heads) {
+            head = 0;
+            do {
+                ++b;
+                req = LoadRequest(p, b);
+            } while (req.rows == 0);
         }
         UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
         place();
@@ -675,8 +639,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         }
         ComputeSync();
         // blocks of threads that hold the first and the last part of the unit
-        const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : unit_begin / per;
-        const int64_t part_last = unit_end <= share_end ? blockIdx.x : (unit_end - 1) / per;
+        const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : Divide(unit_begin, per);
+        const int64_t part_last = unit_end <= share_end ? blockIdx.x : Divide(unit_end - 1, per);
         const bool whole = part_first == part_last;
         const int valid_rows = req.rows - row < R ? req.rows - row : R;
         const int64_t slot_floats = static_cast<int64_t>(R) * kRow<D>;

@@ -90,6 +90,18 @@ __device__ __forceinline__ void UnitTiles(const AttentionParams& p, const Reques
     if (*last <= *first) *last = *first + 1;
 }
 
+// a / b of numbers that are not negative; most fit 32 bits, whose division is much shorter.
+__device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
+    return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// Sum of v over the warp.
+__device__ __forceinline__ int64_t WarpSum(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 // ---- arithmetic -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void MmaF16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

@@ -129,16 +129,6 @@ __device__ __forceinline__ void ScaleResults(uint32_t o_tmem, float factor) {
     }
     TmemStoreWait();
 }
-__device__ __forceinline__ int64_t Divide(int64_t a, int64_t b) {
-    return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
-}
-
-// Sum of v over the warp.
-__device__ __forceinline__ int64_t WarpSum(int64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
 // Token tiles of all units of one kv head of a request, by a whole warp.
 template <int UNIT>
 __device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, const Request& r) {
