@@ -551,9 +551,13 @@ int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* desc, fth_b200_stream_t 
  * q head h reads kv head h / (q_heads / kv_heads).
  *   out = softmax(scale * q . K) . V,  lse (optional, FP32 [tokens, q_heads]) = ln(sum(exp(scale * q . K)))
  * A row that sees nothing gets zeros and lse = -infinity.  Rows behind query_start[requests] are left as they were.
- * Scores, softmax statistics and sums are FP32.  q enters exactly (FP16 with a power of two per row; |q| < 2^100), codes
- * are exact; a probability times the scale of its value is rounded to FP16 (11 bits, down to 2^-20 of the largest scale
- * among the values seen).
+ * Scores, softmax statistics and sums are FP32.  With up to 16 rows to a kv head (max_query * q_heads / kv_heads) codes enter
+ * exactly and the product of a probability and the scale of its value is rounded to FP16 (11 bits, down to 2^-20 of the
+ * largest scale among the values seen).  With more rows probabilities and values are rounded to FP16 one by one, and with BF16
+ * rows the keys too (11 bits, down to 2^-28 of the largest among 128 tokens; values: among those before them as well).
+ * q enters as FP16 times one power of two for the rows that are worked on together, which are of one request and kv head:
+ * exactly, down to 2^-28 of their largest finite element (|q| < 2^100, |v| < 2^100).
+ * A NaN in q makes its own row NaN, a NaN in a key or value (or in its scale or minimum) the rows that see the token.
  * A block number outside the cache hides its tokens and is reported through fth_b200_device_status (site 42).
  * max_query bounds the rows of a request (host-known; rows beyond it are not computed), max_blocks * block_size the tokens.
  * The result does not depend on what else is in the batch only up to FP32 summation order; it is the same from run to run.

@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 v = HalfPair<DTYPE>(raw[n][w][i]);
-                        big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
+                        big = fmaxf(big, fmaxf(FiniteAbs(v.x), FiniteAbs(v.y)));
                         sum += v.x + v.y;
                     }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);

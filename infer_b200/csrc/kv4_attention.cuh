@@ -131,6 +131,8 @@ __device__ __forceinline__ float Reciprocal(float x) {
 }
 __device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
+// |x|, 0 for what is not finite: an infinity spoils its own row, and must not take the others' bits by the power of two.
+__device__ __forceinline__ float FiniteAbs(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
 // Power of two that brings the largest query element to [2^14, 2^15); 24 - e stays an FP32 exponent.
 __device__ __forceinline__ int QueryExponent(float biggest) {
     if (biggest == 0.0f) return 0;

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
     __shared__ float4 about[P];            // power of two on the values; 1 / that on the keys; 1: all present, none spoiled
     __shared__ int64_t place_of[P][kTokens / 16];   // offset of the codes of sixteen tokens, -1: no block
     __shared__ __align__(16) __half value_scale[P][kTokens], value_min[P][kTokens], key_scale[P][kTokens], key_min[P][kTokens];
-    __shared__ float q_big[4 * G], unit_back;
+    __shared__ float q_big[2][4 * G], unit_back;
     __shared__ int join_last[G];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kUnpackWarp = T::kSoftmax / 32, kParamWarp = kUnpackWarp + 4, kIssueWarp = kParamWarp + 1;
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             const int query = valid ? QueryOf(p, row) : 0;
             const auto piece = [&](int of, int w) { return reinterpret_cast<uint4*>(q_smem + (w >> 3) * T::kPieceBytes + of * 128 + (((w & 7) ^ (of & 7)) << 4)); };
             const int64_t own = (u.req.first_row + static_cast<int64_t>(query)) * p.ldq + (static_cast<int64_t>(u.head) * p.group + (row - query * p.group)) * D;
-            {   // the 32 rows of a warp, neighbouring lanes neighbouring pieces of a row
+            if (active) {   // the 32 rows of a warp, neighbouring lanes neighbouring pieces of a row
                 constexpr int kLanes = D / 8 < 32 ? D / 8 : 32, kRowsAtOnce = 32 / kLanes;
                 const int w = lane % kLanes;
                 const auto copy = [&](int i, auto fetch) {
@@ -445,23 +445,24 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             }
             float big = 0.0f, qsum = 0.0f;
 #pragma unroll 2
-            for (int w = 0; w < D / 8; ++w) {
+            for (int w = 0; active && w < D / 8; ++w) {
                 const uint4 x = *piece(r, w);
                 const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 v = HalfPair<DTYPE>(raw[i]);
-                    big = Max3(big, fabsf(v.x), fabsf(v.y));
+                    big = Max3(big, FiniteAbs(v.x), FiniteAbs(v.y));
                     if constexpr (kKeyCodes) qsum += v.x + v.y;
                 }
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-            if (lane == 0) q_big[warp] = big;
+            float* const bigs = q_big[unit_count & 1u];   // one of the groups may be a unit ahead
+            if (lane == 0) bigs[warp] = big;
             // one power of two for the unit where it goes into the keys' parameters, else one for the tile of rows
             WarpsSync(kKeyCodes ? 3 : 1 + g, kKeyCodes ? T::kSoftmax : 128);
 #pragma unroll
-            for (int w = 0; w < (kKeyCodes ? 4 * G : 4); ++w) big = fmaxf(big, q_big[kKeyCodes ? w : 4 * g + w]);
+            for (int w = 0; w < (kKeyCodes ? 4 * G : 4); ++w) big = fmaxf(big, bigs[kKeyCodes ? w : 4 * g + w]);
             const int e = QueryExponent(big);
             const float up = PowerOfTwo(e), back = p.scale_log2 * PowerOfTwo((kKeyCodes ? 24 : 0) - e);
             if (kKeyCodes && threadIdx.x == 0) {
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             }
             qsum *= p.scale_log2;
 #pragma unroll 2
-            for (int w = 0; w < D / 8; ++w) {
+            for (int w = 0; active && w < D / 8; ++w) {
                 const uint4 x = *piece(r, w);
                 const uint32_t raw[4] = {x.x, x.y, x.z, x.w};
                 uint32_t f[4];
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 *piece(r, w) = make_uint4(f[0], f[1], f[2], f[3]);
             }
             FenceProxyAsync();
-            MbarArrive(&q_full[g]);
+            if (active) MbarArrive(&q_full[g]);
             int low = 0, high = 0;
             if (valid) Visible(p, u.req, query, &low, &high);
 
@@ -489,6 +490,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
             if (!active) tile_count += steps;   // no rows
             for (int step = 0; active && step < steps; ++step, ++tile_count, ++used) {
                 const uint32_t par = tile_count % P;
+                // The scores' barrier counts this tile of rows' own tiles.  The parameters' counts all tiles, of which it may have passed
+                // over many (units in which it has no rows): only with the scores there is it known to be at this one.
+                wait(&s_full[g][0], used & 1u, 6);
                 wait(&params_full[par], (tile_count / P) & 1u, 10);
                 const float4 tile = about[par];
                 const int token0 = first_token + step * kTokens;
@@ -509,7 +513,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     const uint32_t p_tmem = s_tmem + h * 64;   // the half's probabilities, over its scores
                     uint32_t s[32];
                     if ((c & 1) == 0) {
-                        wait(&s_full[g][h], used & 1u, 6);
+                        if (h != 0) wait(&s_full[g][h], used & 1u, 6);
                         __syncwarp();
                         umma::FenceAfterThreadSync();
                     }
@@ -896,7 +900,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         const uint32_t q_addr = SmemAddr(smem) + g * T::kOperandBytes, k_addr = SmemAddr(smem) + T::kKeys, v_addr = k_addr + S * T::kOperandBytes;
         const uint32_t s_tmem = __shfl_sync(0xffffffffu, tmem, 0) + g * 256, o_tmem = s_tmem + 128;
         const uint64_t qd = umma::SmemDesc(q_addr, 0, 1024);
-        uint32_t tile_count = 0, unit_count = 0, used = 0;   // tiles of tokens; those that this tile of rows took part in
+        uint32_t tile_count = 0, active_units = 0, used = 0;   // tiles of tokens; units and tiles that this tile of rows took part in
         const auto wait_all = [&](uint64_t* bar, uint32_t parity, int detail) {
             if (!failed && !WaitFor(bar, parity, p.status, 16 + detail)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
@@ -937,8 +941,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
         do {
             const int steps = __shfl_sync(0xffffffffu, place->steps, 0);
             const bool active = g == 0 || __shfl_sync(0xffffffffu, place->req.rows - place->row, 0) > kRows;   // has rows
-            wait_all(&q_full[g], unit_count & 1u, 2);
             if (active) {
+                wait_all(&q_full[g], active_units++ & 1u, 2);
                 wait_all(&k_full[tile_count % S], (tile_count / S) & 1u, 3);
                 if (used > 0) wait_all(&o_done[g][1], (used - 1) & 1u, 8);   // and with it the other half's
                 scores(0, tile_count);
@@ -967,7 +971,6 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     }
                 }
             }
-            ++unit_count;
             __syncwarp();
             if (lane == 0) Advance<kUnit>(p, share_end, cost, place);
             __syncwarp();

@@ -1,0 +1,207 @@
+"""GPU: the 4-bit cache at sizes and in states beyond tests/test_gpu_kv4.py, with its helpers, plain forms and limits: many
+requests, long shares of work, rows beyond max_query, numbers that are none in every place, many tokens stored at once."""
+import math
+
+import numpy as np
+import pytest
+
+import infer_b200 as B
+from tests import kv4_plain as P
+from tests.test_gpu_kv4 import KINDS, attend, dtype_of, half_step, key_rounding, same, special_vectors
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,hq,hk", [(1, 2, 2), (5, 4, 1)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_requests(cuda, new, hq, hk, dim):
+    """More requests than a block has threads, some of them empty or idle, in both kernels."""
+    rng = np.random.default_rng(dim + new)
+    lens = [int(n) for n in rng.integers(0, 150, 700)]
+    rows = [0 if rng.random() < 0.2 else int(rng.integers(1, new + 1)) for _ in lens]
+    attend(cuda, dtype="bf16", lens=lens, new=rows, hq=hq, hk=hk, dim=dim, bs=16, seed=new)
+
+
+@pytest.mark.parametrize("dtype,dim,hq,hk,window", [("bf16", 64, 8, 8, 0), ("fp16", 64, 8, 8, 0), ("bf16", 128, 6, 6, 9000), ("bf16", 256, 4, 4, 0)])
+def test_long_shares_of_many_rows(cuda, dtype, dim, hq, hk, window):
+    """Work enough that the cost of starting a unit moves the cuts; several requests, the last with few rows."""
+    attend(cuda, dtype=dtype, lens=[14000, 5000, 900], new=[4100, 2300, 3], hq=hq, hk=hk, dim=dim, bs=64, seed=dim, window=window, lse=False)
+
+
+@pytest.mark.parametrize("units", [1, 2, 3])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_units_of_every_length(cuda, units, dim):
+    """Batches small enough that shares end with their unit, around the lengths where one more share begins."""
+    for length in (1, 127, 128, 129, 255, 257, 511, 512, 513, 1024, 1025, 2049, 5000):
+        lens = [max(length - 300 * r, 1) for r in range(units)]
+        attend(cuda, dtype="bf16", lens=lens, new=[1] * units, hq=8, hk=2, dim=dim, bs=16, seed=length)
+
+
+@pytest.mark.parametrize("new,most", [([5, 2, 7], 3), ([90, 10, 40], 33)])
+def test_rows_beyond_max_query_are_not_computed(cuda, new, most):
+    """The first max_query rows of a request keep their positions; the rest is left as it was."""
+    torch = cuda
+    hq, hk, dim, bs, lens = 8, 2, 128, 16, [300, 50, 129]
+    r = attend(torch, dtype="bf16", lens=lens, new=new, hq=hq, hk=hk, dim=dim, bs=bs, seed=1)
+    d = r["desc"]
+    d.max_query = most
+    ws = B.kv4_attention_workspace(torch, d)
+    r["out"].fill_(7.0)
+    B.kv4_attention(d)
+    # a row of n stands at total - n + i: the first `most` of n rows are the last of total - (n - most) tokens
+    at = 0
+    for i, n in enumerate(new):
+        kept = min(n, most)
+        q = r["q"][at:at + kept].reshape(kept, hq, dim)
+        want, _, limit, _ = P.attention(torch, r["cache"], bs, r["table"][i:i + 1], q, [lens[i] - (n - kept)], [kept], hk, d.scale, True, 0,
+                                        key_rounding=key_rounding("bf16", most * hq // hk))
+        got = r["out"][at:at + kept].reshape(kept, hq, dim).double()
+        assert ((got - want).abs() <= limit + 2.0 ** -8 * want.abs() + 1e-30).all()
+        assert (r["out"][at + kept:at + n] == 7.0).all()
+        at += n
+    del ws
+    assert B.device_status() == 0
+
+
+def near(torch, a, b, dtype):
+    a, b = a.double(), b.double()
+    assert not a.isnan().any() and b.abs().max() < 5
+    assert ((a - b).abs() <= 2 * half_step(torch, dtype_of(torch, dtype)) * (b.abs() + 0.1) + 2 * 2 * 2.0 ** -12 * 10).all()
+
+
+@pytest.mark.parametrize("name,which", [("k_params", 0), ("k_params", 1), ("v_params", 0), ("v_params", 1)])
+@pytest.mark.parametrize("dtype,new", [("bf16", 1), ("bf16", 64), ("fp16", 64)])
+def test_scales_and_minima_that_are_no_numbers(cuda, name, which, dtype, new):
+    """The token's scale or minimum of keys or values: the rows that see it are NaN, the others (behind the mask or the window, of
+    other heads and requests) are what they were up to the roundings, which depend on the rows worked on together: each result is
+    within 2 * 2^-12 of |v| + |out| < 10 (a probability's rounding) and half a step of the exact one."""
+    torch = cuda
+
+    def spoil(cache, table, **_):
+        for token in (60, 97):
+            cache[name][int(table[0, token // 16]), 1, token % 16, which] = math.nan
+    args = dict(dtype=dtype, lens=[100, 200], new=[new, new], hq=4, hk=2, dim=128, bs=16, seed=5, lse=False)
+    for window in (0, 20):
+        clean = attend(torch, window=window, **args)
+        torch.cuda.synchronize()
+        keep = clean["out"].clone()
+        spoil(clean["cache"], clean["table"])
+        B.kv4_attention(clean["desc"])
+        rows = torch.arange(new, device="cuda") + 100 - new
+        sees = torch.zeros(new, dtype=torch.bool, device="cuda")
+        for token in (60, 97):
+            sees |= (rows >= token) & ((rows - token < window) if window else True)
+        got = clean["out"][:2 * new].view(-1, 4, 128)
+        assert got[:new][sees][:, 2:].isnan().all()
+        others = got.clone().view(torch.int16)
+        others[:new, 2:][sees] = 0
+        before = keep[:2 * new].view(-1, 4, 128).clone().view(torch.int16)
+        before[:new, 2:][sees] = 0
+        near(torch, others.view(keep.dtype), before.view(keep.dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("new", [2, 64])
+def test_an_infinity_in_one_row_leaves_the_others(cuda, dtype, new):
+    torch = cuda
+    r = attend(torch, dtype=dtype, lens=[300], new=[new], hq=4, hk=2, dim=128, bs=16, seed=4, lse=False)
+    before = r["out"].clone()
+    r["q"][new - 1, 7] = math.inf
+    B.kv4_attention(r["desc"])
+    got = r["out"].view(-1, 4, 128)
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[new - 1, 0] = False
+    keep[new:] = False
+    near(torch, got[keep], before.view(-1, 4, 128)[keep], dtype)
+    assert got[new - 1, 0].isnan().all() and (r["out"][new:] == 7.0).all()
+
+
+def test_two_graphs_share_a_workspace(cuda):
+    """Captured calls of both kernels on one workspace, replayed in any order, give the eager results."""
+    torch = cuda
+    few = attend(torch, dtype="bf16", lens=[5000, 90], new=[1, 1], hq=8, hk=2, dim=128, bs=16, seed=2)
+    many = attend(torch, dtype="bf16", lens=[5000, 90], new=[70, 30], hq=8, hk=2, dim=128, bs=16, seed=3)
+    ws = max((few["ws"], many["ws"]), key=lambda t: t.numel())
+    graphs = []
+    for r in (few, many):
+        r["desc"].workspace, r["desc"].workspace_bytes = ws.data_ptr(), ws.numel()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            B.kv4_attention(r["desc"])
+        graphs.append((g, r, r["out"].clone()))
+    for i in (0, 1, 1, 0, 0, 1):
+        g, r, want = graphs[i]
+        r["out"].fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want[-2:] = 7.0
+        assert torch.equal(r["out"], want)
+    assert B.device_status() == 0
+
+
+# ---- storing and reading back -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,tokens,heads,dim,bs", [("bf16", 5001, 8, 64, 16), ("fp16", 2601, 8, 128, 64), ("fp32", 2600, 4, 256, 256)])
+@pytest.mark.parametrize("order", ["row", "odd", "random", "holes"])
+def test_many_tokens_at_once(cuda, dtype, tokens, heads, dim, bs, order):
+    """Enough tokens that they are worked on in pairs: neighbours in the cache, neighbours across a block, strangers, gaps."""
+    torch = cuda
+    dt = dtype_of(torch, dtype)
+    blocks = P.blocks(tokens, bs) + 2
+    cache = P.new_cache(torch, blocks, heads, bs, dim, seed=1)
+    want = {n: t.clone() for n, t in cache.items()}
+    k, v = special_vectors(torch, tokens, heads, dim, dt, 2), special_vectors(torch, tokens, heads, dim, dt, 3)
+    k[100, 0, 3], v[101, heads - 1, 0] = math.nan, -math.inf
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    slots = torch.arange(tokens, device="cuda")
+    if order == "odd":
+        slots = slots + 1
+    elif order == "random":
+        slots = torch.randperm(blocks * bs, generator=gen, device="cuda")[:tokens]
+    elif order == "holes":
+        slots = torch.where(torch.rand(tokens, generator=gen, device="cuda") < 0.3, -1, slots)
+    slots = slots.to(torch.int32)
+    b = P.bind(B, cache, bs)
+    B.kv4_append(B.kv4_append_desc(cache=b, dtype=KINDS[dtype], tokens=tokens, k=k, v=v, slots=slots))
+    P.append(torch, want, bs, k, v, slots)
+    for n in cache:
+        same(cache[n], want[n])
+    kb, vb = (torch.full((tokens, heads, dim), 7.0, dtype=dt, device="cuda") for _ in range(2))
+    B.kv4_gather(B.kv4_gather_desc(cache=b, dtype=KINDS[dtype], tokens=tokens, slots=slots, k_out=kb, v_out=vb))
+    keep = slots >= 0
+    for got, (mean, size) in zip((kb, vb), P.read(torch, cache, bs, slots.clamp(min=0).long())):
+        mean, size, g = mean[keep], size[keep], got[keep].double()
+        nan = mean.isnan()
+        assert torch.equal(g.isnan(), nan)
+        limit = 2.0 ** -23 * size + half_step(torch, dt) * mean.abs() * (1 + 2.0 ** -8) + torch.finfo(dt).smallest_normal * half_step(torch, dt)
+        assert ((g - mean).abs() <= limit)[~nan].all()
+        assert (got[~keep] == 7.0).all()
+    assert B.device_status() == 0
+
+
+def test_ranges_at_the_end_of_the_numbers(cuda):
+    """Differences that round up past the largest FP32 number, spreads below the smallest scale, signed zeros."""
+    torch = cuda
+    big = torch.finfo(torch.float32).max
+    rows = [[-1.0, big], [-1e38, 2.4e38], [-big / 2, big / 2], [0.0, 1e-38], [0.0, 1e-44], [-0.0, 0.0], [-1e-40, 1e-40], [1e38, 1.5e38]]
+    x = torch.zeros((len(rows), 1, 64), device="cuda")
+    for i, (low, high) in enumerate(rows):
+        x[i, 0] = torch.linspace(0, 1, 64, device="cuda") * 1e-3 * high
+        x[i, 0, :20], x[i, 0, 40:] = low, high
+    slots = torch.arange(len(rows), dtype=torch.int32, device="cuda")
+    cache = P.new_cache(torch, 1, 1, 16, 64, seed=1)
+    want = P.append(torch, {n: t.clone() for n, t in cache.items()}, 16, x, x, slots)
+    # a range that leaves FP32 is stored with scale NaN, the codes and the minimum as zeros
+    _, _, minimum = P.quantise(torch, x)
+    beyond = (x.double().amax(-1) - minimum).float().isinf()[:, 0]
+    assert beyond.any() and not beyond[0]
+    for t in slots[beyond].tolist():
+        want["k_codes"][0, :, t] = 0
+        want["v_codes"].view(1, 1, 8, 16, 2, 2)[0, :, t // 2, :, t % 2] = 0
+        for n in ("k_params", "v_params"):
+            want[n][0, :, t, 0], want[n][0, :, t, 1] = math.nan, 0.0
+    B.kv4_append(B.kv4_append_desc(cache=P.bind(B, cache, 16), dtype=B.FP32, tokens=len(rows), k=x, v=x, slots=slots))
+    for n in cache:
+        a, b = (t.float() + 0.0 if "params" in n else t for t in (cache[n], want[n]))   # -0 is 0
+        same(a, b)
+    assert B.device_status() == 0
