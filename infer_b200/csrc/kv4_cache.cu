@@ -8,7 +8,7 @@
 // eight elements are looked at again, in 64 bits, only if one's estimate is within 10^-4 of a half.
 // One pass over the data: 2 * tokens * kv_heads * head_dim * size bytes in, head_dim + 8 bytes per token and head out;
 // a launch for single tokens; for prompts reading back is bound by memory (16384 tokens of 8 heads of 128 in BF16: 23 us,
-// 3.6 TB/s) and storing by its arithmetic, some 400 instructions for four vectors (43 us, 2.0 TB/s).  A vector belongs to
+// 3.6 TB/s) and storing by its arithmetic, some 400 instructions for four vectors (40 us, 2.1 TB/s).  A vector belongs to
 // head_dim / 8 neighbouring lanes, eight elements each, so minimum and maximum are three to five shuffles (both in one word for
 // 16-bit types) and a lane's codes are one 32-bit word.
 #include <type_traits>
@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t ScaleBits(float spread) {
 }
 
 // One code, decided in 64 bits: nearest((x - minimum) / scale), ties to even.
-__device__ __noinline__ uint32_t ExactCode(float x, float minimum, float scale, float estimate) {
+__device__ __forceinline__ uint32_t ExactCode(float x, float minimum, float scale, float estimate) {
     const float fl = floorf(estimate);
     const double d = static_cast<double>(x) - static_cast<double>(minimum);
     const double border = (static_cast<double>(fl) + 0.5) * static_cast<double>(scale);
@@ -447,7 +447,7 @@ template <int D, int L> struct RunGather {
 };
 
 // Two tokens at a time once one at a time would fill every SM twice over: 64 tokens of 8 heads of 128 are stored in 2.5 us one
-// at a time and 3.3 us in pairs, 16384 of them in 52 and 43 us, and read back in 35 and 23 us.
+// at a time and 3.3 us in pairs, 16384 of them in 52 and 43 us (both are a tenth less by now), and read back in 35 and 23 us.
 int TwoAtATime(int64_t threads) { return threads >= static_cast<int64_t>(SmCount()) * 2048 * 2 ? 1 : 0; }
 // No more blocks than run at once, `per_sm` on each SM: every thread walks on.
 unsigned SpreadBlocks(int64_t threads, int per_sm) {
