@@ -24,7 +24,9 @@
 // takes an equal, contiguous share, found from the lengths on the device.  A unit cut by shares leaves partial results
 // (maximum, sum, weighted values, FP32) in the workspace; the part that arrives last joins them in order.
 //
-// Bound: cache bytes, tokens * (head_dim + 8) per kv head.
+// Bound: cache bytes, tokens * (head_dim + 8) per kv head.  64 tokens over up to 6000 tokens each, 64 heads of 128 on 8: 75 us,
+// 3.6 TB/s; one over 200 thousand, 32 heads on 8: 64 us.  Both are 15 us (set-up, the cut units' joining) and 5 TB/s, at
+// which the instructions that unpack and weigh the codes keep up; the same copies without them run at 6.6 TB/s.
 #include "kv4_attention.cuh"
 #include "kv4_prefill.h"
 

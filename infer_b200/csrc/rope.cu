@@ -3,7 +3,8 @@
 // y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin per pair, FP32, one rounding to the output type.  Every element is read and
 // written once (2 * tokens * heads * head_dim * size bytes), three operations each: memory bound, and a launch at decode
 // size.  A block takes a few tokens and all or some of their heads; the cosines and sines of a token are the same for all
-// its heads, so they are computed once per block (64-bit reduction, sincospif) into shared memory.
+// its heads, so they are computed once per block (64-bit reduction, sincospif) into shared memory.  16383 tokens, 16 + 4 heads of
+// 256 in FP16: 61 us, 5.5 TB/s; 16 tokens, 32 + 8 heads of 128: 2.2 us.
 #include "kv4.cuh"
 
 namespace fth {
