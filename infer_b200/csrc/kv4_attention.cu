@@ -1,4 +1,4 @@
-// Attention over the 4-bit cache, few query rows per kv head (single tokens, drafts).
+// Attention over the 4-bit cache, up to 128 query rows per kv head (single tokens, drafts).
 //
 // The codes go into the matrix instructions as they are.  With value = m + s c per token (one scale and minimum for a
 // whole head),
@@ -20,7 +20,7 @@
 // a rounding of that token's share of (v - out), not by one of its code, which is far larger than the value when minimum
 // and code cancel.  The lse is taken from the probabilities before the rounding.
 //
-// Work is the flat list of (request, kv head, tile of tokens; all of a head's query rows, 8 or 16, together); every block of threads
+// Work is the flat list of (request, kv head, block of 8 or 16 query rows, tile of tokens); every block of threads
 // takes an equal, contiguous share, found from the lengths on the device.  A unit cut by shares leaves partial results
 // (maximum, sum, weighted values, FP32) in the workspace; the part that arrives last joins them in order.
 //
@@ -74,14 +74,18 @@ __device__ __forceinline__ void ComputeSync() {
     asm volatile("barrier.cta.sync 1, %0;" ::"n"(kCompute) : "memory");   // not the aligned form: lanes may come one after another
 }
 
-// Token tiles of request b's unit (one per kv head: all its rows), 0 without rows.
+// A kv head of request b in the list of tiles: the tiles of its units (blocks of `unit_rows` rows), each rounded up to a multiple
+// of `whole`.
 template <int TILE>
-__device__ __forceinline__ int RequestTiles(const AttentionParams& p, int b, int unit_rows) {
+__device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, int b, int unit_rows, int64_t whole) {
     const Request r = LoadRequest(p, b);
-    if (r.rows == 0) return 0;
-    int first, last;
-    UnitTiles<TILE>(p, r, 0, unit_rows, &first, &last);
-    return last - first;
+    int64_t sum = 0;
+    for (int row = 0; row < r.rows; row += unit_rows) {
+        int first, last;
+        UnitTiles<TILE>(p, r, row, unit_rows, &first, &last);
+        sum += whole == 1 ? last - first : Divide(last - first + whole - 1, whole) * whole;
+    }
+    return sum;
 }
 
 // A lane's packed words of one token row (or row of a pair of tokens): four words every 64 (K) or 128 (V) bytes.
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     // ---- this block's share of the tiles: every warp finds it by itself, a lane per request --------------------------------
     int64_t work = 0;
 #pragma unroll 4
-    for (int i = lane; i < p.requests; i += 32) work += RequestTiles<T::kTile>(p, i, R);
+    for (int i = lane; i < p.requests; i += 32) work += RequestTiles<T::kTile>(p, i, R, 1);
     work = WarpSum(work) * p.kv_heads;
     int64_t per = Divide(work + gridDim.x - 1, gridDim.x);
     if (per < kMinShare) per = kMinShare;
@@ -137,12 +141,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     // is as long as its shares.
     bool apart = static_cast<int64_t>(p.requests) * p.kv_heads <= gridDim.x;
     if (apart) {
-        int64_t shares = 0;
-        for (int i = lane; i < p.requests; i += 32) shares += Divide(RequestTiles<T::kTile>(p, i, R) + per - 1, per);
-        shares = WarpSum(shares) * p.kv_heads;
-        apart = shares <= gridDim.x;
-        if (apart) work = shares * per;
+        int64_t length = 0;
+        for (int i = lane; i < p.requests; i += 32) length += RequestTiles<T::kTile>(p, i, R, per);
+        length = WarpSum(length) * p.kv_heads;
+        apart = length <= per * gridDim.x;
+        if (apart) work = length;
     }
+    const int64_t whole = apart ? per : 1;
     const int64_t share_begin = blockIdx.x * per;
     const int64_t share_end = share_begin + per < work ? share_begin + per : work;
     if (share_begin >= share_end) return;
@@ -152,8 +157,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     int64_t offset_in = 0, per_head = 1;   // of share_begin in the request; the request's length in the list per head
     int64_t passed = 0;
     for (int base = 0; base < p.requests; base += 32) {
-        int64_t length = base + lane < p.requests ? RequestTiles<T::kTile>(p, base + lane, R) : 0;
-        if (apart) length = Divide(length + per - 1, per) * per;
+        const int64_t length = base + lane < p.requests ? RequestTiles<T::kTile>(p, base + lane, R, whole) : 0;
         const int64_t mine = length * p.kv_heads;
         int64_t upto = mine;
 #pragma unroll
@@ -173,10 +177,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     }
     Request req = LoadRequest(p, b);
     int head = static_cast<int>(Divide(offset_in, per_head));
-    constexpr int row = 0;   // a unit holds all rows
+    int row = 0;
     int64_t into = offset_in - head * per_head;  // tiles of the unit that other blocks take
     int tile_first, tile_last;
-    UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
+    for (;;) {
+        UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
+        const int64_t tiles = tile_last - tile_first, length = apart ? Divide(tiles + per - 1, per) * per : tiles;
+        if (into < length || row + R >= req.rows) break;
+        into -= length;
+        row += R;
+    }
     int64_t at = share_begin;
     int t0, steps, first_low, last_high;   // of this block's part of the unit
     const auto place = [&] {
@@ -191,12 +201,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         at += steps;
         if (apart || at >= share_end) return false;
         into = 0;
-        if (++head == p.kv_heads) {
-            head = 0;
-            do {
-                ++b;
-                req = LoadRequest(p, b);
-            } while (req.rows == 0);
+        row += R;
+        if (row >= req.rows) {
+            row = 0;
+            if (++head == p.kv_heads) {
+                head = 0;
+                do {
+                    ++b;
+                    req = LoadRequest(p, b);
+                } while (req.rows == 0);
+            }
         }
         UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
         place();
@@ -710,10 +724,12 @@ int CheckAttention(const fth_b200_kv4_attention_desc* d) {
 constexpr int kMaxGrid = 1024;
 constexpr size_t kCounterBytes = kMaxGrid * sizeof(int);
 
-// Query rows of a unit, in eights: 8 when no request has more.
-int DecodeTiles(const fth_b200_kv4_attention_desc& d) {
-    return static_cast<int64_t>(d.max_query) * (d.q_heads / d.cache.kv_heads) <= 8 ? 1 : 2;
-}
+// Rows of a kv head that a request may have.
+int64_t MostRows(const fth_b200_kv4_attention_desc& d) { return static_cast<int64_t>(d.max_query) * (d.q_heads / d.cache.kv_heads); }
+// Query rows of a unit, in eights.  Sixteen share what unpacking costs (12 requests of 3500 .. 9000 tokens, 2 kv heads of 128, 32 rows:
+// 27.5 us, 32.4 us in eights), unless half of the last ones would be missing (32 requests, 8 kv heads, 20 rows: 123 us, 113 us in eights); 256-wide
+// heads leave no registers for them (20 rows: 69 us, 42 us in eights).
+int DecodeTiles(const fth_b200_kv4_attention_desc& d) { return d.cache.head_dim != 256 && (MostRows(d) + 7) / 8 % 2 == 0 ? 2 : 1; }
 // Blocks of threads that are resident together.
 int DecodeGrid(const fth_b200_kv4_attention_desc& d) {
     const int per_sm = d.cache.head_dim == 256 || DecodeTiles(d) == 2 ? kBlocksPerSm<256, 1> : kBlocksPerSm<128, 1>;
@@ -722,8 +738,10 @@ int DecodeGrid(const fth_b200_kv4_attention_desc& d) {
 }
 
 
-// More query rows per kv head than two eights: the kernel with 128-row tiles.
-bool ManyRows(const fth_b200_kv4_attention_desc& d) { return static_cast<int64_t>(d.max_query) * (d.q_heads / d.cache.kv_heads) > 16; }
+// The kernel with 128-row tiles.  It unpacks as much for a row as for 256, and its tiles start late: those 12 requests of 2 kv heads of 128
+// take it 56, 83 and 124 us with 20, 64 and 128 rows, eights and sixteens 27, 44 and 73 us; 256-wide heads 76, 108 and 154 us against
+// 42, 80 and 142 us.
+bool ManyRows(const fth_b200_kv4_attention_desc& d) { return MostRows(d) > 128; }
 
 size_t WorkspaceBytes(const fth_b200_kv4_attention_desc& d) {
     if (ManyRows(d)) return kCounterBytes + static_cast<size_t>(PrefillPartialFloats(d.cache.head_dim)) * sizeof(float);

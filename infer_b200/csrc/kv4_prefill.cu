@@ -1,4 +1,4 @@
-// Attention over the 4-bit cache, many query rows per kv head (prompts, chunks of them, long drafts).
+// Attention over the 4-bit cache, more than 128 query rows per kv head (prompts, chunks of them).
 //
 // A tile of 128 query rows (queries x heads of the group, so a group shares every key) against tiles of 128 tokens,
 //     S = Q K^T     tcgen05.mma kind::f16, both operands in shared memory, accumulator in tensor memory

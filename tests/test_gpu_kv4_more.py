@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("new,hq,hk", [(1, 2, 2), (5, 4, 1)])
+@pytest.mark.parametrize("new,hq,hk", [(1, 2, 2), (5, 4, 1), (40, 4, 1)])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_many_requests(cuda, new, hq, hk, dim):
     """More requests than a block has threads, some of them empty or idle, in both kernels."""
@@ -71,7 +71,7 @@ def near(torch, a, b, dtype):
 
 
 @pytest.mark.parametrize("name,which", [("k_params", 0), ("k_params", 1), ("v_params", 0), ("v_params", 1)])
-@pytest.mark.parametrize("dtype,new", [("bf16", 1), ("bf16", 64), ("fp16", 64)])
+@pytest.mark.parametrize("dtype,new", [("bf16", 1), ("bf16", 64), ("fp16", 64), ("bf16", 80), ("fp16", 80)])
 def test_scales_and_minima_that_are_no_numbers(cuda, name, which, dtype, new):
     """The token's scale or minimum of keys or values: the rows that see it are NaN, the others (behind the mask or the window, of
     other heads and requests) are what they were up to the roundings, which depend on the rows worked on together: each result is
@@ -102,7 +102,7 @@ def test_scales_and_minima_that_are_no_numbers(cuda, name, which, dtype, new):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-@pytest.mark.parametrize("new", [2, 64])
+@pytest.mark.parametrize("new", [2, 64, 80])
 def test_an_infinity_in_one_row_leaves_the_others(cuda, dtype, new):
     torch = cuda
     r = attend(torch, dtype=dtype, lens=[300], new=[new], hq=4, hk=2, dim=128, bs=16, seed=4, lse=False)
@@ -115,6 +115,32 @@ def test_an_infinity_in_one_row_leaves_the_others(cuda, dtype, new):
     keep[new:] = False
     near(torch, got[keep], before.view(-1, 4, 128)[keep], dtype)
     assert got[new - 1, 0].isnan().all() and (r["out"][new:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("fp16", 128), ("bf16", 256)])
+def test_hidden_blocks_of_many_rows(cuda, dtype, dim):
+    """A block number outside the cache hides its tokens and is reported; also the first and the last block."""
+    torch = cuda
+    r = attend(torch, dtype=dtype, lens=[260], new=[80], hq=4, hk=2, dim=dim, bs=16)
+    table = r["table"].clone()
+    for column in (0, 7, 16):
+        r["table"][0, column] = -1
+        B.kv4_attention(r["desc"])
+        assert B.device_status() >> 16 == 42
+        got = r["out"][:80].reshape(80, 4, dim).double()
+        want, _, limit, _ = P.attention(torch, r["cache"], 16, table, r["q"][:80].reshape(80, 4, dim), [260], [80], 2, dim ** -0.5, True, 0,
+                                        hidden=range(column * 16, min(column * 16 + 16, 260)), key_rounding=key_rounding(dtype, 160))
+        assert ((got - want).abs() <= limit + half_step(torch, dtype_of(torch, dtype)) * want.abs() + 1e-6 * (dtype == "fp16") + 1e-30).all()
+        r["table"].copy_(table)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new,hq,hk", [(3, 8, 1), (5, 8, 2), (10, 4, 1), (12, 8, 2), (32, 8, 2), (33, 8, 2), (128, 1, 1), (129, 2, 2)])
+def test_rows_in_blocks_of_eight_and_sixteen(cuda, dtype, dim, new, hq, hk):
+    """17 .. 132 rows to a kv head: several units to a head, of which the first see less; cut and whole; few and many requests."""
+    attend(cuda, dtype=dtype, lens=[1500, new, 40], new=[new, new, 1], hq=hq, hk=hk, dim=dim, bs=32, seed=new)
+    attend(cuda, dtype=dtype, lens=[200 + 13 * i for i in range(60)], new=[new - i % 3 for i in range(60)], hq=hq, hk=hk, dim=dim, bs=16, seed=new, window=150)
 
 
 def test_two_graphs_share_a_workspace(cuda):
