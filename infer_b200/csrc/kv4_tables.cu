@@ -5,8 +5,8 @@
 // block.  Nothing about them is bandwidth or arithmetic; they cost a launch and a few dependent memory round trips.  So:
 // one launch, every block of threads computes all the sums for itself (8 bytes per request, from L2) instead of waiting
 // for another one, and then writes its share of the rows and of the new table entries, found by binary search in shared
-// memory, so that one long prompt spreads over the chip like many short ones.  64 requests with a new token each: 5.7 us a
-// launch; 1000 with up to 400: 8 us.
+// memory, so that one long prompt spreads over the chip like many short ones.  64 requests with a new token each: 3.2 us a
+// launch; 1000 with up to 400: 7 us.
 // What may be updated in place (lengths, the free count) is written by the block that finishes last: by then every
 // block has read it.  The ticket that finds the last block is integer and its order does not reach the results.
 #include "kv4.cuh"
@@ -16,29 +16,51 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMany = 1024, kFew = 256;   // threads of a block; few when that many requests and rows are all there is
 
-// Inclusive sum over the threads of a block, in thread order; `total` receives the sum over all.
-__device__ __forceinline__ int64_t BlockScan(int64_t v, int64_t* shared, int64_t* total) {
+// Inclusive sums of two numbers over the threads of a block, in thread order, their totals, and flags of all threads together.
+template <int THREADS>
+struct Scan {
+    int64_t a[THREADS / 32], b[THREADS / 32];
+    int flags[THREADS / 32];
+};
+struct Sums {
+    int64_t a, b, all_a, all_b;
+    int flags;
+};
+template <int THREADS>
+__device__ __forceinline__ Sums BlockScan(int64_t a, int64_t b, int flags, Scan<THREADS>& shared) {
+    constexpr int kWarps = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t n = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += n;
+        const int64_t x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) {
+            a += x;
+            b += y;
+        }
     }
-    __syncthreads();  // `shared` may still be read from the previous call
-    if (lane == 31) shared[warp] = v;
+    flags = __reduce_or_sync(0xffffffffu, flags);
     __syncthreads();
-    int64_t w = lane < kWarps ? shared[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t n = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += n;
+    if (lane == 31) {
+        shared.a[warp] = a;
+        shared.b[warp] = b;
+        shared.flags[warp] = flags;
     }
-    const int64_t before = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
-    *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
-    return v + (warp == 0 ? 0 : before);
+    __syncthreads();
+    int64_t v = lane < kWarps ? shared.a[lane] : 0, w = lane < kWarps ? shared.b[lane] : 0;
+    flags = __reduce_or_sync(0xffffffffu, lane < kWarps ? shared.flags[lane] : 0);
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, v, o), y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) {
+            v += x;
+            w += y;
+        }
+    }
+    const int before = warp == 0 ? 0 : warp - 1;
+    const int64_t before_a = __shfl_sync(0xffffffffu, v, before), before_b = __shfl_sync(0xffffffffu, w, before);
+    return Sums{a + (warp == 0 ? 0 : before_a), b + (warp == 0 ? 0 : before_b), __shfl_sync(0xffffffffu, v, kWarps - 1), __shfl_sync(0xffffffffu, w, kWarps - 1), flags};
 }
 
 // Largest i with starts[i] <= x (starts[0] = 0 <= x).
@@ -80,6 +102,7 @@ __device__ __forceinline__ void Share(int64_t count, int64_t* first, int64_t* la
 __device__ __forceinline__ bool ArriveLast(int32_t* status) {
     __shared__ int last;
     __syncthreads();
+    if (gridDim.x == 1) return true;
     if (threadIdx.x == 0) {
         __threadfence();
         last = atomicAdd(&status[1], 1) == static_cast<int>(gridDim.x) - 1;
@@ -89,37 +112,37 @@ __device__ __forceinline__ bool ArriveLast(int32_t* status) {
     return last != 0;
 }
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) AssignKernel(const __grid_constant__ AssignParams p) {
-    __shared__ int64_t scan[kWarps];
+    __shared__ Scan<kThreads> scan;
     __shared__ int row_start[kThreads + 1];
     __shared__ int need_start[kThreads + 1];
     __shared__ int cached_s[kThreads];
     WaitForPrevious();
     // totals over all requests, and whether the step fits
     const int free_count = *p.free_count;
-    int64_t rows = 0, need = 0;
-    int bad_length = 0, table_full = 0;
+    int64_t rows = 0, need = 0, n = 0, b = 0;
+    int c = 0, flags = 0;   // flags: 1 a bad length, 2 a row of the table that is too short
+    Sums sums;
     for (int base = 0; base < p.requests; base += kThreads) {
         const int r = base + threadIdx.x;
-        int64_t n = 0, b = 0;
+        n = b = c = 0;
+        int mine = 0;
         if (r < p.requests) {
-            const int64_t c = p.cached[r];
+            c = p.cached[r];
             n = p.fresh[r];
-            if (c < 0 || n < 0) bad_length = 1;
+            if (c < 0 || n < 0) mine = 1;
             b = BlocksFor(c + n, p.shift) - BlocksFor(c, p.shift);
-            if (BlocksFor(c + n, p.shift) > p.max_blocks) table_full = 1;
+            if (BlocksFor(c + n, p.shift) > p.max_blocks) mine |= 2;
         }
-        int64_t total;
-        BlockScan(n, scan, &total);
-        rows += total;
-        BlockScan(b, scan, &total);
-        need += total;
+        sums = BlockScan(n, b, mine, scan);
+        rows += sums.all_a;
+        need += sums.all_b;
+        flags |= sums.flags;
     }
-    bad_length = __syncthreads_or(bad_length);
-    table_full = __syncthreads_or(table_full);
     int refused = FTH_B200_KV4_OK;
-    if (bad_length) refused = FTH_B200_KV4_BAD_LENGTH;
-    else if (table_full) refused = FTH_B200_KV4_TABLE_FULL;
+    if (flags & 1) refused = FTH_B200_KV4_BAD_LENGTH;
+    else if (flags & 2) refused = FTH_B200_KV4_TABLE_FULL;
     else if (rows > p.tokens) refused = FTH_B200_KV4_TOO_MANY_TOKENS;
     else if (free_count < 0 || free_count > p.blocks || need > free_count) refused = FTH_B200_KV4_NO_BLOCKS;
 
@@ -131,15 +154,17 @@ __global__ void __launch_bounds__(kThreads) AssignKernel(const __grid_constant__
         for (int base = 0; base < p.requests; base += kThreads) {
             const int r = base + threadIdx.x;
             const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
-            int64_t n = 0, b = 0, rows_here, need_here;
-            int c = 0;
-            if (r < p.requests) {
-                c = p.cached[r];
-                n = p.fresh[r];
-                b = BlocksFor(c + n, p.shift) - BlocksFor(c, p.shift);
+            if (p.requests > kThreads) {   // else the sums of all are there
+                n = b = c = 0;
+                if (r < p.requests) {
+                    c = p.cached[r];
+                    n = p.fresh[r];
+                    b = BlocksFor(c + n, p.shift) - BlocksFor(c, p.shift);
+                }
+                sums = BlockScan(n, b, 0, scan);
+                __syncthreads();  // the previous chunk's searches are done
             }
-            const int64_t row_end = BlockScan(n, scan, &rows_here), need_end = BlockScan(b, scan, &need_here);
-            __syncthreads();  // the previous chunk's searches are done
+            const int64_t row_end = sums.a, need_end = sums.b, rows_here = sums.all_a, need_here = sums.all_b;
             if (threadIdx.x == 0) row_start[0] = need_start[0] = 0;
             row_start[threadIdx.x + 1] = static_cast<int>(row_end);
             need_start[threadIdx.x + 1] = static_cast<int>(need_end);
@@ -203,32 +228,34 @@ struct ReleaseParams {
     int32_t* status;
 };
 
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) ReleaseKernel(const __grid_constant__ ReleaseParams p) {
-    __shared__ int64_t scan[kWarps];
+    __shared__ Scan<kThreads> scan;
     __shared__ int back_start[kThreads + 1];
     __shared__ int first_s[kThreads];
     WaitForPrevious();
     const int free_count = *p.free_count;
-    int64_t back = 0;
-    int bad_length = 0, table_full = 0;
+    int64_t back = 0, b = 0;
+    int first = 0, flags = 0;   // flags as above
+    Sums sums;
     for (int base = 0; base < p.requests; base += kThreads) {
         const int r = base + threadIdx.x;
-        int64_t b = 0;
+        b = first = 0;
+        int mine = 0;
         if (r < p.requests) {
             const int64_t n = p.lens[r], k = p.keep[r];
-            if (k < 0 || k > n) bad_length = 1;
+            if (k < 0 || k > n) mine = 1;
+            first = static_cast<int>(BlocksFor(k, p.shift));
             b = BlocksFor(n, p.shift) - BlocksFor(k, p.shift);
-            if (BlocksFor(n, p.shift) > p.max_blocks) table_full = 1;
+            if (BlocksFor(n, p.shift) > p.max_blocks) mine |= 2;
         }
-        int64_t total;
-        BlockScan(b, scan, &total);
-        back += total;
+        sums = BlockScan(b, int64_t{0}, mine, scan);
+        back += sums.all_a;
+        flags |= sums.flags;
     }
-    bad_length = __syncthreads_or(bad_length);
-    table_full = __syncthreads_or(table_full);
     int refused = FTH_B200_KV4_OK;
-    if (bad_length) refused = FTH_B200_KV4_BAD_LENGTH;
-    else if (table_full) refused = FTH_B200_KV4_TABLE_FULL;
+    if (flags & 1) refused = FTH_B200_KV4_BAD_LENGTH;
+    else if (flags & 2) refused = FTH_B200_KV4_TABLE_FULL;
     else if (free_count < 0 || free_count + back > p.blocks) refused = FTH_B200_KV4_NO_BLOCKS;
     if (refused == FTH_B200_KV4_OK) {
         int64_t mine_first, mine_last;
@@ -237,14 +264,16 @@ __global__ void __launch_bounds__(kThreads) ReleaseKernel(const __grid_constant_
         for (int base = 0; base < p.requests; base += kThreads) {
             const int r = base + threadIdx.x;
             const int count = p.requests - base < kThreads ? p.requests - base : kThreads;
-            int64_t b = 0, here;
-            int first = 0;
-            if (r < p.requests) {
-                first = static_cast<int>(BlocksFor(p.keep[r], p.shift));
-                b = BlocksFor(p.lens[r], p.shift) - first;
+            if (p.requests > kThreads) {
+                b = first = 0;
+                if (r < p.requests) {
+                    first = static_cast<int>(BlocksFor(p.keep[r], p.shift));
+                    b = BlocksFor(p.lens[r], p.shift) - first;
+                }
+                sums = BlockScan(b, int64_t{0}, 0, scan);
+                __syncthreads();
             }
-            const int64_t end = BlockScan(b, scan, &here);
-            __syncthreads();
+            const int64_t end = sums.a, here = sums.all_a;
             if (threadIdx.x == 0) back_start[0] = 0;
             back_start[threadIdx.x + 1] = static_cast<int>(end);
             first_s[threadIdx.x] = first;
@@ -279,11 +308,14 @@ int CheckTables(const Desc* d) {
     return FTH_B200_OK;
 }
 
-// One block of threads up to a few thousand writes; a whole chip's worth for long prompts.
-unsigned TableBlocks(int64_t writes) {
-    const int64_t blocks = (writes + 4 * kThreads - 1) / (4 * kThreads);
+// One block of threads up to `each` writes, which needs no ticket; a whole chip's worth for long prompts.
+unsigned TableBlocks(int64_t writes, int each) {
+    const int64_t blocks = (writes + each - 1) / each;
     return static_cast<unsigned>(blocks < 1 ? 1 : blocks > SmCount() ? SmCount() : blocks);
 }
+// A block of few threads has its sums sooner (64 requests with a token each, assign and release: 6.5 us; 11.4 us with 1024 threads, every
+// sum by itself and a ticket).
+bool Few(int64_t requests, int64_t writes) { return requests <= kFew && writes <= 2 * kFew; }
 
 }  // namespace
 }  // namespace kv4
@@ -302,7 +334,9 @@ extern "C" int fth_b200_kv4_assign(const fth_b200_kv4_assign_desc* d, fth_b200_s
     const kv4::AssignParams p{d->requests, d->max_blocks, kv4::Log2(d->block_size), static_cast<int>(d->blocks), static_cast<int>(d->tokens),
                               d->cached_lens, d->new_lens, d->free_blocks, d->free_count, d->free_count_out, d->block_table, d->total_lens,
                               d->query_start, d->slots, d->positions, d->status};
-    const int status = kv4::Launch(kv4::AssignKernel, dim3(kv4::TableBlocks(d->tokens)), kv4::kThreads, 0, static_cast<cudaStream_t>(stream), p);
+    auto s = static_cast<cudaStream_t>(stream);
+    const int status = kv4::Few(d->requests, d->tokens) ? kv4::Launch(kv4::AssignKernel<kv4::kFew>, dim3(1), kv4::kFew, 0, s, p)
+                                                        : kv4::Launch(kv4::AssignKernel<kv4::kMany>, dim3(kv4::TableBlocks(d->tokens, 4 * kv4::kMany)), kv4::kMany, 0, s, p);
     if (status == FTH_B200_OK) NoteLaunch("kv4_assign");
     return status;
 }
@@ -314,9 +348,12 @@ extern "C" int fth_b200_kv4_release(const fth_b200_kv4_release_desc* d, fth_b200
     if (rc != FTH_B200_OK) return rc;
     const kv4::ReleaseParams p{d->requests, d->max_blocks, kv4::Log2(d->block_size), static_cast<int>(d->blocks), d->lens, d->keep_lens,
                                d->free_blocks, d->free_count, d->free_count_out, d->block_table, d->lens_out, d->status};
-    const int64_t most = static_cast<int64_t>(d->requests) * d->max_blocks;
-    const int status = kv4::Launch(kv4::ReleaseKernel, dim3(kv4::TableBlocks(most < d->blocks ? most : d->blocks)), kv4::kThreads, 0,
-                                   static_cast<cudaStream_t>(stream), p);
+    int64_t most = static_cast<int64_t>(d->requests) * d->max_blocks;
+    if (most > d->blocks) most = d->blocks;
+    auto s = static_cast<cudaStream_t>(stream);
+    // how many blocks come back is not known here: few, mostly, of all that could
+    const int status = kv4::Few(d->requests, most) ? kv4::Launch(kv4::ReleaseKernel<kv4::kFew>, dim3(1), kv4::kFew, 0, s, p)
+                                                   : kv4::Launch(kv4::ReleaseKernel<kv4::kMany>, dim3(kv4::TableBlocks(most, 32 * kv4::kMany)), kv4::kMany, 0, s, p);
     if (status == FTH_B200_OK) NoteLaunch("kv4_release");
     return status;
 }
