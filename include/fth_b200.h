@@ -550,7 +550,7 @@ int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* desc, fth_b200_stream_t 
  * total_lens[r] without `causal`), of those the last `window` (window > 0; counted from p).  kv_heads divides q_heads;
  * q head h reads kv head h / (q_heads / kv_heads).
  *   out = softmax(scale * q . K) . V,  lse (optional, FP32 [tokens, q_heads]) = ln(sum(exp(scale * q . K)))
- * A row that sees nothing gets zeros and lse = -infinity.  Rows behind query_start[requests] are left as they were.
+ * out must not overlap q.  A row that sees nothing gets zeros and lse = -infinity.  Rows behind query_start[requests] are left as they were.
  * Scores, softmax statistics and sums are FP32.  With up to 128 rows to a kv head (max_query * q_heads / kv_heads) codes enter
  * exactly and the product of a probability and the scale of its value is rounded to FP16 (11 bits, down to 2^-20 of the
  * largest scale among the values seen).  With more rows probabilities and values are rounded to FP16 one by one, and with BF16

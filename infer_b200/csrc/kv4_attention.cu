@@ -56,16 +56,12 @@ struct Shape {
 template <int D, int NT>
 constexpr int kBlocksPerSm = D == 256 || NT == 2 ? 2 : 3;
 
-template <int D, int NT>
-constexpr bool kQueriesInShared = D == 256 && NT == 2;   // 64 registers of fragments would not fit beside 128 accumulators
-
-// Dynamic shared memory: the ring, the place where the warps' results are joined, then query operands.
+// Dynamic shared memory: the ring, then the place where the warps' results are joined.
 template <int D, int NT>
 struct Layout {
     static constexpr size_t kJoin = static_cast<size_t>(Shape<D>::kStages) * Shape<D>::kStageBytes;
     static constexpr size_t kJoinFloats = static_cast<size_t>(kWarps) * 8 * NT * kRow<D>;
-    static constexpr size_t kQueries = kJoin + kJoinFloats * sizeof(float);
-    static constexpr size_t kBytes = kQueries + (kQueriesInShared<D, NT> ? NT * Shape<D>::kWords * 32 * 16 : 0);
+    static constexpr size_t kBytes = kJoin + kJoinFloats * sizeof(float);
 };
 
 // Barrier of the warps that compute.
@@ -111,7 +107,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     constexpr int CW = W == 2 ? 2 : 4;        // words of a chunk
     constexpr int S = T::kStages;
     constexpr int R = 8 * NT;
-    constexpr bool QS = kQueriesInShared<D, NT>;
     constexpr int I = 2;   // sixteens of tokens worked on together
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int join_last;
@@ -294,8 +289,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         const int64_t unit_end = unit_begin + (tile_last - tile_first);
 
         // ---- query rows ----------------------------------------------------------------------------------------------------
-        uint32_t qf[QS ? 1 : NT][2 * W][2];
-        uint4* const q_shared = reinterpret_cast<uint4*>(smem + Layout<D, NT>::kQueries);
+        uint32_t qf[NT][2 * W][2];
         float qsum[NT][2];   // of the columns 2 * quad, 2 * quad + 1
         int row_low[NT][2], row_high[NT][2];
         int all_low = 0, all_high = 0x7fffffff;
@@ -365,17 +359,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                 for (int w = 0; w < W; ++w) {
                     uint32_t f[4];
                     QueryOperands<DTYPE>(raw[n][w], up, 0.0625f, f);
-                    if constexpr (QS) {
-                        if (warp == 0) q_shared[(n * W + w) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
-                    } else {
-                        qf[n][2 * w][0] = f[0];
-                        qf[n][2 * w][1] = f[1];
-                        qf[n][2 * w + 1][0] = f[2];
-                        qf[n][2 * w + 1][1] = f[3];
-                    }
+                    qf[n][2 * w][0] = f[0];
+                    qf[n][2 * w][1] = f[1];
+                    qf[n][2 * w + 1][0] = f[2];
+                    qf[n][2 * w + 1][1] = f[3];
                 }
             }
-            if constexpr (QS) ComputeSync();
         }
 
         // ---- tokens -----------------------------------------------------------------------------------------------------------
@@ -426,9 +415,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                             const uint32_t x0 = k0[i], x1 = k1[i], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                uint4 f;
-                                if constexpr (QS) f = q_shared[(n * W + w) * 32 + lane];
-                                else f = make_uint4(qf[n][2 * w][0], qf[n][2 * w][1], qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                                const uint4 f = make_uint4(qf[n][2 * w][0], qf[n][2 * w][1], qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
                                 if (w == 0) MmaF16First(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, f.x, f.y);
                                 else MmaF16(z[s][n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, f.x, f.y);
                                 MmaF16(z[s][n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, f.z, f.w);
@@ -754,7 +741,10 @@ int LaunchDecode(const AttentionParams& p, int tiles, int grid, cudaStream_t s) 
         if (EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), smem) != FTH_B200_OK) return static_cast<int>(FTH_B200_ERR_CUDA);
         return Launch(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, s, p);
     };
-    return tiles == 1 ? run(DecodeKernel<D, DTYPE, 1>, Layout<D, 1>::kBytes) : run(DecodeKernel<D, DTYPE, 2>, Layout<D, 2>::kBytes);
+    if constexpr (D != 256) {
+        if (tiles == 2) return run(DecodeKernel<D, DTYPE, 2>, Layout<D, 2>::kBytes);
+    }
+    return run(DecodeKernel<D, DTYPE, 1>, Layout<D, 1>::kBytes);
 }
 
 }  // namespace
