@@ -70,8 +70,9 @@ __device__ __forceinline__ void ComputeSync() {
     asm volatile("barrier.cta.sync 1, %0;" ::"n"(kCompute) : "memory");   // not the aligned form: lanes may come one after another
 }
 
-// A kv head of request b in the list of tiles: the tiles of its units (blocks of `unit_rows` rows), each rounded up to a multiple
-// of `whole`.
+// Tiles of a unit in the list: a multiple of `whole`.
+__device__ __forceinline__ int64_t Rounded(int tiles, int64_t whole) { return whole == 1 ? tiles : Divide(tiles + whole - 1, whole) * whole; }
+// A kv head of request b in the list: its units (blocks of `unit_rows` rows).
 template <int TILE>
 __device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, int b, int unit_rows, int64_t whole) {
     const Request r = LoadRequest(p, b);
@@ -79,7 +80,7 @@ __device__ __forceinline__ int64_t RequestTiles(const AttentionParams& p, int b,
     for (int row = 0; row < r.rows; row += unit_rows) {
         int first, last;
         UnitTiles<TILE>(p, r, row, unit_rows, &first, &last);
-        sum += whole == 1 ? last - first : Divide(last - first + whole - 1, whole) * whole;
+        sum += Rounded(last - first, whole);
     }
     return sum;
 }
@@ -100,6 +101,11 @@ __device__ __forceinline__ void LoadChunk(const uint8_t* row, int place, int chu
     }
 }
 
+struct Shares {
+    int64_t begin, end;   // this block's share of the list
+    int64_t per, whole;   // the length of a share, of which a unit's length in the list is a multiple
+};
+
 template <int D, int DTYPE, int NT>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(const __grid_constant__ AttentionParams p) {
     using T = Shape<D>;
@@ -109,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     constexpr int R = 8 * NT;
     constexpr int I = 2;   // sixteens of tokens worked on together
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Shares share;    // not held in registers over the tokens
     __shared__ int join_last;
     __shared__ __align__(8) uint64_t full[S], empty[S];
     __shared__ uint32_t stage_present[S];   // a bit for every 16 tokens of the stage that are there
@@ -129,23 +136,25 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll 4
     for (int i = lane; i < p.requests; i += 32) work += RequestTiles<T::kTile>(p, i, R, 1);
     work = WarpSum(work) * p.kv_heads;
-    int64_t per = Divide(work + gridDim.x - 1, gridDim.x);
+    int64_t per = Divide(work + gridDim.x - 1, gridDim.x), whole = 1;
     if (per < kMinShare) per = kMinShare;
     // With fewer units than blocks of threads a share ends with its unit, if there are blocks enough: units up to `per` tiles
     // are not cut then (one request of 333 tokens, 2 kv heads: 13.9 us when the second unit was).  In the list such a unit
     // is as long as its shares.
-    bool apart = static_cast<int64_t>(p.requests) * p.kv_heads <= gridDim.x;
-    if (apart) {
+    if (static_cast<int64_t>(p.requests) * p.kv_heads <= gridDim.x) {
         int64_t length = 0;
         for (int i = lane; i < p.requests; i += 32) length += RequestTiles<T::kTile>(p, i, R, per);
         length = WarpSum(length) * p.kv_heads;
-        apart = length <= per * gridDim.x;
-        if (apart) work = length;
+        if (length <= per * gridDim.x) {
+            whole = per;
+            work = length;
+        }
     }
-    const int64_t whole = apart ? per : 1;
     const int64_t share_begin = blockIdx.x * per;
     const int64_t share_end = share_begin + per < work ? share_begin + per : work;
     if (share_begin >= share_end) return;
+    if (threadIdx.x == 0) share = Shares{share_begin, share_end, per, whole};
+    __syncthreads();
 
     // ---- the first unit: request, head, tiles -----------------------------------------------------------------------------
     int b = 0;
@@ -177,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     int tile_first, tile_last;
     for (;;) {
         UnitTiles<T::kTile>(p, req, row, R, &tile_first, &tile_last);
-        const int64_t tiles = tile_last - tile_first, length = apart ? Divide(tiles + per - 1, per) * per : tiles;
+        const int64_t length = Rounded(tile_last - tile_first, whole);
         if (into < length || row + R >= req.rows) break;
         into -= length;
         row += R;
@@ -185,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
     int64_t at = share_begin;
     int t0, steps, first_low, last_high;   // of this block's part of the unit
     const auto place = [&] {
-        const int64_t left = share_end - at, tiles = tile_last - tile_first - into;
+        const int64_t left = share.end - at, tiles = tile_last - tile_first - into;
         t0 = tile_first + static_cast<int>(into);
         steps = static_cast<int>(tiles < left ? tiles : left);
         int unused;
@@ -193,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         Visible(p, req, QueryOf(p, (row + R < req.rows ? row + R : req.rows) - 1), &unused, &last_high);
     };
     const auto next_unit = [&] {   // false: the share is done
-        at += steps;
-        if (apart || at >= share_end) return false;
+        at += Rounded(tile_last - tile_first, share.whole) - into;
+        if (at >= share.end) return false;
         into = 0;
         row += R;
         if (row >= req.rows) {
@@ -642,8 +651,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
         }
         ComputeSync();
         // blocks of threads that hold the first and the last part of the unit
-        const int64_t part_first = unit_begin >= share_begin ? blockIdx.x : Divide(unit_begin, per);
-        const int64_t part_last = unit_end <= share_end ? blockIdx.x : Divide(unit_end - 1, per);
+        const int64_t part_first = unit_begin >= share.begin ? blockIdx.x : Divide(unit_begin, share.per);
+        const int64_t part_last = unit_end <= share.end ? blockIdx.x : Divide(unit_end - 1, share.per);
         const bool whole = part_first == part_last;
         const int valid_rows = req.rows - row < R ? req.rows - row : R;
         const int64_t slot_floats = static_cast<int64_t>(R) * kRow<D>;

@@ -308,7 +308,8 @@ int CheckTables(const Desc* d) {
     return FTH_B200_OK;
 }
 
-// One block of threads up to `each` writes, which needs no ticket; a whole chip's worth for long prompts.
+// One block of threads up to `each` writes, which needs no ticket; a whole chip's worth for long prompts (1000 requests
+// with up to 400 new tokens: 14.5 us with 4096 rows to a block, 12.8 with 2048, 12.5 with 1024).
 unsigned TableBlocks(int64_t writes, int each) {
     const int64_t blocks = (writes + each - 1) / each;
     return static_cast<unsigned>(blocks < 1 ? 1 : blocks > SmCount() ? SmCount() : blocks);
@@ -336,7 +337,7 @@ extern "C" int fth_b200_kv4_assign(const fth_b200_kv4_assign_desc* d, fth_b200_s
                               d->query_start, d->slots, d->positions, d->status};
     auto s = static_cast<cudaStream_t>(stream);
     const int status = kv4::Few(d->requests, d->tokens) ? kv4::Launch(kv4::AssignKernel<kv4::kFew>, dim3(1), kv4::kFew, 0, s, p)
-                                                        : kv4::Launch(kv4::AssignKernel<kv4::kMany>, dim3(kv4::TableBlocks(d->tokens, 4 * kv4::kMany)), kv4::kMany, 0, s, p);
+                                                        : kv4::Launch(kv4::AssignKernel<kv4::kMany>, dim3(kv4::TableBlocks(d->tokens, 2 * kv4::kMany)), kv4::kMany, 0, s, p);
     if (status == FTH_B200_OK) NoteLaunch("kv4_assign");
     return status;
 }
