@@ -9,7 +9,8 @@
 // the higher places, a power of two that puts the largest element of the rows at 2^14) and into the results; all are exact.
 //
 // S^T = K q^T: tokens are the 16 rows of the instruction, query rows its 8 columns, so a group of up to eight query
-// heads fills it and the products of one K word serve all of them.  O^T = V^T P^T likewise: head elements are its rows.
+// heads fills it and the products of one K word serve all of them (up to four take every other column, and what a lane
+// would do for the other ones is left out).  O^T = V^T P^T likewise: head elements are its rows.
 // P^T comes from S^T by transposing 8 x 8 tiles within the warp.  One warp of a block of threads streams the tokens of its
 // share through a ring in shared memory with bulk copies (a block's codes of one head are contiguous), also across units,
 // so that the next unit's tokens fly while this one's results are joined; four warps compute, each on its 32 or 64 tokens
@@ -20,12 +21,12 @@
 // a rounding of that token's share of (v - out), not by one of its code, which is far larger than the value when minimum
 // and code cancel.  The lse is taken from the probabilities before the rounding.
 //
-// Work is the flat list of (request, kv head, block of 8 or 16 query rows, tile of tokens); every block of threads
+// Work is the flat list of (request, kv head, block of 4, 8 or 16 query rows, tile of tokens); every block of threads
 // takes an equal, contiguous share, found from the lengths on the device.  A unit cut by shares leaves partial results
 // (maximum, sum, weighted values, FP32) in the workspace; the part that arrives last joins them in order.
 //
 // Bound: cache bytes, tokens * (head_dim + 8) per kv head.  64 tokens over up to 6000 tokens each, 64 heads of 128 on 8: 75 us,
-// 3.6 TB/s; one over 200 thousand, 32 heads on 8: 64 us.  Both are 15 us (set-up, the cut units' joining) and 5 TB/s, at
+// 3.6 TB/s; one over 200 thousand, 32 heads on 8: 66 us.  Both are 15 us (set-up, the cut units' joining) and 5 TB/s, at
 // which the instructions that unpack and weigh the codes keep up; the same copies without them run at 6.6 TB/s.
 #include "kv4_attention.cuh"
 #include "kv4_prefill.h"
@@ -106,13 +107,16 @@ struct Shares {
     int64_t per, whole;   // the length of a share, of which a unit's length in the list is a multiple
 };
 
-template <int D, int DTYPE, int NT>
+// C: columns of the score tile that a lane works on.  1: up to four rows, in the columns 2 * quad; the odd ones are zeros and nothing
+// is computed for them.
+template <int D, int DTYPE, int NT, int C>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(const __grid_constant__ AttentionParams p) {
     using T = Shape<D>;
     constexpr int W = T::kWords;
     constexpr int CW = W == 2 ? 2 : 4;        // words of a chunk
     constexpr int S = T::kStages;
-    constexpr int R = 8 * NT;
+    constexpr int R = 4 * NT * C;             // rows of a unit
+    static_assert(C == 2 || NT == 1, "");
     constexpr int I = 2;   // sixteens of tokens worked on together
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Shares share;    // not held in registers over the tokens
@@ -308,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
             float big = 0.0f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int r = row + n * 8 + g;
-                const bool valid = r < req.rows;
+                const int r = row + n * 8 + (C == 1 ? g >> 1 : g);   // in column g
+                const bool valid = r < req.rows && (C == 2 || (g & 1) == 0);
                 const int query = valid ? QueryOf(p, r) : 0;
                 const uint16_t* from = static_cast<const uint16_t*>(p.q) + (req.first_row + static_cast<int64_t>(query)) * p.ldq +
                                        (static_cast<int64_t>(head) * p.group + r - query * p.group) * D;
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                 qsum[n][0] = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8);
                 qsum[n][1] = p.scale_log2 * __shfl_sync(0xffffffffu, sum, quad * 8 + 4);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < C; ++c) {
                     row_low[n][c] = __shfl_sync(0xffffffffu, low, quad * 8 + c * 4);
                     row_high[n][c] = __shfl_sync(0xffffffffu, high, quad * 8 + c * 4);
                 }
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < C; ++c) {
                 top[n][c] = sum[n][c] = mass[n][c] = offset[n][c] = 0.0f;
                 limit[n][c] = kNotStarted;
             }
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
+                            for (int c = 0; c < C; ++c) {
                                 float& score = z[s][n][2 * h + c];
                                 score = fmaf(ks, score, fmaf(km, qsum[n][c], -top[n][c]));
                             }
@@ -467,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                                for (int c = 0; c < 2; ++c) {
+                                for (int c = 0; c < C; ++c) {
                                     const bool seen = there && token >= row_low[n][c] && token < row_high[n][c];
                                     if (!seen) z[s][n][2 * h + c] = -INFINITY;
                                     any = any || seen;
@@ -485,14 +489,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < C; ++c)
 #pragma unroll
                         for (int s = 0; s < I; ++s) best[n][c] = fmaxf(best[n][c], fmaxf(z[s][n][c], z[s][n][2 + c]));
                 float biggest = __uint_as_float(scale_top);
                 if (!(biggest < INFINITY)) biggest = scale_limit;   // NaN: the weights show it
                 bool rescale = biggest > scale_limit;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) rescale = rescale || best[n][0] > limit[n][0] || best[n][1] > limit[n][1];
+                for (int n = 0; n < NT; ++n) rescale = rescale || best[n][0] > limit[n][0] || (C == 2 && best[n][1] > limit[n][1]);
                 if (__any_sync(0xffffffffu, rescale)) {
                     float change = 1.0f;
                     if (biggest > scale_limit) {
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                     for (int n = 0; n < NT; ++n) {
                         float moved[2], factor[2];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
+                        for (int c = 0; c < C; ++c) {
                             float m = best[n][c];
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -525,14 +529,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                         for (int m = 0; m < 2 * W; ++m) {
                             acc[n][m][0] *= factor[0];
-                            acc[n][m][1] *= factor[1];
                             acc[n][m][2] *= factor[0];
-                            acc[n][m][3] *= factor[1];
+                            if constexpr (C == 2) {
+                                acc[n][m][1] *= factor[1];
+                                acc[n][m][3] *= factor[1];
+                            }
                         }
 #pragma unroll
                         for (int s = 0; s < I; ++s)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) z[s][n][i] -= moved[i & 1];
+                            for (int i = 0; i < 4; i += 3 - C) z[s][n][i] -= moved[i & 1];
                     }
                 }
                 // probabilities, weights, weighted values
@@ -553,15 +559,17 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                             const float inverse = Reciprocal(vs[h]), ratio = vm[h] * inverse;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                const float p0 = Exp2(z[s][n][2 * h]), p1 = Exp2(z[s][n][2 * h + 1]);
+                                const float p0 = Exp2(z[s][n][2 * h]), p1 = C == 2 ? Exp2(z[s][n][2 * h + 1]) : 0.0f;
                                 mass[n][0] += p0;
-                                mass[n][1] += p1;
-                                const uint32_t packed = PackHalf(p0 * vs[h], p1 * vs[h]);
+                                const uint32_t packed = PackHalf(p0 * vs[h], C == 2 ? p1 * vs[h] : 0.0f);
                                 const float2 w = HalfPair<FTH_B200_FP16>(packed);
                                 sum[n][0] = fmaf(w.x, inverse, sum[n][0]);
-                                sum[n][1] = fmaf(w.y, inverse, sum[n][1]);
                                 offset[n][0] = fmaf(w.x, ratio, offset[n][0]);
-                                offset[n][1] = fmaf(w.y, ratio, offset[n][1]);
+                                if constexpr (C == 2) {
+                                    mass[n][1] += p1;
+                                    sum[n][1] = fmaf(w.y, inverse, sum[n][1]);
+                                    offset[n][1] = fmaf(w.y, ratio, offset[n][1]);
+                                }
                                 pt[n][h] = Transpose8x8(packed);
                             }
                         }
@@ -572,9 +580,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                         for (int h = 0; h < 2; ++h) {
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                float w[2];
+                                float w[2] = {};
 #pragma unroll
-                                for (int c = 0; c < 2; ++c) {
+                                for (int c = 0; c < C; ++c) {
                                     const float score = z[s][n][2 * h + c];
                                     const bool hidden = score == -INFINITY;
                                     const float prob = Exp2(score);
@@ -624,14 +632,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < C; ++c) {
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
                         sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o);
                         mass[n][c] += __shfl_xor_sync(0xffffffffu, mass[n][c], o);
                         offset[n][c] += __shfl_xor_sync(0xffffffffu, offset[n][c], o);
                     }
-                    float* out = join + static_cast<size_t>(warp * R + n * 8 + quad * 2 + c) * kRow<D>;
+                    float* out = join + static_cast<size_t>(warp * R + n * 8 + quad * C + c) * kRow<D>;
                     const float shift = offset[n][c];
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
@@ -745,15 +753,15 @@ size_t WorkspaceBytes(const fth_b200_kv4_attention_desc& d) {
 }
 
 template <int D, int DTYPE>
-int LaunchDecode(const AttentionParams& p, int tiles, int grid, cudaStream_t s) {
+int LaunchDecode(const AttentionParams& p, int tiles, bool four, int grid, cudaStream_t s) {
     const auto run = [&](auto kernel, size_t smem) {
         if (EnsureDynamicSmem(reinterpret_cast<const void*>(kernel), smem) != FTH_B200_OK) return static_cast<int>(FTH_B200_ERR_CUDA);
         return Launch(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, s, p);
     };
     if constexpr (D != 256) {
-        if (tiles == 2) return run(DecodeKernel<D, DTYPE, 2>, Layout<D, 2>::kBytes);
+        if (tiles == 2) return run(DecodeKernel<D, DTYPE, 2, 2>, Layout<D, 2>::kBytes);
     }
-    return run(DecodeKernel<D, DTYPE, 1>, Layout<D, 1>::kBytes);
+    return four ? run(DecodeKernel<D, DTYPE, 1, 1>, Layout<D, 1>::kBytes) : run(DecodeKernel<D, DTYPE, 1, 2>, Layout<D, 1>::kBytes);
 }
 
 }  // namespace
@@ -808,15 +816,18 @@ extern "C" int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* d, fth_
         if (status == FTH_B200_OK) NoteLaunch("kv4_attention_rows");
         return status;
     }
+    // units of four rows where no request has more: half of a score tile is left out then (40 requests of 3000 tokens, one row to a head,
+    // 16 heads of 64: 48.7 us, 45.3 us with four; 4 heads of 256: 43.1 and 39.9 us; one request of 200 thousand tokens: 64.4 and 66.5 us)
+    const bool four = kv4::MostRows(*d) <= 4;
     const int tiles = kv4::DecodeTiles(*d), grid = kv4::DecodeGrid(*d);
     if (d->dtype == FTH_B200_BF16) {
-        if (d->cache.head_dim == 64) status = kv4::LaunchDecode<64, FTH_B200_BF16>(p, tiles, grid, s);
-        else if (d->cache.head_dim == 128) status = kv4::LaunchDecode<128, FTH_B200_BF16>(p, tiles, grid, s);
-        else status = kv4::LaunchDecode<256, FTH_B200_BF16>(p, tiles, grid, s);
+        if (d->cache.head_dim == 64) status = kv4::LaunchDecode<64, FTH_B200_BF16>(p, tiles, four, grid, s);
+        else if (d->cache.head_dim == 128) status = kv4::LaunchDecode<128, FTH_B200_BF16>(p, tiles, four, grid, s);
+        else status = kv4::LaunchDecode<256, FTH_B200_BF16>(p, tiles, four, grid, s);
     } else {
-        if (d->cache.head_dim == 64) status = kv4::LaunchDecode<64, FTH_B200_FP16>(p, tiles, grid, s);
-        else if (d->cache.head_dim == 128) status = kv4::LaunchDecode<128, FTH_B200_FP16>(p, tiles, grid, s);
-        else status = kv4::LaunchDecode<256, FTH_B200_FP16>(p, tiles, grid, s);
+        if (d->cache.head_dim == 64) status = kv4::LaunchDecode<64, FTH_B200_FP16>(p, tiles, four, grid, s);
+        else if (d->cache.head_dim == 128) status = kv4::LaunchDecode<128, FTH_B200_FP16>(p, tiles, four, grid, s);
+        else status = kv4::LaunchDecode<256, FTH_B200_FP16>(p, tiles, four, grid, s);
     }
     if (status == FTH_B200_OK) NoteLaunch("kv4_attention");
     return status;
