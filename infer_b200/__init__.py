@@ -416,24 +416,23 @@ def _count(name, t, count):
         raise ValueError(f"{name} has {t.element_size()}-byte elements, needs 4")
 
 
-def _raw_stream(device):
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _call(name, desc, stream):
     """Runs an entry point with the descriptor's GPU current."""
     call = getattr(desc, "_call", None)
-    if call is None:  # the foreign function and its argument, looked up once per descriptor
+    if call is None:  # what every call of the descriptor needs, looked up once
         import torch
-        call = desc._call = (getattr(lib(), name), C.byref(desc), torch.cuda)
-    fn, arg, cuda = call
-    device = getattr(desc, "_device", None)
-    if device is None or cuda.current_device() == device:
-        code = fn(arg, stream or C.c_void_p(_raw_stream(device)))
+        fn = getattr(lib(), name)
+        fn.argtypes = [C.c_void_p, C.c_void_p]
+        # the current stream's handle without a Stream object, which costs as much as the launch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        call = desc._call = (fn, C.byref(desc), torch.cuda, raw)
+    fn, arg, cuda, raw = call
+    device, now = getattr(desc, "_device", None), cuda.current_device()
+    if device is None or now == device:
+        code = fn(arg, stream or raw(now))
     else:
         with cuda.device(device):
-            code = fn(arg, stream or C.c_void_p(_raw_stream(device)))
+            code = fn(arg, stream or raw(device))
     if code != OK:
         raise B200Error(code, name)
 

@@ -7,7 +7,7 @@ import pytest
 
 import infer_b200 as B
 from tests import kv4_plain as P
-from tests.test_gpu_kv4 import KINDS, attend, dtype_of, half_step, key_rounding, same, special_vectors
+from tests.test_gpu_kv4 import KINDS, SCALINGS, attend, dtype_of, half_step, key_rounding, make_rope, same, special_vectors
 
 pytestmark = pytest.mark.gpu
 
@@ -231,3 +231,76 @@ def test_ranges_at_the_end_of_the_numbers(cuda):
         a, b = (t.float() + 0.0 if "params" in n else t for t in (cache[n], want[n]))   # -0 is 0
         same(a, b)
     assert B.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("tokens,hq,hk,dim,rotary,layout", [(1301, 4, 2, 128, 128, "half"), (2500, 8, 2, 64, 32, "interleaved"), (4001, 0, 1, 256, 64, "half")])
+def test_many_turned_tokens_at_once(cuda, dtype, tokens, hq, hk, dim, rotary, layout):
+    """Blocks of several tokens, odd ones behind, rows without a slot: the bytes of the separate calls."""
+    torch = cuda
+    bs = 64
+    q, k, turns, amplitude = make_rope(torch, dtype, tokens, hq, hk, dim, rotary, layout, SCALINGS[0], None, seed=tokens)
+    v = torch.randn((tokens, hk, dim), device="cuda").to(k.dtype)
+    positions = torch.arange(5, 5 + tokens, device="cuda", dtype=torch.int32)
+    slots = torch.arange(1, 1 + tokens, device="cuda", dtype=torch.int32)
+    slots[100], positions[100], slots[tokens - 2] = -1, -1, -1
+    common = dict(dtype=KINDS[dtype], layout=B.ROPE_HALF if layout == "half" else B.ROPE_INTERLEAVED, tokens=tokens, head_dim=dim, rotary_dim=rotary,
+                  positions=positions, turns=turns, amplitude=amplitude, q_heads=hq, k_heads=hk, q=q if hq else None, k=k)
+    one, two = (P.new_cache(torch, P.blocks(tokens, bs) + 1, hk, bs, dim, seed=1) for _ in range(2))
+    qa, qb, kr = torch.full_like(q, 7.0), torch.full_like(q, 7.0), torch.zeros_like(k)
+    B.rope(B.rope_desc(q_out=qa if hq else None, k_out=kr, **common))
+    B.kv4_append(B.kv4_append_desc(cache=P.bind(B, one, bs), dtype=KINDS[dtype], tokens=tokens, k=kr, v=v, slots=slots))
+    fused = B.rope_desc(q_out=qb if hq else None, **common)
+    B.kv4_append(B.kv4_append_desc(cache=P.bind(B, two, bs), dtype=KINDS[dtype], tokens=tokens, k=k, v=v, slots=slots, rope=fused))
+    for n in one:
+        same(one[n], two[n])
+    same(qa, qb)
+    assert B.device_status() == 0
+
+
+@pytest.mark.parametrize("requests,grow", [(200, 1), (256, 2), (257, 2), (300, 1), (1024, 3), (1025, 7), (2100, 5)])
+def test_tables_of_every_block_size(cuda, requests, grow):
+    """Few threads, many threads, several blocks, more requests than a block has threads: assign, then release, against the plain
+    form; lengths in place."""
+    torch = cuda
+    rng = np.random.default_rng(requests)
+    cached = [int(n) for n in rng.integers(0, 60, requests)]
+    new = [int(n) for n in rng.integers(0, grow + 1, requests)]
+    bs, width = 16, 6
+    blocks = sum(P.blocks(c + n, bs) for c, n in zip(cached, new)) + 5
+    order = rng.permutation(blocks)
+    table = np.full((requests, width), -1, np.int32)
+    at = 0
+    for r, c in enumerate(cached):
+        held = P.blocks(c, bs)
+        table[r, :held] = order[at:at + held]
+        at += held
+    free = list(order[at:])
+    capacity = sum(new) + 3
+    i32 = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")  # noqa: E731
+    stack = np.zeros(blocks, np.int32)
+    stack[:len(free)] = free
+    lens, fresh, dtable, dfree, count = i32(cached), i32(new), i32(table), i32(stack), i32([len(free)])
+    starts, slots, positions, status = i32([0] * (requests + 1)), i32([7] * capacity), i32([7] * capacity), i32([0, 0])
+    B.kv4_assign(B.kv4_assign_desc(requests=requests, max_blocks=width, block_size=bs, blocks=blocks, tokens=capacity, cached_lens=lens, new_lens=fresh,
+                                   free_blocks=dfree, free_count=count, free_count_out=count, block_table=dtable, total_lens=lens, query_start=starts,
+                                   slots=slots, positions=positions, status=status))
+    want_slots, want_positions, left = [], [], len(free)
+    for r, (c, n) in enumerate(zip(cached, new)):
+        for j in range(P.blocks(c, bs), P.blocks(c + n, bs)):
+            left -= 1
+            table[r, j] = free[left]
+        want_positions += range(c, c + n)
+        want_slots += [int(table[r, t // bs]) * bs + t % bs for t in range(c, c + n)]
+    assert status.cpu().tolist() == [0, 0] and count.item() == left
+    assert lens.cpu().tolist() == [c + n for c, n in zip(cached, new)]
+    assert (dtable.cpu().numpy() == table).all() and starts.cpu().tolist() == [0] + np.cumsum(new).tolist()
+    assert slots.cpu().tolist() == want_slots + [-1] * 3 and positions.cpu().tolist() == want_positions + [-1] * 3
+    # half of the requests shrink, some to nothing
+    keep = [int(rng.integers(0, n + 1)) if r % 2 else n for r, n in enumerate(lens.cpu().tolist())]
+    now = lens.cpu().tolist()
+    B.kv4_release(B.kv4_release_desc(requests=requests, max_blocks=width, block_size=bs, blocks=blocks, lens=lens, keep_lens=i32(keep), free_blocks=dfree,
+                                     free_count=count, free_count_out=count, block_table=dtable, lens_out=lens, status=status))
+    back = [int(table[r, j]) for r in range(requests) for j in range(P.blocks(keep[r], bs), P.blocks(now[r], bs))]
+    assert status.cpu().tolist() == [0, 0] and count.item() == left + len(back) and lens.cpu().tolist() == keep
+    assert dfree.cpu().tolist()[left:left + len(back)] == back[::-1] and dfree.cpu().tolist()[:left] == [int(f) for f in free[:left]]
