@@ -7,7 +7,7 @@ Tolerances count roundings.  eps(t) / 2 is the largest relative error of one rou
 * attention: q and codes enter exactly, scores are FP32 sums of at most 256 products of both signs of the minimum and the
   code part.  With A = scale * sum |q| * (|min| + 15 s) the score is off by at most 2^-23 * (256 / 16 + 8) * A (the matrix
   instruction adds 16 products at a time and truncates, a unit of 2^-23 each time), which multiplies a probability by at most
-  1 + that; a probability (times its scale, with few rows) is rounded to 11 bits, 2^-12.  With more than 16 rows a kv head values enter
+  1 + that; a probability (times its scale, with few rows) is rounded to 11 bits, 2^-12.  With more than 128 rows a kv head values enter
   rounded to 11 bits, 2^-12 * |v| each, which the bound below holds room for (the probabilities' part is 2^-12 * |v| then, and
   |v| <= spread), and with BF16 queries the keys too: 2^-12 * A more on a score.  Weights off by a relative w each move a weighted mean
   of values by at most 2 w * mean(|v - out|) <= 2 w * spread, spread the largest |v - out|.  The sums over tokens add
@@ -317,7 +317,7 @@ def test_rope_in_the_append_launch(cuda, dtype, tokens, hq, hk, dim, rotary, lay
 
 
 def key_rounding(dtype, rows):
-    return 2.0 ** -12 if dtype == "bf16" and rows > 16 else 0.0
+    return 2.0 ** -12 if dtype == "bf16" and rows > 128 else 0.0
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------

@@ -4,7 +4,7 @@ single tokens, from one AttentionState.
 * One layer, step by step: every node that is not new is run again through its own entry point from the step's own buffers and
   gives the step's bytes; what is new (tables, cache contents, attention) is compared with the plain forms of kv4_plain.py.
   A row of attention is off by at most the limit that kv4_plain.attention derives (the kernels' arithmetic), half a BF16 step
-  (2^-8 of the value at most) and, with more than 16 rows to a key head, the keys' rounding to FP16.
+  (2^-8 of the value at most) and, with more than 128 rows to a key head, the keys' rounding to FP16.
 * Fused calls, node-by-node calls and replays of a captured step give the same bytes."""
 import ctypes as C
 
@@ -124,7 +124,7 @@ def test_steps_of_one_layer(cuda, hq, hk, dim, window, layout, fused):
         B.kv4_gather(B.kv4_gather_desc(cache=cache, dtype=B.FP32, tokens=rows, slots=step.slots, k_out=keys, v_out=values))
         (want_k, _), (want_v, _) = P.read(torch, mirror, bs, step.slots[:rows].long())
         assert torch.equal(keys, want_k.float()) and torch.equal(values, want_v.float())
-        many = step.max_query * (hq // hk) > 16
+        many = step.max_query * (hq // hk) > 128
         want, _, limit, _ = P.attention(torch, mirror, bs, state.table, bf16(torch, step.q_turned)[:rows], have, grow, hk, state.scale, True, window,
                                         key_rounding=2.0 ** -12 if many else 0.0)
         got = bf16(torch, step.attended)[:rows].double()
