@@ -83,6 +83,11 @@ __device__ __forceinline__ float ParamScale(uint32_t p) { return __uint_as_float
 __device__ __forceinline__ float ParamMin(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
 // ---- arithmetic ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float Reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // Two FP32 operations per instruction.
 __device__ __forceinline__ float2 Fma2(float2 a, float2 b, float2 c) {
     float2 d;

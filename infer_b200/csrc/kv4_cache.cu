@@ -8,7 +8,7 @@
 // eight elements are looked at again, in 64 bits, only if one's estimate is within 10^-4 of a half.
 // One pass over the data: 2 * tokens * kv_heads * head_dim * size bytes in, head_dim + 8 bytes per token and head out;
 // a launch for single tokens; for prompts reading back is bound by memory (16384 tokens of 8 heads of 128 in BF16: 23 us,
-// 3.6 TB/s) and storing by its arithmetic, some 400 instructions for four vectors (40 us, 2.1 TB/s).  A vector belongs to
+// 3.6 TB/s) and storing by its arithmetic, some 350 instructions for four vectors (36 us, 2.4 TB/s).  A vector belongs to
 // head_dim / 8 neighbouring lanes, eight elements each, so minimum and maximum are three to five shuffles (both in one word for
 // 16-bit types) and a lane's codes are one 32-bit word.
 #include <type_traits>
@@ -169,7 +169,7 @@ __device__ __forceinline__ uint32_t QuantiseEight(const Eight<DTYPE>& e, uint32_
     }
     const uint32_t scale_bits = ScaleBits(fminf(__fsub_ru(high, minimum), 3.402823466e38f));   // the largest scale reaches past 2^128
     const float scale = Bf16At(scale_bits);
-    const float inverse = scale_bits == 0 ? 0.0f : __fdiv_rn(1.0f, scale);
+    const float inverse = scale_bits == 0 ? 0.0f : Reciprocal(scale);   // scale < 2^125, so it is no subnormal
     *params = scale_bits | (min_bits << 16);
     // estimates are in [0, 15.0001]; added to 1.5 * 2^23 their nearest integers are the sum's last bits
     constexpr float kMagic = 12582912.0f;
@@ -241,12 +241,10 @@ __device__ __forceinline__ bool SharePairs(int slot0, int slot1) { return slot0 
 // hold two tokens, are written whole when the tokens are neighbours in the cache too.
 template <int DTYPE, int LANES>
 __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t first, int tokens, int start, int stride, const float2* angles) {
-    constexpr int kGroups = 32 / LANES;  // vectors a warp works on side by side
     const int lane = (threadIdx.x & 31) % LANES;
     const int heads = p.cache.kv_heads;
     PairWalk walk(tokens, p.two, heads, start / LANES, stride / LANES);
-    PairWalk warp_first(tokens, p.two, heads, start / 32 * kGroups, stride / LANES);   // of the warp's groups: the loop is the warp's
-    for (; warp_first.pair < warp_first.pairs; warp_first.Next(), walk.Next()) {
+    for (; __any_sync(0xffffffffu, walk.pair < walk.pairs); walk.Next()) {   // the loop is the warp's
         const int64_t row = walk.pair << p.two;
         const bool has0 = row < tokens, has1 = p.two != 0 && row + 1 < tokens;
         const bool is_key = walk.h2 < heads;
@@ -275,19 +273,23 @@ __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t fir
             good[j] = slots[j] >= 0 && slots[j] < p.slots_limit;
             if (slots[j] >= p.slots_limit && lane == 0) ReportTimeout(p.status, kSiteAppend, static_cast<int>(token + j));
         }
-        if (is_key) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (good[j]) StoreKey<LANES>(p.cache, slots[j], head, lane, codes[j], params[j]);
-        } else if (good[0] && good[1] && SharePairs(slots[0], slots[1])) {
+        if (good[0] && good[1] && SharePairs(slots[0], slots[1])) {
             const int64_t at = HeadBase(p.cache, slots[0] >> p.cache.block_shift, head) + (slots[0] & ((1 << p.cache.block_shift) - 1));
-            *reinterpret_cast<uint2*>(p.cache.v_codes + at * (LANES * 4) + lane * 8) =
-                make_uint2(__byte_perm(codes[0], codes[1], 0x5410), __byte_perm(codes[0], codes[1], 0x7632));
-            if (lane == 0) *reinterpret_cast<uint2*>(p.cache.v_params + at) = make_uint2(params[0], params[1]);
+            uint8_t* const to = (is_key ? p.cache.k_codes : p.cache.v_codes) + at * (LANES * 4);
+            if (is_key) {
+                *reinterpret_cast<uint32_t*>(to + lane * 4) = codes[0];
+                *reinterpret_cast<uint32_t*>(to + (LANES + lane) * 4) = codes[1];
+            } else {
+                *reinterpret_cast<uint2*>(to + lane * 8) = make_uint2(__byte_perm(codes[0], codes[1], 0x5410), __byte_perm(codes[0], codes[1], 0x7632));
+            }
+            if (lane == 0) *reinterpret_cast<uint2*>((is_key ? p.cache.k_params : p.cache.v_params) + at) = make_uint2(params[0], params[1]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (good[j]) StoreValue<LANES>(p.cache, slots[j], head, lane, codes[j], params[j]);
+            for (int j = 0; j < 2; ++j) {
+                if (!good[j]) continue;
+                if (is_key) StoreKey<LANES>(p.cache, slots[j], head, lane, codes[j], params[j]);
+                else StoreValue<LANES>(p.cache, slots[j], head, lane, codes[j], params[j]);
+            }
         }
     }
 }
@@ -447,7 +449,7 @@ template <int D, int L> struct RunGather {
 };
 
 // Two tokens at a time once one at a time would fill every SM twice over: 64 tokens of 8 heads of 128 are stored in 2.5 us one
-// at a time and 3.3 us in pairs, 16384 of them in 52 and 43 us (both are a tenth less by now), and read back in 35 and 23 us.
+// at a time and 3.3 us in pairs, 16384 of them in 52 and 43 us (36 us in pairs by now), and read back in 35 and 23 us.
 int TwoAtATime(int64_t threads) { return threads >= static_cast<int64_t>(SmCount()) * 2048 * 2 ? 1 : 0; }
 // No more blocks than run at once, `per_sm` on each SM: every thread walks on.
 unsigned SpreadBlocks(int64_t threads, int per_sm) {
