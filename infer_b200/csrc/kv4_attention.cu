@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                         }
                     }
                 }
-                // value scales of these tokens, as bits (positive numbers order like their bits; NaN counts as the largest)
+                // value scales of these tokens, as bits (positive numbers order like their bits; NaN comes out as the largest)
                 uint32_t scale_bits = v_params[place0 + lane] << 16;
                 if (!inside) {
                     bool lane_seen = false;   // of the token whose scale this lane holds
@@ -493,7 +493,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
 #pragma unroll
                         for (int s = 0; s < I; ++s) best[n][c] = fmaxf(best[n][c], fmaxf(z[s][n][c], z[s][n][2 + c]));
                 float biggest = __uint_as_float(scale_top);
-                if (!(biggest < INFINITY)) biggest = scale_limit;   // NaN: the weights show it
+                // a scale that is no number spoils the rows that see its token, through their weights; the others' weights need the
+                // largest scale beside it
+                if (!(biggest < INFINITY)) biggest = __uint_as_float(__reduce_max_sync(0xffffffffu, scale_bits < 0x7f800000u ? scale_bits : 0u));
                 bool rescale = biggest > scale_limit;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) rescale = rescale || best[n][0] > limit[n][0] || (C == 2 && best[n][1] > limit[n][1]);
