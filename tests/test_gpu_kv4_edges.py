@@ -44,3 +44,31 @@ def test_large_values_beside_a_spoiled_one(cuda, dim, length, rows):
     take the others at their size."""
     attend(cuda, dtype="bf16", lens=[length], new=[rows], hq=1, hk=1, dim=dim, bs=16, seed=rows, mutate=spoil_value(length - 1),
            v_gain=lambda torch, n: torch.where(torch.arange(n, device="cuda") >= n - 32, 2.0 ** 14, 1.0))
+
+
+# ---- rows ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,tokens", [([5, 2, 7], 10), ([5, 2, 7], 6), ([5, 2, 7], 3), ([90, 10, 40], 120), ([90, 10, 40], 70)])
+@pytest.mark.parametrize("window", [0, 60])
+def test_rows_behind_tokens_are_left_and_the_others_keep_their_positions(cuda, new, tokens, window):
+    """query_start goes beyond `tokens`: row i of n stands at total - n + i all the same."""
+    torch = cuda
+    hq, hk, dim, bs, lens = 8, 2, 128, 16, [300, 50, 129]
+    r = attend(torch, dtype="bf16", lens=lens, new=new, hq=hq, hk=hk, dim=dim, bs=bs, seed=1, window=window)
+    d = r["desc"]
+    d.tokens = tokens
+    r["out"].fill_(7.0)
+    r["lse"].fill_(7.0)
+    B.kv4_attention(d)
+    at = 0
+    for i, n in enumerate(new):
+        kept = max(min(n, tokens - at), 0)
+        if kept:
+            q = r["q"][at:at + kept].reshape(kept, hq, dim)
+            want, want_lse, limit, limit_lse = P.attention(torch, r["cache"], bs, r["table"][i:i + 1], q, [lens[i] - (n - kept)], [kept], hk, d.scale, True,
+                                                           window, key_rounding=key_rounding("bf16", d.max_query * hq // hk))
+            got = r["out"][at:at + kept].reshape(kept, hq, dim).double()
+            assert ((got - want).abs() <= limit + 2.0 ** -8 * want.abs() + 1e-30).all()
+            assert ((r["lse"][at:at + kept].double() - want_lse).abs() <= limit_lse).all()
+        at += n
+    assert (r["out"][tokens:] == 7.0).all() and (r["lse"][tokens:] == 7.0).all()
+    assert B.device_status() == 0
