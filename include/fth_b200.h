@@ -564,7 +564,7 @@ int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* desc, fth_b200_stream_t 
  * The result does not depend on what else is in the batch only up to FP32 summation order; it is the same from run to run.
  * workspace: device, 256-byte aligned, zero-filled once after allocation, left ready for the next call; calls that share
  * one must not overlap.  fth_b200_kv4_attention_workspace_bytes depends on requests, tokens, max_query, heads and the
- * cache's geometry only. */
+ * cache's geometry only, and not less for a larger max_query: the largest step's workspace serves the smaller ones. */
 typedef struct {
     fth_b200_kv4_cache cache;
     int32_t dtype;       /* FP16 or BF16: q and out */

@@ -737,21 +737,24 @@ int64_t MostRows(const fth_b200_kv4_attention_desc& d) { return static_cast<int6
 // heads leave no registers for them (20 rows: 69 us, 42 us in eights).
 int DecodeTiles(const fth_b200_kv4_attention_desc& d) { return d.cache.head_dim != 256 && (MostRows(d) + 7) / 8 % 2 == 0 ? 2 : 1; }
 // Blocks of threads that are resident together.
-int DecodeGrid(const fth_b200_kv4_attention_desc& d) {
-    const int per_sm = d.cache.head_dim == 256 || DecodeTiles(d) == 2 ? kBlocksPerSm<256, 1> : kBlocksPerSm<128, 1>;
+int DecodeGrid(int head_dim, int tiles) {
+    const int per_sm = head_dim == 256 || tiles == 2 ? kBlocksPerSm<256, 1> : kBlocksPerSm<128, 1>;
     const int grid = SmCount() * per_sm;
     return grid < kMaxGrid ? grid : kMaxGrid;
 }
-
 
 // The kernel with 128-row tiles.  It unpacks as much for a row as for 256, and its tiles start late: those 12 requests of 2 kv heads of 128
 // take it 56, 83 and 124 us with 20, 64 and 128 rows, eights and sixteens 27, 44 and 73 us; 256-wide heads 76, 108 and 154 us against
 // 42, 80 and 142 us.
 bool ManyRows(const fth_b200_kv4_attention_desc& d) { return MostRows(d) > 128; }
 
+// What a call with these or fewer rows needs, so that the largest step's workspace serves all: units of sixteen rows, in fewer blocks of
+// threads, need more than the units of eight that some larger steps have.
 size_t WorkspaceBytes(const fth_b200_kv4_attention_desc& d) {
     if (ManyRows(d)) return kCounterBytes + static_cast<size_t>(PrefillPartialFloats(d.cache.head_dim)) * sizeof(float);
-    return kCounterBytes + static_cast<size_t>(DecodeGrid(d)) * 2 * 8 * DecodeTiles(d) * (d.cache.head_dim + 4) * sizeof(float);
+    const auto need = [&](int tiles) { return static_cast<size_t>(DecodeGrid(d.cache.head_dim, tiles)) * 2 * 8 * tiles * (d.cache.head_dim + 4) * sizeof(float); };
+    const size_t eights = need(1), sixteens = d.cache.head_dim != 256 && MostRows(d) > 8 ? need(2) : 0;
+    return kCounterBytes + (eights > sixteens ? eights : sixteens);
 }
 
 template <int D, int DTYPE>
@@ -821,7 +824,7 @@ extern "C" int fth_b200_kv4_attention(const fth_b200_kv4_attention_desc* d, fth_
     // units of four rows where no request has more: half of a score tile is left out then (40 requests of 3000 tokens, one row to a head,
     // 16 heads of 64: 48.7 us, 45.3 us with four; 4 heads of 256: 43.1 and 39.9 us; one request of 200 thousand tokens: 64.4 and 66.5 us)
     const bool four = kv4::MostRows(*d) <= 4;
-    const int tiles = kv4::DecodeTiles(*d), grid = kv4::DecodeGrid(*d);
+    const int tiles = kv4::DecodeTiles(*d), grid = kv4::DecodeGrid(d->cache.head_dim, tiles);
     if (d->dtype == FTH_B200_BF16) {
         if (d->cache.head_dim == 64) status = kv4::LaunchDecode<64, FTH_B200_BF16>(p, tiles, four, grid, s);
         else if (d->cache.head_dim == 128) status = kv4::LaunchDecode<128, FTH_B200_BF16>(p, tiles, four, grid, s);

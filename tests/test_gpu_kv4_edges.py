@@ -72,3 +72,18 @@ def test_rows_behind_tokens_are_left_and_the_others_keep_their_positions(cuda, n
         at += n
     assert (r["out"][tokens:] == 7.0).all() and (r["lse"][tokens:] == 7.0).all()
     assert B.device_status() == 0
+
+
+# ---- workspaces ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_the_workspace_of_the_largest_step_serves_smaller_ones(cuda, dim):
+    torch = cuda
+    big = attend(torch, dtype="bf16", lens=[5000, 90], new=[20, 20], hq=2, hk=2, dim=dim, bs=16, seed=2)
+    for rows in (16, 9, 1):
+        r = attend(torch, dtype="bf16", lens=[5000, 90], new=[rows, 1], hq=2, hk=2, dim=dim, bs=16, seed=3)
+        want = r["out"].clone()
+        r["out"].fill_(7.0)
+        r["desc"].workspace, r["desc"].workspace_bytes = big["ws"].data_ptr(), big["ws"].numel()
+        B.kv4_attention(r["desc"])
+        same(r["out"], want)
+    assert B.device_status() == 0
