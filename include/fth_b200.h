@@ -475,7 +475,8 @@ typedef struct {
  * A step that does not fit is refused as a whole, on the device: status[0] = FTH_B200_KV4_*, nothing is taken, total_lens =
  * cached_lens (0 where that is negative), query_start all 0, slots and positions all -1.
  * In place: total_lens may be cached_lens, free_count_out may be free_count.  status: two words, zero-filled once. */
-enum { FTH_B200_KV4_OK = 0, FTH_B200_KV4_NO_BLOCKS = 1, FTH_B200_KV4_TABLE_FULL = 2, FTH_B200_KV4_TOO_MANY_TOKENS = 3, FTH_B200_KV4_BAD_LENGTH = 4 };
+enum { FTH_B200_KV4_OK = 0, FTH_B200_KV4_NO_BLOCKS = 1, FTH_B200_KV4_TABLE_FULL = 2, FTH_B200_KV4_TOO_MANY_TOKENS = 3, FTH_B200_KV4_BAD_LENGTH = 4,
+       FTH_B200_KV4_BAD_BLOCK = 5 };
 typedef struct {
     int32_t requests;
     int32_t max_blocks;   /* row length of block_table */
@@ -499,7 +500,9 @@ int fth_b200_kv4_assign(const fth_b200_kv4_assign_desc* desc, fth_b200_stream_t 
 /* Gives blocks back: request r shrinks from lens[r] to keep_lens[r] tokens (0: done; less than lens: rejected drafts).
  * Blocks that hold none of the kept tokens go on the stack so that releasing what the last fth_b200_kv4_assign took
  * restores it.  block_table is only read; lens_out (may be lens) = keep_lens.  Refused as a whole with BAD_LENGTH (negative,
- * or keep > lens), TABLE_FULL (lens beyond the row) or NO_BLOCKS (more free blocks than there are); lens_out = lens then. */
+ * or keep > lens), TABLE_FULL (lens beyond the row), NO_BLOCKS (more free blocks than there are) or BAD_BLOCK (an entry to be
+ * given back is no block); lens_out = lens and the stack is as it was then, but for free_blocks behind free_count with BAD_BLOCK.
+ * That a block is not given back twice is the caller's to see to. */
 typedef struct {
     int32_t requests;
     int32_t max_blocks;

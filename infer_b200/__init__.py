@@ -43,7 +43,7 @@ EXPORTS = [
 BINARY_ADD, BINARY_MUL = 0, 1
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "banded": 4}
-KV4_OK, KV4_NO_BLOCKS, KV4_TABLE_FULL, KV4_TOO_MANY_TOKENS, KV4_BAD_LENGTH = 0, 1, 2, 3, 4
+KV4_OK, KV4_NO_BLOCKS, KV4_TABLE_FULL, KV4_TOO_MANY_TOKENS, KV4_BAD_LENGTH, KV4_BAD_BLOCK = 0, 1, 2, 3, 4, 5
 
 
 class Fp8LinearDesc(C.Structure):

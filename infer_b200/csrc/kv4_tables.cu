@@ -8,7 +8,8 @@
 // memory, so that one long prompt spreads over the chip like many short ones.  64 requests with a new token each: 3.2 us a
 // launch; 1000 with up to 400: 7 us.
 // What may be updated in place (lengths, the free count) is written by the block that finishes last: by then every
-// block has read it.  The ticket that finds the last block is integer and its order does not reach the results.
+// block has read it.  The ticket that finds the last block is integer and its order does not reach the results.  Entries of
+// the table that are no blocks are found while they are copied, and refuse the release when that block finishes.
 #include "kv4.cuh"
 
 namespace fth {
@@ -98,18 +99,22 @@ __device__ __forceinline__ void Share(int64_t count, int64_t* first, int64_t* la
     *last = count * (blockIdx.x + 1) / gridDim.x;
 }
 
-// True in the block that arrives last (all its threads).
-__device__ __forceinline__ bool ArriveLast(int32_t* status) {
-    __shared__ int last;
-    __syncthreads();
-    if (gridDim.x == 1) return true;
+// Arrivals of a launch's blocks of threads.  kNot: others are still to come; else this block is the last one (kLast), and one of
+// them brought a bad mark (kLastBad).  All threads of a block get the same; `bad` may differ among them.
+enum Arrival { kNot, kLast, kLastBad };
+__device__ __forceinline__ Arrival Arrive(int32_t* status, bool bad) {
+    __shared__ Arrival result;
+    const bool mine = __syncthreads_or(bad ? 1 : 0) != 0;
+    if (gridDim.x == 1) return mine ? kLastBad : kLast;
     if (threadIdx.x == 0) {
         __threadfence();
-        last = atomicAdd(&status[1], 1) == static_cast<int>(gridDim.x) - 1;
-        if (last) status[1] = 0;
+        // arrivals in the low half, bad marks in the high one: both up to gridDim.x
+        const int before = atomicAdd(&status[1], mine ? 0x10001 : 1);
+        result = (before & 0xffff) != static_cast<int>(gridDim.x) - 1 ? kNot : mine || (before >> 16) != 0 ? kLastBad : kLast;
+        if (result != kNot) status[1] = 0;
     }
     __syncthreads();
-    return last != 0;
+    return result;
 }
 
 template <int kThreads>
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) AssignKernel(const __grid_constant__
         p.slots[i] = -1;
         p.positions[i] = -1;
     }
-    if (!ArriveLast(p.status)) return;
+    if (Arrive(p.status, false) == kNot) return;
     for (int r = threadIdx.x; r < p.requests; r += kThreads) {
         const int c = p.cached[r];
         p.total_lens[r] = refused == FTH_B200_KV4_OK ? c + p.fresh[r] : (c < 0 ? 0 : c);
@@ -257,6 +262,7 @@ __global__ void __launch_bounds__(kThreads) ReleaseKernel(const __grid_constant_
     if (flags & 1) refused = FTH_B200_KV4_BAD_LENGTH;
     else if (flags & 2) refused = FTH_B200_KV4_TABLE_FULL;
     else if (free_count < 0 || free_count + back > p.blocks) refused = FTH_B200_KV4_NO_BLOCKS;
+    bool bad = false;   // an entry that is no block
     if (refused == FTH_B200_KV4_OK) {
         int64_t mine_first, mine_last;
         Share(back, &mine_first, &mine_last);
@@ -282,13 +288,17 @@ __global__ void __launch_bounds__(kThreads) ReleaseKernel(const __grid_constant_
             const int hi = static_cast<int>((mine_last < before + here ? mine_last : before + here) - before);
             for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
                 const int at = Find(back_start, count, i);
-                p.free_blocks[free_count + back - 1 - (before + i)] =
-                    p.table[static_cast<int64_t>(base + at) * p.max_blocks + first_s[at] + i - back_start[at]];
+                const int block = p.table[static_cast<int64_t>(base + at) * p.max_blocks + first_s[at] + i - back_start[at]];
+                bad = bad || block < 0 || block >= p.blocks;
+                p.free_blocks[free_count + back - 1 - (before + i)] = block;
             }
             before += here;
         }
     }
-    if (!ArriveLast(p.status)) return;
+    // What has been written stands behind the stack's top, which moves only now.
+    const Arrival arrival = Arrive(p.status, bad);
+    if (arrival == kNot) return;
+    if (arrival == kLastBad) refused = FTH_B200_KV4_BAD_BLOCK;
     for (int r = threadIdx.x; r < p.requests; r += kThreads) p.lens_out[r] = refused == FTH_B200_KV4_OK ? p.keep[r] : p.lens[r];
     if (threadIdx.x == 0) {
         *p.free_count_out = refused == FTH_B200_KV4_OK ? static_cast<int>(free_count + back) : free_count;

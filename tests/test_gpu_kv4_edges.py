@@ -87,3 +87,44 @@ def test_the_workspace_of_the_largest_step_serves_smaller_ones(cuda, dim):
         B.kv4_attention(r["desc"])
         same(r["out"], want)
     assert B.device_status() == 0
+
+
+# ---- tables -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("requests,width", [(3, 8), (250, 2), (300, 4), (1100, 6), (600, 300)])
+@pytest.mark.parametrize("bad", [-1, "blocks", 1 << 30])
+def test_release_refuses_a_table_entry_that_is_no_block(cuda, requests, width, bad):
+    """One block of few threads, one of many, several blocks, more requests than a block has threads; the entry in the first, the
+    last or a middle request, at the begin or the end of what comes back.  The stack keeps its blocks; an entry among the kept
+    tokens is not looked at."""
+    torch = cuda
+    bs, held = 16, width - 1
+    blocks = requests * width + 5
+    i32 = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.full((requests, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :held] = torch.randperm(requests * held, device="cuda").to(torch.int32).view(requests, held)
+    good = table.clone()
+    spare = blocks - requests * held
+    lens, keep = i32([held * bs] * requests), i32([bs // 2] * requests)   # the first block stays
+    keep[0] = 0
+    status = i32([0, 0])
+
+    def release():
+        free = torch.full((blocks,), -7, dtype=torch.int32, device="cuda")
+        free[:spare] = torch.arange(requests * held, blocks, device="cuda", dtype=torch.int32)
+        count, now = i32([spare]), lens.clone()
+        B.kv4_release(B.kv4_release_desc(requests=requests, max_blocks=width, block_size=bs, blocks=blocks, lens=now, keep_lens=keep, free_blocks=free,
+                                         free_count=count, free_count_out=count, block_table=table, lens_out=now, status=status))
+        return free, count, now
+    start = torch.arange(requests * held, blocks, device="cuda", dtype=torch.int32)
+    if held > 1:
+        for r, j in ((0, 0), (requests - 1, held - 1), (requests // 2, 1)):
+            table[r, j] = blocks if bad == "blocks" else bad
+            free, count, now = release()
+            assert status.cpu().tolist() == [B.KV4_BAD_BLOCK, 0]
+            assert count.item() == spare and torch.equal(free[:spare], start) and torch.equal(now, lens)
+            table.copy_(good)
+    table[requests - 1, 0] = table[requests // 2, held] = -3   # held by the tokens that stay; behind the last token
+    free, count, now = release()
+    back = torch.cat([good[0, :held], good[1:, 1:held].reshape(-1)])
+    assert status.cpu().tolist() == [0, 0] and count.item() == spare + back.numel() and torch.equal(now, keep)
+    assert torch.equal(free[:spare], start) and torch.equal(free[spare:spare + back.numel()], back.flip(0))
