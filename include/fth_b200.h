@@ -523,7 +523,8 @@ int fth_b200_kv4_release(const fth_b200_kv4_release_desc* desc, fth_b200_stream_
  * negative slot skips the row; a slot beyond the cache skips it and is reported through fth_b200_device_status (site 40).
  * The slots of one call differ from each other.  With `rope` (its k_heads = kv_heads, k = this k, same tokens, dtype and
  * head_dim; k_out must be null; q optional) keys are turned before they are stored and q in the same launch; the cache
- * and q_out receive the bytes of fth_b200_rope followed by fth_b200_kv4_append. */
+ * and q_out receive the bytes of fth_b200_rope (of the keys in place) followed by fth_b200_kv4_append: a key at a negative position
+ * is stored as it is. */
 typedef struct {
     fth_b200_kv4_cache cache;
     int32_t dtype; /* FP32, FP16 or BF16 */

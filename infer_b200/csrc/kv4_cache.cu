@@ -251,12 +251,14 @@ __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t fir
         const int head = is_key ? walk.h2 : walk.h2 - heads;
         const int64_t token = first + row;
         const int slots[2] = {has0 ? p.slots[token] : -1, has1 ? p.slots[token + 1] : -1};
-                Eight<DTYPE> x[2] = {};
+        // a negative position: the row is not turned, its key is stored as it is
+        const bool turned[2] = {is_key && p.turn && has0 && p.rope.positions[token] >= 0, is_key && p.turn && has1 && p.rope.positions[token + 1] >= 0};
+        Eight<DTYPE> x[2] = {};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (!(j == 0 ? has0 : has1)) continue;
             const int64_t at = (token + j) * (is_key ? p.ldk : p.ldv) + static_cast<int64_t>(head) * (LANES * 8);
-            if (is_key && p.turn) {
+            if (turned[j]) {
                 float v[8];
                 RopeEight<DTYPE>(p.rope, p.k, at, lane * 8, angles + (row + j) * (p.rope.rotary_dim >> 1), p.vec_k != 0, v);
                 x[j].Set(v);

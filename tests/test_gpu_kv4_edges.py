@@ -128,3 +128,32 @@ def test_release_refuses_a_table_entry_that_is_no_block(cuda, requests, width, b
     back = torch.cat([good[0, :held], good[1:, 1:held].reshape(-1)])
     assert status.cpu().tolist() == [0, 0] and count.item() == spare + back.numel() and torch.equal(now, keep)
     assert torch.equal(free[:spare], start) and torch.equal(free[spare:spare + back.numel()], back.flip(0))
+
+
+# ---- storing ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("tokens,layout,rotary", [(6, "half", 128), (6, "interleaved", 48), (6, "half", 20), (1301, "half", 128)])
+def test_a_negative_position_with_a_slot(cuda, dtype, tokens, layout, rotary):
+    """The row is not turned: its key is stored as it is, as by fth_b200_rope in place and fth_b200_kv4_append; q is left."""
+    torch = cuda
+    hq, hk, dim, bs = 4, 2, 128, 16
+    q, k, turns, amplitude = make_rope(torch, dtype, tokens, hq, hk, dim, rotary, layout, SCALINGS[3], None, seed=tokens)
+    k[4] = k[4].abs() * (torch.arange(hk * dim, device="cuda") % 3).to(k.dtype) * -0.0   # zeros of both signs: a sign is a byte's too
+    k[4, ::2] *= -1.0
+    v = torch.randn((tokens, hk, dim), device="cuda").to(k.dtype)
+    positions = torch.arange(100, 100 + tokens, device="cuda", dtype=torch.int32)
+    positions[1], positions[4], positions[tokens - 1] = -1, -(1 << 31), -77
+    slots = torch.arange(3, 3 + tokens, device="cuda", dtype=torch.int32)
+    common = dict(dtype=KINDS[dtype], layout=B.ROPE_HALF if layout == "half" else B.ROPE_INTERLEAVED, tokens=tokens, head_dim=dim, rotary_dim=rotary,
+                  positions=positions, turns=turns, amplitude=amplitude, q_heads=hq, k_heads=hk, q=q)
+    one, two = (P.new_cache(torch, P.blocks(tokens, bs) + 1, hk, bs, dim, seed=1) for _ in range(2))
+    qa, qb, kr = torch.full_like(q, 7.0), torch.full_like(q, 7.0), k.clone()
+    B.rope(B.rope_desc(q_out=qa, k=kr, k_out=kr, **common))
+    assert torch.equal(kr[1], k[1])
+    B.kv4_append(B.kv4_append_desc(cache=P.bind(B, one, bs), dtype=KINDS[dtype], tokens=tokens, k=kr, v=v, slots=slots))
+    B.kv4_append(B.kv4_append_desc(cache=P.bind(B, two, bs), dtype=KINDS[dtype], tokens=tokens, k=k, v=v, slots=slots,
+                                   rope=B.rope_desc(q_out=qb, k=k, **common)))
+    for n in one:
+        same(one[n], two[n])
+    same(qa, qb)
+    assert (qa[1] == 7.0).all() and B.device_status() == 0
