@@ -65,8 +65,13 @@ int fth_b200_abi_version(void);
 /* Name of the kernel family the last call on this host thread launched ("skinny", "tcgen05", "simt", …);
  * the counterpart of LastCudaFp8MatmulBackend() (src/kernel/cuda/runtime.h:141-143). */
 const char* fth_b200_last_variant(void);
-/* Reads and clears the per-device status word (synchronises the device): 0 when no bounded device-side wait
- * ever gave up, else (site << 16) | detail of the first that did. */
+/* Reads and clears the per-device status word (synchronises the device): 0 when no bounded device-side wait ever gave up and no
+ * call met a slot or block number outside its cache, else (site << 16) | detail of the first of these.
+ *   40   a peer's flag did not come; detail: the rank.  With bit 15 of the detail: fth_b200_kv4_append met a slot beyond the
+ *        cache; the lower bits: the row's, modulo 2^15
+ *   41   a peer's previous step did not end; detail: the rank.  With bit 15: the same slot in fth_b200_kv4_gather
+ *   42   fth_b200_kv4_attention met a block number outside the cache; detail: the request, modulo 2^16
+ *   others: a wait inside a kernel */
 int fth_b200_device_status(void);
 /* Kernels launched by this library on this host thread since the last reset. */
 int64_t fth_b200_launch_count(void);
@@ -520,7 +525,8 @@ typedef struct {
 int fth_b200_kv4_release(const fth_b200_kv4_release_desc* desc, fth_b200_stream_t stream);
 
 /* Stores k and v [tokens, kv_heads, head_dim] (heads head_dim apart, row strides ldk / ldv, 0: dense) at slots[t].  A
- * negative slot skips the row; a slot beyond the cache skips it and is reported through fth_b200_device_status (site 40).
+ * negative slot skips the row; a slot beyond the cache skips it and is reported through fth_b200_device_status (site 40,
+ * bit 15 of the detail).
  * The slots of one call differ from each other.  With `rope` (its k_heads = kv_heads, k = this k, same tokens, dtype and
  * head_dim; k_out must be null; q optional) keys are turned before they are stored and q in the same launch; the cache
  * and q_out receive the bytes of fth_b200_rope (of the keys in place) followed by fth_b200_kv4_append: a key at a negative position
@@ -537,7 +543,7 @@ typedef struct {
 } fth_b200_kv4_append_desc;
 int fth_b200_kv4_append(const fth_b200_kv4_append_desc* desc, fth_b200_stream_t stream);
 /* Reads slots back as values, rounded once to dtype: k_out, v_out [tokens, kv_heads, head_dim], row strides ldk / ldv;
- * either may be null.  Rows with a negative slot (or one beyond the cache, reported as site 41) are left as they were. */
+ * either may be null.  Rows with a negative slot (or one beyond the cache, reported as site 41, bit 15) are left as they were. */
 typedef struct {
     fth_b200_kv4_cache cache;
     int32_t dtype;

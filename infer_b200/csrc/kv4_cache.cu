@@ -24,7 +24,11 @@ using namespace rowops;
 
 constexpr int kThreads = 256;
 constexpr int kAppendBlocks = 4, kGatherBlocks = 6;   // on an SM at once
-constexpr int kSiteAppend = 40, kSiteGather = 41;
+// Waits for a rank report under the same two sites; kBadSlot in the detail, which no rank reaches, tells a slot beyond the cache.
+constexpr int kSiteAppend = 40, kSiteGather = 41, kBadSlot = 0x8000;
+__device__ __forceinline__ void ReportSlot(int* status, int site, int64_t token) {
+    ReportTimeout(status, site, kBadSlot | static_cast<int>(token & (kBadSlot - 1)));
+}
 
 struct AppendParams {
     Cache cache;
@@ -273,7 +277,7 @@ __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t fir
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             good[j] = slots[j] >= 0 && slots[j] < p.slots_limit;
-            if (slots[j] >= p.slots_limit && lane == 0) ReportTimeout(p.status, kSiteAppend, static_cast<int>(token + j));
+            if (slots[j] >= p.slots_limit && lane == 0) ReportSlot(p.status, kSiteAppend, token + j);
         }
         if (good[0] && good[1] && SharePairs(slots[0], slots[1])) {
             const int64_t at = HeadBase(p.cache, slots[0] >> p.cache.block_shift, head) + (slots[0] & ((1 << p.cache.block_shift) - 1));
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, kGatherBlocks) GatherKernel(const __
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             good[j] = slots[j] >= 0 && slots[j] < p.slots_limit;
-            if (slots[j] >= p.slots_limit && lane == 0) ReportTimeout(p.status, kSiteGather, static_cast<int>(token + j));
+            if (slots[j] >= p.slots_limit && lane == 0) ReportSlot(p.status, kSiteGather, token + j);
             base[j] = good[j] ? HeadBase(p.cache, slots[j] >> p.cache.block_shift, head) : 0;
             offset[j] = good[j] ? slots[j] & ((1 << p.cache.block_shift) - 1) : 0;
             codes[j] = params[j] = 0;

@@ -81,8 +81,8 @@ bool MakeTensorMap4D(CUtensorMap* map, const void* base, const uint64_t dims_[4]
 
 }  // namespace fth
 
-// Reads and clears the device status word (synchronises the device).  0 = no bounded wait ever gave up;
-// otherwise (site << 16) | detail of the first one that did.
+// Reads and clears the device status word (synchronises the device).  0 = no bounded wait ever gave up and no number that
+// addresses the cache was out of its range; otherwise (site << 16) | detail of the first that did or was.
 extern "C" int fth_b200_device_status(void) {
     int value = 0;
     int* ptr = fth::DeviceStatusPtr();

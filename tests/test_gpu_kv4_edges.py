@@ -157,3 +157,18 @@ def test_a_negative_position_with_a_slot(cuda, dtype, tokens, layout, rotary):
         same(one[n], two[n])
     same(qa, qb)
     assert (qa[1] == 7.0).all() and B.device_status() == 0
+
+
+def test_the_status_of_a_bad_slot_is_no_wait_for_a_peer(cuda):
+    """Sites 40 and 41 are also those of waits for a rank (detail: the rank, below 2^15); a slot beyond the cache sets bit 15 of the detail."""
+    torch = cuda
+    cache = P.bind(B, P.new_cache(torch, 2, 1, 16, 64, seed=1), 16)
+    k = torch.randn((40003, 1, 64), device="cuda", dtype=torch.bfloat16)
+    slots = torch.full((40003,), -1, dtype=torch.int32, device="cuda")
+    for token in (0, 1, 40002):
+        slots.fill_(-1)
+        slots[token] = 32
+        B.kv4_append(B.kv4_append_desc(cache=cache, dtype=B.BF16, tokens=40003, k=k, v=k, slots=slots))
+        assert B.device_status() == (40 << 16 | 0x8000 | token & 0x7fff)
+        B.kv4_gather(B.kv4_gather_desc(cache=cache, dtype=B.BF16, tokens=40003, slots=slots, k_out=k))
+        assert B.device_status() == (41 << 16 | 0x8000 | token & 0x7fff)
