@@ -9,8 +9,8 @@ namespace kv4 {
 
 constexpr int kSiteAttention = 42, kSiteAttentionWait = 43;
 constexpr float kLazy = 8.0f;     // a running maximum may lag by 2^8 before sums are rescaled
-constexpr float kNotStarted = -3e38f;
-constexpr float kNoMax = -1e30f;  // the maximum of no scores: below all, and finite, so that differences stay numbers
+constexpr float kNotStarted = -INFINITY;
+constexpr float kNoMax = -3.402823466e38f;  // the maximum of no scores: not above any, and finite, so that kNoMax - kNoMax is 0
 
 struct AttentionParams {
     Cache cache;

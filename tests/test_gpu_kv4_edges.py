@@ -172,3 +172,41 @@ def test_the_status_of_a_bad_slot_is_no_wait_for_a_peer(cuda):
         assert B.device_status() == (40 << 16 | 0x8000 | token & 0x7fff)
         B.kv4_gather(B.kv4_gather_desc(cache=cache, dtype=B.BF16, tokens=40003, slots=slots, k_out=k))
         assert B.device_status() == (41 << 16 | 0x8000 | token & 0x7fff)
+
+
+# ---- scores at the end of the numbers ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,length", [(1, 1), (1, 5000), (12, 3), (200, 1), (200, 5000)])
+def test_rows_whose_scores_are_far_below_zero(cuda, dtype, dim, rows, length):
+    """All tokens have one key and one value, and the key's product with every row is about -2^105.  FP32 scores of that size are 2^82
+    apart, so the weights are whatever the last bit makes them, but the value comes out: FP16 weights or probabilities are off by 2^-12
+    each, and values by 2^-12, of |v| <= 5, FP32 sums by 2^-23 * (tokens / 16 + 8) of it.  The lse is off by a score's FP32
+    roundings: its two parts (minimum and codes) are up to 15 times as large, and BF16 rows take keys rounded to 2^-12."""
+    torch = cuda
+    dt, bs = dtype_of(torch, dtype), 64
+    blocks = P.blocks(length, bs)
+    cache = P.new_cache(torch, blocks, 1, bs, dim, seed=1)
+    gen = torch.Generator(device="cuda").manual_seed(rows + dim)
+    key = torch.rand(dim, generator=gen, device="cuda") + 1.0
+    k = key.expand(length, 1, dim).to(dt).contiguous()
+    v = torch.randn((1, 1, dim), generator=gen, device="cuda").clamp(-5, 5).to(dt).expand(length, 1, dim).contiguous()
+    slots = torch.arange(length, device="cuda", dtype=torch.int32)
+    P.append(torch, cache, bs, k, v, slots)
+    q = -(torch.rand((rows, 1, dim), generator=gen, device="cuda") + 1.0).to(dt)
+    scale = 2.0 ** 98
+    out, lse = torch.empty_like(q), torch.zeros((rows, 1), device="cuda")
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    d = B.kv4_attention_desc(cache=P.bind(B, cache, bs), dtype=KINDS[dtype], requests=1, tokens=rows, q_heads=1, q=q, out=out,
+                             block_table=torch.arange(blocks, device="cuda", dtype=torch.int32)[None], max_blocks=blocks, total_lens=i32([length]),
+                             query_start=i32([0, rows]), max_query=rows, scale=scale, causal=False, lse=lse)
+    ws = B.kv4_attention_workspace(torch, d)
+    B.kv4_attention(d)
+    (keys, _), (values, _) = P.read(torch, cache, bs, slots.long())
+    want = values[0].expand(rows, dim)
+    score = (q[:, 0].double() @ keys[0, 0]) * scale
+    assert (score < -1e31).all()
+    limit = 5 * (2 * 2.0 ** -12 + 2.0 ** -20 + 2.0 ** -23 * (length / 16 + 8)) + half_step(torch, dt) * want.abs()
+    assert not out.isnan().any() and ((out[:, 0].double() - want).abs() <= limit).all()
+    assert ((lse[:, 0].double() - score).abs() <= 15 * 2.0 ** -23 * (dim / 16 + 8) * score.abs() + 2.0 ** -12 * (rows > 128) * score.abs()).all()
+    assert ws is not None and B.device_status() == 0
