@@ -51,17 +51,13 @@ __device__ __forceinline__ Request LoadRequest(const AttentionParams& p, int b) 
         r.first_row = p.query_start[b];
         end = p.query_start[b + 1];
     }
+    const int limit = static_cast<int>(p.tokens);
+    if (r.first_row < 0 || r.first_row >= limit) r.first_row = end = 0;
     // rows are the request's last tokens: those beyond max_query or behind `tokens` are not computed, the others keep their positions
-    const int64_t given = static_cast<int64_t>(end) - r.first_row, room_for = p.tokens - r.first_row;
-    int n = 0;
-    r.total = p.total_lens[b];
-    if (r.first_row < 0 || room_for <= 0) {
-        r.first_row = 0;
-    } else if (given > 0) {
-        n = static_cast<int>(given < room_for ? given : room_for);
-        if (n > p.max_query) n = p.max_query;
-        r.total -= static_cast<int>(given - n);
-    }
+    const int given = end > r.first_row ? end - r.first_row : 0;
+    int n = given > p.max_query ? p.max_query : given;
+    if (n > limit - r.first_row) n = limit - r.first_row;
+    r.total = p.total_lens[b] - (given - n);
     r.queries = n;
     r.rows = n * p.group;
     const int64_t room = static_cast<int64_t>(p.max_blocks) << p.cache.block_shift;

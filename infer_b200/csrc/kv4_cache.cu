@@ -41,7 +41,6 @@ struct AppendParams {
     int* status;
     int block_tokens;  // tokens of one block of threads (with rope)
     int vec_k, vec_v, vec_q;
-    int turn;
     int two;           // 1: two tokens at a time
     Rope rope;
 };
@@ -243,7 +242,7 @@ __device__ __forceinline__ bool SharePairs(int slot0, int slot1) { return slot0 
 
 // A group of lanes takes two neighbouring tokens' vectors at a time: twice the loads in flight, and the words of values, which
 // hold two tokens, are written whole when the tokens are neighbours in the cache too.
-template <int DTYPE, int LANES>
+template <int DTYPE, int LANES, bool TURN>
 __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t first, int tokens, int start, int stride, const float2* angles) {
     const int lane = (threadIdx.x & 31) % LANES;
     const int heads = p.cache.kv_heads;
@@ -256,7 +255,7 @@ __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t fir
         const int64_t token = first + row;
         const int slots[2] = {has0 ? p.slots[token] : -1, has1 ? p.slots[token + 1] : -1};
         // a negative position: the row is not turned, its key is stored as it is
-        const bool turned[2] = {is_key && p.turn && has0 && p.rope.positions[token] >= 0, is_key && p.turn && has1 && p.rope.positions[token + 1] >= 0};
+        const bool turned[2] = {TURN && is_key && has0 && p.rope.positions[token] >= 0, TURN && is_key && has1 && p.rope.positions[token + 1] >= 0};
         Eight<DTYPE> x[2] = {};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -303,7 +302,7 @@ __device__ __forceinline__ void AppendVectors(const AppendParams& p, int64_t fir
 template <int DTYPE, int LANES>
 __global__ void __launch_bounds__(kThreads, kAppendBlocks) AppendKernel(const __grid_constant__ AppendParams p) {
     WaitForPrevious();
-    AppendVectors<DTYPE, LANES>(p, 0, static_cast<int>(p.tokens), blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads, nullptr);
+    AppendVectors<DTYPE, LANES, false>(p, 0, static_cast<int>(p.tokens), blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads, nullptr);
 }
 
 // With rope: a block of threads takes a few tokens (blockIdx.x) and a share of their vectors (blockIdx.y).
@@ -321,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) RopeAppendKernel(const __grid_consta
     }
     __syncthreads();
     const int start = blockIdx.y * kThreads + threadIdx.x, stride = gridDim.y * kThreads;
-    AppendVectors<DTYPE, LANES>(p, first, mine, start, stride, angles);
+    AppendVectors<DTYPE, LANES, true>(p, first, mine, start, stride, angles);
     // q: both members of a pair are read before either is written (the rows may be turned in place)
     const int half = pairs;
     const int items = p.vec_q ? r.head_dim >> 4 : r.head_dim - pairs;
@@ -512,7 +511,6 @@ extern "C" int fth_b200_kv4_append(const fth_b200_kv4_append_desc* d, fth_b200_s
         if (status == FTH_B200_OK) NoteLaunch("kv4_append");
         return status;
     }
-    p.turn = 1;
     p.rope = kv4::MakeRope(*d->rope);
     p.rope.k_out = nullptr;
     const bool whole = p.rope.rotary_dim % 16 == 0;
