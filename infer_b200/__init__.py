@@ -388,24 +388,33 @@ def _dense(**tensors):
 
 
 _SIZES = {FP32: 4, FP16: 2, BF16: 2}
+_NAMES = {FP32: "torch.float32", FP16: "torch.float16", BF16: "torch.bfloat16"}
 
 
 def _rows(name, t, dtype, tokens, heads, head_dim, ld):
-    """Row stride of [tokens, heads, head_dim] (or [tokens, heads * head_dim])."""
+    """Row stride of [tokens, heads, head_dim] (or [tokens, heads * head_dim], or elements in a row); the rows lie inside the tensor.
+    Bits held in integers may be of any type."""
     if t is None or not hasattr(t, "stride"):
         return ld
     if t.element_size() != _SIZES.get(dtype, t.element_size()):
         raise ValueError(f"{name} has {t.element_size()}-byte elements")
+    if t.is_floating_point() and str(t.dtype) != _NAMES.get(dtype, str(t.dtype)):
+        raise ValueError(f"{name} is {t.dtype}, not {_NAMES[dtype]}")
+    row = heads * head_dim
     if ld == 0 and t.dim() >= 2:
         inner = t.stride(-1) == 1 or t.shape[-1] == 1
         if t.dim() == 3:
-            inner = inner and (t.stride(1) == head_dim or t.shape[1] == 1) and t.shape[1] * t.shape[2] == heads * head_dim
+            inner = inner and (t.stride(1) == head_dim or t.shape[1] == 1) and t.shape[1] * t.shape[2] == row
         else:
-            inner = inner and t.dim() == 2 and t.shape[1] == heads * head_dim
-        if not inner or t.shape[0] < tokens:
+            inner = inner and t.dim() == 2 and t.shape[1] == row
+        if not inner or t.shape[0] < tokens or (tokens > 1 and t.stride(0) == 0):
             raise ValueError(f"{name}: expected [{tokens}, {heads}, {head_dim}] with heads {head_dim} apart, got {tuple(t.shape)}, strides {t.stride()}")
         if t.shape[0] > 1:
-            return t.stride(0)
+            ld = t.stride(0)
+    span = 1 + sum((n - 1) * step for n, step in zip(t.shape, t.stride())) if t.numel() else 0
+    need = (tokens - 1) * (ld or row) + row if tokens > 0 else 0
+    if span < need:
+        raise ValueError(f"{name}: {tokens} rows of {row}, {ld or row} apart, take {need} elements, the tensor holds {span}")
     return ld
 
 
@@ -575,6 +584,8 @@ def kv4_attention_desc(*, cache, dtype, requests, tokens, q_heads, q, out, block
     _count("total_lens", total_lens, requests)
     _count("query_start", query_start, requests + 1)
     _count("lse", lse, tokens * q_heads)
+    if hasattr(workspace, "numel") and workspace.numel() * workspace.element_size() < workspace_bytes:
+        raise ValueError(f"workspace has {workspace.numel() * workspace.element_size()} bytes, not {workspace_bytes}")
     return _tensors(d, q=q, out=out, lse=lse, block_table=block_table, total_lens=total_lens, query_start=query_start, workspace=workspace)
 
 

@@ -14,3 +14,48 @@ def test_a_larger_step_never_needs_a_smaller_workspace(dim, q_heads, kv_heads):
     need = [B.lib().fth_b200_kv4_attention_workspace_bytes(C.byref(attention_desc(dict(head_dim=dim, kv_heads=kv_heads), q_heads=q_heads, max_query=n)))
             for n in range(1, 300)]
     assert need[0] > 0 and need == sorted(need)
+
+
+def test_builders_refuse_rows_that_a_tensor_does_not_hold():
+    """One-dimensional tensors, strides given by hand, rows that repeat (stride 0): the last row has to lie inside the tensor."""
+    bf16 = dict(dtype=torch.bfloat16)
+    x = torch.zeros((4, 4, 128), **bf16)
+    for bad in (torch.zeros(8, **bf16), torch.zeros(4 * 512 - 1, **bf16), torch.zeros((1, 128), **bf16).expand(16, 128).flatten()[:100]):
+        with pytest.raises(ValueError, match="elements"):
+            rope_desc(q=bad, q_out=x)
+    with pytest.raises(ValueError, match="elements"):
+        rope_desc(q=x, q_out=x, ldq=513)                     # three strides and a row are one element too many ...
+    with pytest.raises(ValueError, match="not on a GPU"):
+        rope_desc(q=torch.zeros(3 * 513 + 512, **bf16), q_out=x, ldq=513)   # ... and these hold them
+    for name in ("q", "q_out", "k", "k_out"):
+        with pytest.raises(ValueError, match=f"{name}: .*elements"):
+            rope_desc(**{name: torch.zeros(8, **bf16), "ld" + name: 512})
+    for name in ("k", "v"):
+        with pytest.raises(ValueError, match=f"{name}: .*elements"):
+            append_desc(**{name: torch.zeros(8, **bf16), "ld" + name: 256})
+    for name in ("k", "v"):
+        with pytest.raises(ValueError, match=f"{name}_out: .*elements"):
+            gather_desc(**{name + "_out": torch.zeros(8, **bf16), "ld" + name: 256})
+    for name, ld in (("q", "ldq"), ("out", "ldo")):
+        with pytest.raises(ValueError, match=f"{name}: .*elements"):
+            attention_desc(**{name: torch.zeros(8, **bf16), ld: 1024})
+    with pytest.raises(ValueError, match="heads 128 apart"):
+        rope_desc(q=torch.zeros((1, 4, 128), **bf16).expand(4, 4, 128), q_out=x)
+
+
+def test_builders_tell_fp16_from_bf16():
+    """Bits in integers are anybody's; numbers have to be of the type that the descriptor names."""
+    half, bits = torch.zeros((4, 4, 128), dtype=torch.float16), torch.zeros((4, 4, 128), dtype=torch.int16)
+    with pytest.raises(ValueError, match="float16"):
+        rope_desc(q=half, q_out=bits)
+    with pytest.raises(ValueError, match="bfloat16"):
+        rope_desc(dtype=B.FP16, q=half.bfloat16(), q_out=bits)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        rope_desc(dtype=B.FP16, q=half, q_out=bits)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        rope_desc(q=bits, q_out=bits)
+
+
+def test_a_workspace_tensor_is_as_large_as_it_is_said_to_be():
+    with pytest.raises(ValueError, match="workspace has"):
+        attention_desc(workspace=torch.zeros(100, dtype=torch.uint8), workspace_bytes=101)
