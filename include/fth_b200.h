@@ -401,7 +401,7 @@ int fth_b200_silu_mul(int32_t dtype, const void* gate, const void* up, void* out
  * the tables that address it, and the attention that reads it.  No counterpart in the reference's FP8 / INT8 path.  All
  * are launched as programmatic dependents of the kernel in front; none allocates, synchronises or reads back, and every
  * length that changes from step to step is read on the device, so a captured step can be replayed with other lengths.
- * All pointers are device pointers unless a comment says "host".  Strides count elements.
+ * All pointers are device pointers unless a comment says "host", each aligned to its element.  Strides count elements.
  *
  * Rotary positions.  Pair i of a head (elements i and i + rotary_dim / 2, or 2i and 2i + 1) is turned by
  * positions[t] * turns[i] full turns:

@@ -38,6 +38,9 @@ __device__ __forceinline__ void WaitForPrevious() {
 }
 
 inline bool AlignedTo(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// Arrays of 32-bit numbers; null is aligned.
+template <typename... Pointers>
+bool WordAligned(Pointers... p) { return (AlignedTo(p, 4) && ...); }
 inline int ElementBytes(int dtype) { return dtype == FTH_B200_FP32 ? 4 : 2; }
 inline bool FloatType(int dtype) { return dtype == FTH_B200_FP32 || dtype == FTH_B200_BF16 || dtype == FTH_B200_FP16; }
 inline int Log2(int v) { int s = 0; while ((1 << s) < v) ++s; return s; }

@@ -720,7 +720,7 @@ int CheckAttention(const fth_b200_kv4_attention_desc* d) {
     const int64_t row = static_cast<int64_t>(d->q_heads) * d->cache.head_dim;
     if ((d->ldq != 0 && d->ldq < row) || (d->ldo != 0 && d->ldo < row)) return FTH_B200_ERR_INVALID;
     if (d->dtype != FTH_B200_BF16 && d->dtype != FTH_B200_FP16) return FTH_B200_ERR_UNSUPPORTED;
-    if (!AlignedTo(d->q, 2) || !AlignedTo(d->out, 2) || !AlignedTo(d->lse, 4)) return FTH_B200_ERR_INVALID;
+    if (!AlignedTo(d->q, 2) || !AlignedTo(d->out, 2) || !WordAligned(d->lse, d->block_table, d->total_lens, d->query_start)) return FTH_B200_ERR_INVALID;
     if (d->tokens > 0x7fffffff || d->q_heads > 65536 || static_cast<int64_t>(d->max_query) * (d->q_heads / d->cache.kv_heads) > 0x7fffffff)
         return FTH_B200_ERR_UNSUPPORTED;
     if (static_cast<int64_t>(d->max_blocks) * d->cache.block_size > 0x7fffffff) return FTH_B200_ERR_UNSUPPORTED;

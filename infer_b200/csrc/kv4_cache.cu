@@ -479,7 +479,7 @@ extern "C" int fth_b200_kv4_append(const fth_b200_kv4_append_desc* d, fth_b200_s
     if (d->tokens > 0x7fffffff) return FTH_B200_ERR_UNSUPPORTED;
     if (d->tokens > 0 && (d->k == nullptr || d->v == nullptr || d->slots == nullptr)) return FTH_B200_ERR_INVALID;
     const int size = kv4::ElementBytes(d->dtype);
-    if (!kv4::AlignedTo(d->k, size) || !kv4::AlignedTo(d->v, size)) return FTH_B200_ERR_INVALID;
+    if (!kv4::AlignedTo(d->k, size) || !kv4::AlignedTo(d->v, size) || !kv4::WordAligned(d->slots)) return FTH_B200_ERR_INVALID;
     if (d->rope != nullptr) {
         rc = kv4::CheckRope(d->rope, true);
         if (rc != FTH_B200_OK) return rc;
@@ -541,7 +541,7 @@ extern "C" int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* d, fth_b200_s
     if (d->tokens > 0x7fffffff) return FTH_B200_ERR_UNSUPPORTED;
     if (d->k_out == nullptr && d->v_out == nullptr) return FTH_B200_ERR_INVALID;
     const int size = kv4::ElementBytes(d->dtype);
-    if (!kv4::AlignedTo(d->k_out, size) || !kv4::AlignedTo(d->v_out, size)) return FTH_B200_ERR_INVALID;
+    if (!kv4::AlignedTo(d->k_out, size) || !kv4::AlignedTo(d->v_out, size) || !kv4::WordAligned(d->slots)) return FTH_B200_ERR_INVALID;
     if (d->tokens == 0) return FTH_B200_OK;
     if (d->slots == nullptr) return FTH_B200_ERR_INVALID;
     const int per16 = 16 / size;

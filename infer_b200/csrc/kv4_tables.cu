@@ -311,6 +311,7 @@ int CheckTables(const Desc* d) {
     if (d->requests <= 0 || d->max_blocks <= 0) return FTH_B200_ERR_INVALID;
     if (d->free_blocks == nullptr || d->free_count == nullptr || d->free_count_out == nullptr || d->block_table == nullptr || d->status == nullptr)
         return FTH_B200_ERR_INVALID;
+    if (!WordAligned(d->free_blocks, d->free_count, d->free_count_out, d->block_table, d->status)) return FTH_B200_ERR_INVALID;
     const int rc = CheckPool(d->blocks, d->block_size);
     if (rc != FTH_B200_OK) return rc;
     // positions are 31 bits
@@ -339,6 +340,7 @@ extern "C" int fth_b200_kv4_assign(const fth_b200_kv4_assign_desc* d, fth_b200_s
     if (d == nullptr || d->tokens < 0 || d->cached_lens == nullptr || d->new_lens == nullptr || d->total_lens == nullptr || d->query_start == nullptr)
         return FTH_B200_ERR_INVALID;
     if (d->tokens > 0 && (d->slots == nullptr || d->positions == nullptr)) return FTH_B200_ERR_INVALID;
+    if (!kv4::WordAligned(d->cached_lens, d->new_lens, d->total_lens, d->query_start, d->slots, d->positions)) return FTH_B200_ERR_INVALID;
     const int rc = kv4::CheckTables(d);
     if (rc != FTH_B200_OK) return rc;
     if (d->tokens > 0x7fffffff) return FTH_B200_ERR_UNSUPPORTED;
@@ -355,6 +357,7 @@ extern "C" int fth_b200_kv4_assign(const fth_b200_kv4_assign_desc* d, fth_b200_s
 extern "C" int fth_b200_kv4_release(const fth_b200_kv4_release_desc* d, fth_b200_stream_t stream) {
     ClearStaleError();
     if (d == nullptr || d->lens == nullptr || d->keep_lens == nullptr || d->lens_out == nullptr) return FTH_B200_ERR_INVALID;
+    if (!kv4::WordAligned(d->lens, d->keep_lens, d->lens_out)) return FTH_B200_ERR_INVALID;
     const int rc = kv4::CheckTables(d);
     if (rc != FTH_B200_OK) return rc;
     const kv4::ReleaseParams p{d->requests, d->max_blocks, kv4::Log2(d->block_size), static_cast<int>(d->blocks), d->lens, d->keep_lens,

@@ -126,6 +126,7 @@ int CheckRope(const fth_b200_rope_desc* d, bool keys_stay) {
     if (d->layout != FTH_B200_ROPE_HALF && d->layout != FTH_B200_ROPE_INTERLEAVED) return FTH_B200_ERR_INVALID;
     if (d->rotary_dim % 2 != 0 || d->rotary_dim > d->head_dim) return FTH_B200_ERR_INVALID;
     if (d->positions == nullptr || d->turns == nullptr || !std::isfinite(d->amplitude)) return FTH_B200_ERR_INVALID;
+    if (!WordAligned(d->positions) || !AlignedTo(d->turns, alignof(double))) return FTH_B200_ERR_INVALID;
     if (d->q_heads > 0 && (d->q == nullptr || d->q_out == nullptr)) return FTH_B200_ERR_INVALID;
     if (d->k_heads > 0 && (d->k == nullptr || (d->k_out == nullptr) != keys_stay)) return FTH_B200_ERR_INVALID;
     const int64_t q_row = static_cast<int64_t>(d->q_heads) * d->head_dim, k_row = static_cast<int64_t>(d->k_heads) * d->head_dim;

@@ -59,3 +59,21 @@ def test_builders_tell_fp16_from_bf16():
 def test_a_workspace_tensor_is_as_large_as_it_is_said_to_be():
     with pytest.raises(ValueError, match="workspace has"):
         attention_desc(workspace=torch.zeros(100, dtype=torch.uint8), workspace_bytes=101)
+
+
+@pytest.mark.parametrize("off", [1, 2])
+def test_addresses_of_numbers_are_aligned(off):
+    """A word read from an odd address would end the context."""
+    for name in ("positions", "turns"):
+        refused("fth_b200_rope", rope_desc(**{name: A + off}), B.ERR_INVALID)
+    refused("fth_b200_rope", rope_desc(turns=A + 4), B.ERR_INVALID)
+    refused("fth_b200_kv4_append", append_desc(rope=rope_desc(k_out=None, positions=A + off)), B.ERR_INVALID)
+    refused("fth_b200_kv4_append", append_desc(slots=A + off), B.ERR_INVALID)
+    refused("fth_b200_kv4_gather", gather_desc(slots=A + off), B.ERR_INVALID)
+    for name in ("block_table", "total_lens", "query_start"):
+        refused("fth_b200_kv4_attention", attention_desc(**{name: A + off}), B.ERR_INVALID)
+    for name in ("cached_lens", "new_lens", "free_blocks", "free_count", "free_count_out", "block_table", "total_lens", "query_start", "slots", "positions",
+                 "status"):
+        refused("fth_b200_kv4_assign", B.kv4_assign_desc(**{**ASSIGN, name: A + off}), B.ERR_INVALID)
+    for name in ("lens", "keep_lens", "free_blocks", "free_count", "free_count_out", "block_table", "lens_out", "status"):
+        refused("fth_b200_kv4_release", B.kv4_release_desc(**{**RELEASE, name: A + off}), B.ERR_INVALID)
