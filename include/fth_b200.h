@@ -569,7 +569,7 @@ int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* desc, fth_b200_stream_t 
  * exactly, down to 2^-28 of their largest finite element (|q| < 2^100, |v| < 2^100).
  * A NaN in q makes its own row NaN, a NaN in a key or value (or in its scale or minimum) the rows that see the token.
  * A block number outside the cache hides its tokens and is reported through fth_b200_device_status (site 42).
- * max_query bounds the rows of a request (host-known), max_blocks * block_size the tokens.  A request's rows beyond max_query, and rows
+ * max_query bounds the rows of a request (host-known), max_blocks * block_size (up to 2^31 - 512) the tokens.  A request's rows beyond max_query, and rows
  * from `tokens` on, are not computed; its other rows keep their positions.
  * The result does not depend on what else is in the batch only up to FP32 summation order; it is the same from run to run.
  * workspace: device, 256-byte aligned, zero-filled once after allocation, left ready for the next call; calls that share

@@ -723,7 +723,8 @@ int CheckAttention(const fth_b200_kv4_attention_desc* d) {
     if (!AlignedTo(d->q, 2) || !AlignedTo(d->out, 2) || !WordAligned(d->lse, d->block_table, d->total_lens, d->query_start)) return FTH_B200_ERR_INVALID;
     if (d->tokens > 0x7fffffff || d->q_heads > 65536 || static_cast<int64_t>(d->max_query) * (d->q_heads / d->cache.kv_heads) > 0x7fffffff)
         return FTH_B200_ERR_UNSUPPORTED;
-    if (static_cast<int64_t>(d->max_blocks) * d->cache.block_size > 0x7fffffff) return FTH_B200_ERR_UNSUPPORTED;
+    // places of tokens are 31 bits, also one tile (of up to 256) behind the last
+    if (static_cast<int64_t>(d->max_blocks) * d->cache.block_size > 0x7fffffff - 511) return FTH_B200_ERR_UNSUPPORTED;
     return FTH_B200_OK;
 }
 

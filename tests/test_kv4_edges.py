@@ -77,3 +77,11 @@ def test_addresses_of_numbers_are_aligned(off):
         refused("fth_b200_kv4_assign", B.kv4_assign_desc(**{**ASSIGN, name: A + off}), B.ERR_INVALID)
     for name in ("lens", "keep_lens", "free_blocks", "free_count", "free_count_out", "block_table", "lens_out", "status"):
         refused("fth_b200_kv4_release", B.kv4_release_desc(**{**RELEASE, name: A + off}), B.ERR_INVALID)
+
+
+@pytest.mark.parametrize("block_size,max_blocks", [(16, (1 << 27) - 1), (256, (1 << 23) - 1), (16, (1 << 27) - 31)])
+def test_attention_refuses_tables_whose_last_tile_passes_31_bits(block_size, max_blocks):
+    d = attention_desc(dict(block_size=block_size), max_blocks=max_blocks)
+    assert B.lib().fth_b200_kv4_attention_supported(C.byref(d)) == B.ERR_UNSUPPORTED
+    d = attention_desc(dict(block_size=block_size), max_blocks=((1 << 31) - 512) // block_size)
+    assert B.lib().fth_b200_kv4_attention_supported(C.byref(d)) == B.OK
