@@ -212,6 +212,13 @@ __device__ __forceinline__ bool WaitFor(uint64_t* bar, uint32_t parity, int* sta
     }
     return true;
 }
+// Sixteen bytes of codes, not kept in L1.  Not by the read-only path: the kernel in front may still store the step's tokens when
+// this one has started (it waits for it before the first of these loads).
+__device__ __forceinline__ uint4 LoadCodes(const uint8_t* from) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from) : "memory");
+    return v;
+}
 // Whether some row sees one of the sixteen tokens around `token`.
 __device__ __forceinline__ bool SomeSeen(const Place& u, int token) { return (token & ~15) < u.high && (token & ~15) + 16 > u.low; }
 // What the table names as the block of `token` if any of its sixteen neighbours is seen by a row, else -1.
@@ -709,7 +716,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                 for (int j = 0; j < kPieces; ++j) {
                     const int64_t from = place_of[tile % P][token_of(j) >> 4];
                     keys[j] = make_uint4(0, 0, 0, 0);
-                    if (from >= 0) keys[j] = LoadStream16(p.cache.k_codes + from + (token_of(j) & 15) * (D / 2) + piece_of(j) * 16);
+                    if (from >= 0) keys[j] = LoadCodes(p.cache.k_codes + from + (token_of(j) & 15) * (D / 2) + piece_of(j) * 16);
                 }
             };
             const auto load_values = [&](uint32_t tile) {
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1) PrefillKernel(const __g
                     for (int j = 0; j < 4; ++j) {
                         const uint8_t* row = codes + j * D + 8 * t * (kWords * 4);
                         if constexpr (kWords == 4) {
-                            const uint4 x = from >= 0 ? LoadStream16(row) : make_uint4(0, 0, 0, 0);
+                            const uint4 x = from >= 0 ? LoadCodes(row) : make_uint4(0, 0, 0, 0);
                             values[t][j][0] = x.x;
                             values[t][j][1] = x.y;
                             values[t][j][2] = x.z;

@@ -210,3 +210,51 @@ def test_rows_whose_scores_are_far_below_zero(cuda, dtype, dim, rows, length):
     assert not out.isnan().any() and ((out[:, 0].double() - want).abs() <= limit).all()
     assert ((lse[:, 0].double() - score).abs() <= 15 * 2.0 ** -23 * (dim / 16 + 8) * score.abs() + 2.0 ** -12 * (rows > 128) * score.abs()).all()
     assert ws is not None and B.device_status() == 0
+
+
+# ---- one launch behind another ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_reads_what_the_launch_in_front_stored(cuda, rows, dim):
+    """The same slots stored anew and read at once, many times over, eagerly and in a graph: each reading is that of its own storing, to
+    the bit.  Every launch may start before the one in front has ended."""
+    torch = cuda
+    length, bs, hk, times = 1000, 16, 2, 12
+    blocks = P.blocks(length, bs)
+    cache = B.kv4_new_cache(torch, blocks=blocks, block_size=bs, kv_heads=hk, head_dim=dim)
+    gen = torch.Generator(device="cuda").manual_seed(rows + dim)
+    kv = torch.randn((2, times, length, hk, dim), generator=gen, device="cuda").to(torch.bfloat16)
+    q = torch.randn((rows, 2 * hk, dim), generator=gen, device="cuda").to(torch.bfloat16)
+    outs = torch.zeros((times, rows, 2 * hk, dim), dtype=torch.bfloat16, device="cuda")
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    slots = torch.arange(length, dtype=torch.int32, device="cuda")
+    stores = [B.kv4_append_desc(cache=cache, dtype=B.BF16, tokens=length, k=kv[0, i], v=kv[1, i], slots=slots) for i in range(times)]
+    reads = [B.kv4_attention_desc(cache=cache, dtype=B.BF16, requests=1, tokens=rows, q_heads=2 * hk, q=q, out=outs[i],
+                                  block_table=torch.arange(blocks, dtype=torch.int32, device="cuda")[None], max_blocks=blocks, total_lens=i32([length]),
+                                  query_start=i32([0, rows]), max_query=rows, scale=dim ** -0.5) for i in range(times)]
+    ws = B.kv4_attention_workspace(torch, reads[0])
+    for r in reads[1:]:
+        r.workspace, r.workspace_bytes = ws.data_ptr(), ws.numel()
+    for s, r in zip(stores, reads):
+        B.kv4_append(s)
+        torch.cuda.synchronize()
+        B.kv4_attention(r)
+        torch.cuda.synchronize()
+    want = outs.clone()
+    assert not (want[0] == want[1]).all()
+
+    def run():
+        for s, r in zip(stores, reads):
+            B.kv4_append(s)
+            B.kv4_attention(r)
+    outs.zero_()
+    run()
+    same(outs, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        outs.zero_()
+        graph.replay()
+        same(outs, want)
+    assert B.device_status() == 0
