@@ -566,12 +566,14 @@ int fth_b200_kv4_gather(const fth_b200_kv4_gather_desc* desc, fth_b200_stream_t 
  * largest scale among the values seen).  With more rows probabilities and values are rounded to FP16 one by one, and with BF16
  * rows the keys too (11 bits, down to 2^-28 of the largest among 128 tokens; values: among those before them as well).
  * q enters as FP16 times one power of two for the rows that are worked on together, which are of one request and kv head:
- * exactly, down to 2^-28 of their largest finite element (|q| < 2^100, |v| < 2^100).
+ * exactly, down to 2^-28 of their largest finite element with more than 128 BF16 rows; elsewhere odd elements are multiplied by a
+ * further 1/16, and FP16's 11 bits are kept down to 2^-24 of it, BF16's 8 down to 2^-27 (|q| < 2^100, |v| < 2^100, with more than 128 BF16
+ * rows |k| < 2^100).
  * A NaN in q makes its own row NaN, a NaN in a key or value (or in its scale or minimum) the rows that see the token.
  * A block number outside the cache hides its tokens and is reported through fth_b200_device_status (site 42).
  * max_query bounds the rows of a request (host-known), max_blocks * block_size (up to 2^31 - 512) the tokens.  A request's rows beyond max_query, and rows
  * from `tokens` on, are not computed; its other rows keep their positions.
- * The result does not depend on what else is in the batch only up to FP32 summation order; it is the same from run to run.
+ * What else is in the batch changes a result by the order of FP32 sums only; it is the same from run to run.
  * workspace: device, 256-byte aligned, zero-filled once after allocation, left ready for the next call; calls that share
  * one must not overlap.  fth_b200_kv4_attention_workspace_bytes depends on requests, tokens, max_query, heads and the
  * cache's geometry only, and not less for a larger max_query: the largest step's workspace serves the smaller ones. */

@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm<D, NT>) DecodeKernel(co
                 all_low = l > all_low ? l : all_low;
                 all_high = h < all_high ? h : all_high;
             }
-            // one power of two for all rows: what lies 2^28 below the largest element of the largest row keeps FP16's 11 bits
+            // one power of two for all rows, the largest element to 2^14: odd elements, with their 1/16, keep FP16's 11 bits down to 2^-24
+            // of it (its normal numbers end at 2^-14) and BF16's 8 down to 2^-27, even ones 16 times farther
             const int e = QueryExponent(big);
             back = p.scale_log2 * PowerOfTwo(24 - e);
             const float up = PowerOfTwo(e);

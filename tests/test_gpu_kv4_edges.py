@@ -258,3 +258,48 @@ def test_attention_reads_what_the_launch_in_front_stored(cuda, rows, dim):
         graph.replay()
         same(outs, want)
     assert B.device_status() == 0
+
+
+# ---- small elements beside large ones -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,rows,exponent", [("fp16", 1, 24), ("fp16", 12, 24), ("fp16", 200, 24), ("bf16", 1, 27), ("bf16", 12, 27), ("bf16", 200, 28)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_small_query_elements_keep_their_bits(cuda, dtype, rows, exponent, dim):
+    """One element of a query is 2^exponent times the others; it meets a key element of zero, so only the others make scores.  Keys are
+    whole numbers from 0 to 15 (scale 1, minimum 0, exact).  A score is off by the FP32 sum of its products, 2^-23 * (dim / 16 + 8) of
+    their sizes' sum A; weights by that, 2^-12 and 2^-20; each moves the result by at most twice that of the largest |v - out|, sums
+    by 2^-23 * (tokens / 16 + 8) of |v| + 15 s <= 4 |v|, values of many rows by 2^-12 |v|.  A is some hundreds: a query
+    element that lost four of its bits would show."""
+    torch = cuda
+    dt, bs, length = dtype_of(torch, dtype), 16, 300
+    gen = torch.Generator(device="cuda").manual_seed(dim + rows)
+    blocks = P.blocks(length, bs)
+    cache = P.new_cache(torch, blocks, 1, bs, dim, seed=1)
+    k = torch.randint(0, 16, (length, 1, dim), generator=gen, device="cuda").to(dt)
+    k[:, 0, 0], k[:, 0, 1] = 0.0, 15.0
+    v = torch.randn((length, 1, dim), generator=gen, device="cuda").to(dt)
+    slots = torch.arange(length, dtype=torch.int32, device="cuda")
+    P.append(torch, cache, bs, k, v, slots)
+    bits = 1024 if dtype == "fp16" else 128
+    small = (1 + torch.randint(0, bits, (rows, 1, dim), generator=gen, device="cuda") / bits) * (torch.randint(0, 2, (rows, 1, dim), generator=gen, device="cuda") * 2 - 1)
+    q = (small * 2.0 ** -12).to(dt)
+    assert torch.equal(q.double(), small.double() * 2.0 ** -12)
+    q[:, 0, 0] = 2.0 ** (exponent - 12)
+    scale = 2.0 ** 12 * 0.125
+    out = torch.empty_like(q)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    d = B.kv4_attention_desc(cache=P.bind(B, cache, bs), dtype=KINDS[dtype], requests=1, tokens=rows, q_heads=1, q=q, out=out,
+                             block_table=torch.arange(blocks, dtype=torch.int32, device="cuda")[None], max_blocks=blocks, total_lens=i32([length]),
+                             query_start=i32([0, rows]), max_query=rows, scale=scale, causal=False)
+    ws = B.kv4_attention_workspace(torch, d)
+    B.kv4_attention(d)
+    (keys, _), (values, _) = P.read(torch, cache, bs, slots.long())
+    assert torch.equal(keys, k.double())
+    keys, values = keys[:, 0], values[:, 0]
+    want = torch.softmax(q[:, 0].double() @ keys.T * scale, dim=-1) @ values
+    size = float((q[:, 0, 1:].double().abs() @ keys[:, 1:].T).max()) * scale
+    assert 100 < size < 8000
+    error = 2.0 ** -23 * (dim / 16 + 8) * size + 2.0 ** -12 + 2.0 ** -20
+    spread = values.abs().max() + want.abs().amax(-1, keepdim=True)
+    limit = 2 * error * spread + (2.0 ** -23 * (length / 16 + 8) * 4 + 2.0 ** -12 * (rows > 128)) * values.abs().max() + half_step(torch, dt) * want.abs() + 1e-7
+    assert ((out[:, 0].double() - want).abs() <= limit).all()
+    assert ws is not None and B.device_status() == 0
