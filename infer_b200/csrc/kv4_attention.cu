@@ -736,7 +736,8 @@ constexpr size_t kCounterBytes = kMaxGrid * sizeof(int);
 int64_t MostRows(const fth_b200_kv4_attention_desc& d) { return static_cast<int64_t>(d.max_query) * (d.q_heads / d.cache.kv_heads); }
 // Query rows of a unit, in eights.  Sixteen share what unpacking costs (12 requests of 3500 .. 9000 tokens, 2 kv heads of 128, 32 rows:
 // 27.5 us, 32.4 us in eights), unless half of the last ones would be missing (32 requests, 8 kv heads, 20 rows: 123 us, 113 us in eights); 256-wide
-// heads leave no registers for them (20 rows: 69 us, 42 us in eights).
+// heads leave no registers for them (20 rows: 69 us, 42 us in eights).  With 9 to 16 rows, one unit of sixteen, two of eight would be as
+// fast or faster: 12 rows of those 12 requests 29 us, 23 us in eights; one request of 8000 tokens, 8 heads of 128, 23 and 20 us.
 int DecodeTiles(const fth_b200_kv4_attention_desc& d) { return d.cache.head_dim != 256 && (MostRows(d) + 7) / 8 % 2 == 0 ? 2 : 1; }
 // Blocks of threads that are resident together.
 int DecodeGrid(int head_dim, int tiles) {
@@ -745,9 +746,12 @@ int DecodeGrid(int head_dim, int tiles) {
     return grid < kMaxGrid ? grid : kMaxGrid;
 }
 
-// The kernel with 128-row tiles.  It unpacks as much for a row as for 256, and its tiles start late: those 12 requests of 2 kv heads of 128
-// take it 56, 83 and 124 us with 20, 64 and 128 rows, eights and sixteens 27, 44 and 73 us; 256-wide heads 76, 108 and 154 us against
-// 42, 80 and 142 us.
+// The kernel with 128-row tiles.  It unpacks as much for a row as for 256, and its tiles start late.  Where the two cross depends on the
+// lengths, which the host does not know: heads of 128 take the kernel for few rows (let on to more) and that for many
+//   12 requests of 3500 .. 9000 tokens, 2 kv heads    132 rows  97 and 136 us   256 rows 135 and 146 us   384 rows 195 and 125 us
+//   one request of 8000 tokens, 8 kv heads            132 rows  57 and 181 us   384 rows  99 and 121 us   768 rows 180 and 135 us
+//   40 requests of 1000 tokens, 4 kv heads            128 rows 106 us           132 rows 129 and  84 us   256 rows 195 and  91 us
+// 64-wide heads cross at the same places, 256-wide ones at 132, 256 and below 128 rows.  128 costs the long requests and spares the short.
 bool ManyRows(const fth_b200_kv4_attention_desc& d) { return MostRows(d) > 128; }
 
 // What a call with these or fewer rows needs, so that the largest step's workspace serves all: units of sixteen rows, in fewer blocks of

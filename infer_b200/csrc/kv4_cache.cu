@@ -7,10 +7,12 @@
 // itself.  Every border is decided exactly: an FP32 estimate of (x - m) / s is off by less than 2^-21 * 15 < 10^-5, so
 // eight elements are looked at again, in 64 bits, only if one's estimate is within 10^-4 of a half.
 // One pass over the data: 2 * tokens * kv_heads * head_dim * size bytes in, head_dim + 8 bytes per token and head out;
-// a launch for single tokens; for prompts reading back is bound by memory (16384 tokens of 8 heads of 128 in BF16: 23 us,
-// 3.6 TB/s) and storing by its arithmetic, some 350 instructions for four vectors (36 us, 2.4 TB/s).  A vector belongs to
-// head_dim / 8 neighbouring lanes, eight elements each, so minimum and maximum are three to five shuffles (both in one word for
-// 16-bit types) and a lane's codes are one 32-bit word.
+// a launch for single tokens.  Prompts, 16384 tokens of 8 heads of 128 in BF16: storing takes 36 us, 2.4 TB/s, 104 warp instructions a
+// vector in 72 % of the issue slots.  Reading back takes 23 us, 3.6 TB/s, half of what memory gives: 62 % of the issue
+// slots, and warps that wait for a lane's four bytes of codes, whose address stands behind a load of the slot.  With rope and 32 query
+// heads 200 us (64 tokens: 5.0 us), more than fth_b200_rope and storing apart (69 + 36 us): 96 registers leave two blocks of threads
+// on an SM and 41 % of the issue slots used.  A vector belongs to head_dim / 8 neighbouring lanes, eight elements each, so minimum
+// and maximum are three to five shuffles (both in one word for 16-bit types) and a lane's codes are one 32-bit word.
 #include <type_traits>
 
 #include "kv4.cuh"

@@ -31,8 +31,9 @@
 //
 // Bound: 4 * rows * tokens * head_dim operations on the matrix units; one exponential per score (16 a clock and SM) takes as
 // long as the products of 128-wide heads do.  Three prompts of up to 4000 rows over up to 8100 tokens, 32 heads of 128 on 8,
-// BF16: 1.01 ms, 0.72 PFLOP/s, 45 % of what a large product reaches.  Neither unit is full (34 % each): the softmax warps, two
-// to a scheduler, need four to five cycles an instruction, one result waiting for the last.
+// BF16: 1.02 ms, 0.71 PFLOP/s, 44 % of what a large product reaches (FP16: 1.27 ms; heads of 64: 0.87 and 1.15 ms, of 256: 3.15 and
+// 3.25 ms).  Neither unit is full (34 % each): the softmax warps, two to a scheduler, need four to five cycles an instruction, one
+// result waiting for the last.
 #include "kv4_attention.cuh"
 #include "kv4_prefill.h"
 #include "tcgen05.cuh"
